@@ -12,6 +12,7 @@ _lib = None
 c_i32p = ctypes.POINTER(ctypes.c_int32)
 c_i64p = ctypes.POINTER(ctypes.c_int64)
 vp = ctypes.c_void_p
+i64 = ctypes.c_int64
 
 # name -> (restype, argtypes); must list every symbol include/cgnet_b200.h declares
 SIGNATURES = {
@@ -48,6 +49,18 @@ SIGNATURES = {
     "cgb200_sh_project": (ctypes.c_int, [vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, vp, ctypes.c_float, vp, vp, ctypes.c_int64, vp, vp]),
     "cgb200_raycast_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64]),
     "cgb200_raycast_sphere": (ctypes.c_int, [vp, ctypes.c_int64, vp, ctypes.c_int64, vp, ctypes.c_int64, vp, vp, ctypes.c_int64, vp, vp]),
+    "cgb200_layer_norm_fwd": (ctypes.c_int, [vp, i64, vp, vp, ctypes.c_float, vp, vp, i64, i64, ctypes.c_int, ctypes.c_int, vp]),
+    "cgb200_layer_norm_bwd_workspace_bytes": (i64, [i64, i64, ctypes.c_int]),
+    "cgb200_layer_norm_bwd": (ctypes.c_int, [vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, ctypes.c_int, ctypes.c_int, vp, i64, vp]),
+    "cgb200_gated_ff_workspace_bytes": (i64, [i64, i64, i64, ctypes.c_int, ctypes.c_int]),
+    "cgb200_gated_ff_fwd": (ctypes.c_int, [vp, i64, vp, i64, vp, i64, ctypes.c_int, vp, vp, i64, i64, i64, ctypes.c_int, vp, i64, vp]),
+    "cgb200_gated_ff_bwd": (ctypes.c_int, [vp, i64, vp, i64, vp, i64, ctypes.c_int, vp, vp, i64, vp, vp, vp, i64, i64, i64, ctypes.c_int,
+                                           vp, i64, vp]),
+    "cgb200_log_probs_fwd": (ctypes.c_int, [vp, i64, vp, ctypes.c_int, vp, vp, vp, vp, vp, i64, i64, ctypes.c_int, vp]),
+    "cgb200_log_probs_bwd": (ctypes.c_int, [vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, ctypes.c_int, vp]),
+    "cgb200_distill_fwd": (ctypes.c_int, [vp, i64, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_float, vp, vp, i64, i64, ctypes.c_int, vp]),
+    "cgb200_distill_bwd": (ctypes.c_int, [vp, i64, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_float, vp, vp, vp, i64, i64, ctypes.c_int,
+                                          vp]),
     "cgb200_launch_count": (ctypes.c_int64, [ctypes.c_int]),
     "cgb200_kernel_count": (ctypes.c_int, []),
     "cgb200_kernel_name": (ctypes.c_char_p, [ctypes.c_int]),
@@ -59,6 +72,9 @@ Q_N_F, Q_N_FF, Q_N_O, Q_W_LEN, Q_SUM_TFF, Q_CG_LEN, Q_N_TRIPLES, Q_TILE = range(
 FN_PRESENT, FN_UPDATE, FN_KEEP_MID = 0x1, 0x2, 0x4
 PLAN_DEPTHWISE = 0x1
 AUTO = -1
+F32, BF16, F16 = range(3)
+ACT_SILU, ACT_GELU, ACT_RELU = range(3)
+MAX_TOP, MAX_TEACHER = 128, 1024
 (OPT_TC_FWD, OPT_TC_GRAD_W, OPT_TC_GRAD_F, OPT_TC_STAGES, OPT_FWD_SLAB, OPT_GRAD_F_SPLIT, OPT_STATS_SPLIT, OPT_BWD_SERIAL,
  OPT_WAIT_POLLS, OPT_TEST_IDLE_MMA, OPT_TC_STAGED, OPT_TC_ABUF, OPT_TC_FWD_SPLIT, OPT_GRAD_MID_GEMM,
  OPT_FWD_KEEP_MID, OPT_SHORT_GROUP) = range(16)

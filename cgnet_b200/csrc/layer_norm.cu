@@ -1,0 +1,533 @@
+// Layer norm over the last axis, forward and backward, with the gradients of weight and bias.
+//
+//   y  = (x - mean) * rstd * w + b,    rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   dx = rstd * (w dy - mean(w dy) - xh * mean(w dy * xh)),   xh = (x - mean) * rstd
+//   dw = sum over rows of dy * xh,     db = sum over rows of dy
+//
+// Everything is held in float32 between the loads and the one rounding of each result.  The variance is taken over centred
+// values that stay in registers (not as a difference of moments), so a large common offset of a row costs no digits.
+#include <algorithm>
+
+#include "row_ops.cuh"
+
+namespace cgb200 {
+
+constexpr int kLnMaxChunks = 4;        // chunks of a row a thread of the forward kernel holds in registers
+constexpr int kLnBwdValues = 16;       // values of a row a thread of the backward kernel holds
+constexpr int kLnBwdMaxThreads = 512;
+
+struct LnArgs {
+    const void* x;
+    int64_t x_stride;       // values between rows
+    const void* w;          // may be null: 1
+    const void* b;          // may be null: 0
+    float eps;
+    int64_t rows, dim;
+};
+
+// Sum over the threads that share a row: a warp, or the whole block.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float* buf) {
+    return WARP ? warp_sum(v) : block_sum(v, buf);
+}
+
+// One row per warp (WARP) or per block; its values stay in registers between the three steps, so x is read once.
+template <typename T, typename P, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, T* __restrict__ y, float2* __restrict__ stats) {
+    constexpr int N = Chunk<T>::N;
+    __shared__ float red[2][32];
+    const int G = WARP ? 32 : (int)blockDim.x;
+    const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
+    const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    if (row >= a.rows) return;               // whole warps or whole blocks leave
+    const T* xr = (const T*)a.x + row * a.x_stride;
+    T* yr = y + row * a.dim;
+    const int ph = row_phase(xr);
+    float v[CH][N];
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        load_chunk(xr, (int64_t)(t + c * G) * N - ph, a.dim, 0.f, v[c]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += v[c][i];
+    }
+    const float mean = row_sum<WARP>(s, red[0]) / (float)a.dim;
+    float q = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int64_t e0 = (int64_t)(t + c * G) * N - ph;
+        const bool full = e0 >= 0 && e0 + N <= a.dim;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[c][i] -= mean;
+            if (full || (e0 + i >= 0 && e0 + i < a.dim)) q += v[c][i] * v[c][i];
+        }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<WARP>(q, red[1]) / (float)a.dim + a.eps);
+    if (stats != nullptr && t == 0) stats[row] = make_float2(mean, rstd);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int64_t e0 = (int64_t)(t + c * G) * N - ph;
+        if (e0 >= a.dim) continue;
+        float w[N], b[N];
+        if (a.w != nullptr) load_params((const P*)a.w, e0, a.dim, w);
+        if (a.b != nullptr) load_params((const P*)a.b, e0, a.dim, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float o = v[c][i] * rstd;
+            if (a.w != nullptr) o *= w[i];
+            if (a.b != nullptr) o += b[i];
+            v[c][i] = o;
+        }
+        store_chunk(yr, e0, a.dim, v[c]);
+    }
+}
+
+// Rows too long for registers: one block per row, three passes over it (the second and third from L2).
+template <typename T, typename P>
+__global__ void ln_fwd_long_kernel(LnArgs a, T* __restrict__ y, float2* __restrict__ stats) {
+    constexpr int N = Chunk<T>::N;
+    __shared__ float red[2][32];
+    const int64_t row = blockIdx.x;
+    const T* xr = (const T*)a.x + row * a.x_stride;
+    T* yr = y + row * a.dim;
+    const int ph = row_phase(xr);
+    float v[N];
+    float s = 0.f;
+    for (int64_t e0 = (int64_t)threadIdx.x * N - ph; e0 < a.dim; e0 += (int64_t)blockDim.x * N) {
+        load_chunk(xr, e0, a.dim, 0.f, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += v[i];
+    }
+    const float mean = block_sum(s, red[0]) / (float)a.dim;
+    float q = 0.f;
+    for (int64_t e0 = (int64_t)threadIdx.x * N - ph; e0 < a.dim; e0 += (int64_t)blockDim.x * N) {
+        load_chunk(xr, e0, a.dim, mean, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) q += (v[i] - mean) * (v[i] - mean);
+    }
+    const float rstd = 1.f / sqrtf(block_sum(q, red[1]) / (float)a.dim + a.eps);
+    if (stats != nullptr && threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
+    for (int64_t e0 = (int64_t)threadIdx.x * N - ph; e0 < a.dim; e0 += (int64_t)blockDim.x * N) {
+        load_chunk(xr, e0, a.dim, 0.f, v);
+        float w[N], b[N];
+        if (a.w != nullptr) load_params((const P*)a.w, e0, a.dim, w);
+        if (a.b != nullptr) load_params((const P*)a.b, e0, a.dim, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float o = (v[i] - mean) * rstd;
+            if (a.w != nullptr) o *= w[i];
+            if (a.b != nullptr) o += b[i];
+            v[i] = o;
+        }
+        store_chunk(yr, e0, a.dim, v);
+    }
+}
+
+struct LnBwdArgs {
+    const void* x;
+    int64_t x_stride;
+    const void* dy;
+    int64_t dy_stride;
+    const void* w;
+    const float2* stats;
+    void* dx;               // may be null: only the parameters' gradients are wanted
+    float* part;            // [gridDim.x][2][dim]; null: the parameters' gradients are not wanted
+    int64_t rows, dim;
+};
+
+template <typename T, int VE>
+__device__ __forceinline__ void load_values(const T* p, int64_t e0, int64_t n, float (&v)[VE]) {
+    if (VE > 1) {
+        if (e0 < n) {
+            float t[Chunk<T>::N];
+            unpack16(*reinterpret_cast<const uint4*>(p + e0), t, (const T*)nullptr);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[i] = t[i % Chunk<T>::N];
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[i] = 0.f;
+        }
+    } else {
+        v[0] = e0 < n ? to_f32(p[e0]) : 0.f;
+    }
+}
+template <typename T, int VE>
+__device__ __forceinline__ void store_values(T* p, int64_t e0, int64_t n, const float (&v)[VE]) {
+    if (e0 >= n) return;
+    if (VE > 1) {
+        float t[Chunk<T>::N];
+#pragma unroll
+        for (int i = 0; i < Chunk<T>::N; ++i) t[i] = v[i % VE];
+        *reinterpret_cast<uint4*>(p + e0) = pack16(t, (const T*)nullptr);
+    } else {
+        p[e0] = from_f32<T>(v[0]);
+    }
+}
+
+// A thread owns the same columns of every row its warp (WARP) or block visits, so the sums over rows stay in registers
+// until the end: x and dy are read once for all three gradients.  VE values per access (16 bytes, or one value where rows do
+// not start on 16-byte boundaries), NC accesses.  Each block leaves one partial sum per column; ln_param_reduce_kernel
+// adds them in block order, so the result does not depend on timing.
+template <typename T, typename P, int VE, int NC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(LnBwdArgs a) {
+    extern __shared__ float sm[];
+    __shared__ float red[4][32];
+    const int G = WARP ? 32 : (int)blockDim.x;
+    const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
+    const int warp = threadIdx.x >> 5, nwarps = (int)(blockDim.x >> 5);
+    const int64_t row0 = WARP ? (int64_t)blockIdx.x * nwarps + warp : (int64_t)blockIdx.x;
+    const int64_t step = WARP ? (int64_t)gridDim.x * nwarps : (int64_t)gridDim.x;
+    const float inv_n = 1.f / (float)a.dim;
+    float w[NC][VE], dw[NC][VE], db[NC][VE];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int64_t e0 = (int64_t)(t + c * G) * VE;
+        if (a.w != nullptr) {
+            load_params<P, VE>((const P*)a.w, e0, a.dim, w[c]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) w[c][i] = 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) dw[c][i] = db[c][i] = 0.f;
+    }
+    int flip = 0;
+    for (int64_t row = row0; row < a.rows; row += step) {
+        const T* xr = (const T*)a.x + row * a.x_stride;
+        const T* gr = (const T*)a.dy + row * a.dy_stride;
+        const float2 st = a.stats[row];
+        float xh[NC][VE], g[NC][VE];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int64_t e0 = (int64_t)(t + c * G) * VE;
+            load_values<T, VE>(xr, e0, a.dim, xh[c]);
+            load_values<T, VE>(gr, e0, a.dim, g[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                xh[c][i] = (xh[c][i] - st.x) * st.y;     // beyond the row g is 0, so xh there counts for nothing
+                dw[c][i] += g[c][i] * xh[c][i];
+                db[c][i] += g[c][i];
+                g[c][i] *= w[c][i];
+                s1 += g[c][i];
+                s2 += g[c][i] * xh[c][i];
+            }
+        }
+        if (a.dx != nullptr) {
+            float m1, m2;
+            if (WARP) {
+                m1 = warp_sum(s1) * inv_n;
+                m2 = warp_sum(s2) * inv_n;
+            } else {
+                s1 = warp_sum(s1);
+                s2 = warp_sum(s2);
+                float* r1 = red[flip], *r2 = red[flip + 2];
+                flip ^= 1;
+                if ((threadIdx.x & 31) == 0) r1[warp] = s1, r2[warp] = s2;
+                __syncthreads();
+                const int lane = threadIdx.x & 31;
+                m1 = warp_sum(lane < nwarps ? r1[lane] : 0.f) * inv_n;
+                m2 = warp_sum(lane < nwarps ? r2[lane] : 0.f) * inv_n;
+            }
+            T* dxr = (T*)a.dx + row * a.dim;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float o[VE];
+#pragma unroll
+                for (int i = 0; i < VE; ++i) o[i] = st.y * (g[c][i] - m1 - xh[c][i] * m2);
+                store_values<T, VE>(dxr, (int64_t)(t + c * G) * VE, a.dim, o);
+            }
+        }
+    }
+    if (a.part == nullptr) return;
+    float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+    if (!WARP) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const int64_t e = (int64_t)(t + c * G) * VE + i;
+                if (e < a.dim) out[e] = dw[c][i], out[a.dim + e] = db[c][i];
+            }
+        return;
+    }
+    // the block's warps, in order
+    const int n2 = 2 * (int)a.dim;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            const int e = (t + c * G) * VE + i;
+            if (e < a.dim) sm[warp * n2 + e] = dw[c][i], sm[warp * n2 + (int)a.dim + e] = db[c][i];
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n2; e += blockDim.x) {
+        float s = 0.f;
+        for (int k = 0; k < nwarps; ++k) s += sm[k * n2 + e];
+        out[e] = s;
+    }
+}
+
+// Rows too long for registers: dx alone, one block per row.
+template <typename T, typename P>
+__global__ void ln_bwd_long_kernel(LnBwdArgs a) {
+    constexpr int N = Chunk<T>::N;
+    __shared__ float red[2][32];
+    const int64_t row = blockIdx.x;
+    const T* xr = (const T*)a.x + row * a.x_stride;
+    const T* gr = (const T*)a.dy + row * a.dy_stride;
+    T* dxr = (T*)a.dx + row * a.dim;
+    const int ph = row_phase(xr);
+    const float2 st = a.stats[row];
+    float s1 = 0.f, s2 = 0.f;
+    float x[N], g[N], w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = 1.f;
+    for (int64_t e0 = (int64_t)threadIdx.x * N - ph; e0 < a.dim; e0 += (int64_t)blockDim.x * N) {
+        load_chunk(xr, e0, a.dim, st.x, x);
+        load_chunk(gr, e0, a.dim, 0.f, g);
+        if (a.w != nullptr) load_params((const P*)a.w, e0, a.dim, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s1 += g[i] * w[i];
+            s2 += g[i] * w[i] * ((x[i] - st.x) * st.y);
+        }
+    }
+    const float m1 = block_sum(s1, red[0]) / (float)a.dim, m2 = block_sum(s2, red[1]) / (float)a.dim;
+    for (int64_t e0 = (int64_t)threadIdx.x * N - ph; e0 < a.dim; e0 += (int64_t)blockDim.x * N) {
+        load_chunk(xr, e0, a.dim, st.x, x);
+        load_chunk(gr, e0, a.dim, 0.f, g);
+        if (a.w != nullptr) load_params((const P*)a.w, e0, a.dim, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = st.y * (g[i] * w[i] - m1 - (x[i] - st.x) * st.y * m2);
+        store_chunk(dxr, e0, a.dim, x);
+    }
+}
+
+// The parameters' gradients for such rows: thread = column, blockIdx.y = one run of rows.
+template <typename T>
+__global__ void ln_bwd_cols_kernel(LnBwdArgs a, int64_t rows_per_part) {
+    const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (e >= a.dim) return;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per_part, r1 = min(a.rows, r0 + rows_per_part);
+    float dw = 0.f, db = 0.f;
+    for (int64_t r = r0; r < r1; ++r) {
+        const float2 st = a.stats[r];
+        const float g = to_f32(((const T*)a.dy)[r * a.dy_stride + e]);
+        dw += g * ((to_f32(((const T*)a.x)[r * a.x_stride + e]) - st.x) * st.y);
+        db += g;
+    }
+    a.part[(int64_t)blockIdx.y * 2 * a.dim + e] = dw;
+    a.part[(int64_t)blockIdx.y * 2 * a.dim + a.dim + e] = db;
+}
+
+// Partial sums [parts][2][dim] -> dw, db: 32 columns per block, thread row y adds parts y, y + 8, ... and the eight sums are
+// added in order.
+template <typename P>
+__global__ void ln_param_reduce_kernel(const float* __restrict__ part, int parts, int64_t dim, P* __restrict__ dw, P* __restrict__ db) {
+    __shared__ float sm[8][33];
+    const int64_t e = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    float s = 0.f;
+    if (e < 2 * dim)
+        for (int p = threadIdx.y; p < parts; p += 8) s += part[(int64_t)p * 2 * dim + e];
+    sm[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && e < 2 * dim) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
+        if (e < dim) {
+            if (dw != nullptr) dw[e] = from_f32<P>(s);
+        } else if (db != nullptr) {
+            db[e - dim] = from_f32<P>(s);
+        }
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------
+template <typename T, typename P, bool WARP>
+static void ln_fwd_launch(int ch, unsigned grid, int threads, const LnArgs& a, T* y, float2* stats, cudaStream_t st) {
+    switch (ch) {
+        case 1: ln_fwd_kernel<T, P, 1, WARP><<<grid, threads, 0, st>>>(a, y, stats); break;
+        case 2: ln_fwd_kernel<T, P, 2, WARP><<<grid, threads, 0, st>>>(a, y, stats); break;
+        default: ln_fwd_kernel<T, P, 4, WARP><<<grid, threads, 0, st>>>(a, y, stats); break;
+    }
+}
+static int pow2_at_least(int64_t n) {
+    int p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+template <typename T, typename P>
+static int ln_fwd(const LnArgs& a, void* y, float2* stats, cudaStream_t st) {
+    constexpr int N = Chunk<T>::N;
+    const int64_t chunks = (a.dim + N - 1 + N - 1) / N;    // with any phase
+    launch_begin(K_LN_FWD, st);
+    if (chunks <= 32 * kLnMaxChunks) {
+        const int ch = pow2_at_least((chunks + 31) / 32);
+        ln_fwd_launch<T, P, true>(ch, (unsigned)((a.rows + 7) / 8), 256, a, (T*)y, stats, st);
+    } else if (chunks <= 1024 * kLnMaxChunks) {
+        // two chunks a thread, four from 2048 chunks on
+        const int threads = (int)std::min<int64_t>(1024, std::max(64, pow2_at_least((chunks + 1) / 2)));
+        ln_fwd_launch<T, P, false>(pow2_at_least((chunks + threads - 1) / threads), (unsigned)a.rows, threads, a, (T*)y, stats, st);
+    } else {
+        ln_fwd_long_kernel<T, P><<<(unsigned)a.rows, 1024, 0, st>>>(a, (T*)y, stats);
+    }
+    launch_end(K_LN_FWD, st);
+    CGB_CUDA(cudaGetLastError());
+    return CGB200_OK;
+}
+
+// Blocks of the backward kernel (= partial sums) for rows a thread can hold, and threads per block.
+struct LnBwdShape {
+    bool fits, warp;
+    int nc, threads, grid;
+};
+static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int ve) {
+    LnBwdShape s{};
+    const int64_t acc = (dim + ve - 1) / ve;      // accesses per row
+    const int ncmax = kLnBwdValues / ve;
+    s.fits = acc <= (int64_t)ncmax * kLnBwdMaxThreads;
+    s.warp = acc <= 32 * ncmax;
+    if (!s.fits) {
+        // column kernel: runs of rows such that about 2048 threads per SM are busy
+        const int64_t cols = (dim + 255) / 256;
+        s.grid = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(rows, 256), (kNumSM * 8 + cols - 1) / cols));
+        return s;
+    }
+    if (s.warp) {
+        s.threads = 256;
+        s.nc = pow2_at_least((acc + 31) / 32);
+        s.grid = (int)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, kNumSM * 4));
+    } else {
+        s.threads = (int)std::min<int64_t>(kLnBwdMaxThreads, std::max(64, pow2_at_least((acc + ncmax - 1) / ncmax)));
+        s.nc = pow2_at_least((acc + s.threads - 1) / s.threads);
+        s.grid = (int)std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)kNumSM * (1024 / s.threads)));
+    }
+    return s;
+}
+template <typename T, typename P, int VE, bool WARP>
+static void ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
+    const size_t smem = WARP ? (size_t)(s.threads / 32) * 2 * a.dim * sizeof(float) : 0;
+#define CGB_LN_BWD(NC_)                                                                              \
+    if constexpr (NC_ * VE <= kLnBwdValues) {                                                        \
+        ln_bwd_kernel<T, P, VE, NC_, WARP><<<s.grid, s.threads, smem, st>>>(a);                      \
+    }
+    switch (s.nc) {
+        case 1: CGB_LN_BWD(1) break;
+        case 2: CGB_LN_BWD(2) break;
+        case 4: CGB_LN_BWD(4) break;
+        case 8: CGB_LN_BWD(8) break;
+        default: CGB_LN_BWD(16) break;
+    }
+#undef CGB_LN_BWD
+}
+
+template <typename T, typename P>
+static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
+    constexpr int N = Chunk<T>::N;
+    auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    const bool vec = a.dim % N == 0 && a.x_stride % N == 0 && a.dy_stride % N == 0 && at16(a.x) && at16(a.dy) && at16(a.dx);
+    const LnBwdShape s = ln_bwd_shape(a.rows, a.dim, vec ? N : 1);
+    if (a.rows > 0) {
+        if (s.fits) {
+            launch_begin(K_LN_BWD, st);
+            if (vec && s.warp) ln_bwd_launch<T, P, N, true>(s, a, st);
+            else if (vec) ln_bwd_launch<T, P, N, false>(s, a, st);
+            else if (s.warp) ln_bwd_launch<T, P, 1, true>(s, a, st);
+            else ln_bwd_launch<T, P, 1, false>(s, a, st);
+            launch_end(K_LN_BWD, st);
+        } else {
+            if (a.dx != nullptr) {
+                launch_begin(K_LN_BWD, st);
+                ln_bwd_long_kernel<T, P><<<(unsigned)a.rows, 1024, 0, st>>>(a);
+                launch_end(K_LN_BWD, st);
+            }
+            if (a.part != nullptr) {
+                launch_begin(K_LN_BWD, st);
+                ln_bwd_cols_kernel<T><<<dim3((unsigned)((a.dim + 255) / 256), s.grid), 256, 0, st>>>(a, (a.rows + s.grid - 1) / s.grid);
+                launch_end(K_LN_BWD, st);
+            }
+        }
+        CGB_CUDA(cudaGetLastError());
+    }
+    if (a.part != nullptr) {
+        launch_begin(K_LN_REDUCE, st);
+        ln_param_reduce_kernel<P><<<(unsigned)((2 * a.dim + 31) / 32), dim3(32, 8), 0, st>>>(a.part, a.rows > 0 ? s.grid : 0, a.dim, (P*)dw, (P*)db);
+        launch_end(K_LN_REDUCE, st);
+        CGB_CUDA(cudaGetLastError());
+    }
+    return CGB200_OK;
+}
+
+}  // namespace cgb200
+
+using namespace cgb200;
+
+#define CGB_LN_TYPES(CALL_)                                                                    \
+    do {                                                                                       \
+        if (dtype == CGB200_F32) return CALL_(float, float);                                   \
+        if (dtype == CGB200_BF16 && param_dtype == CGB200_F32) return CALL_(__nv_bfloat16, float);   \
+        if (dtype == CGB200_BF16) return CALL_(__nv_bfloat16, __nv_bfloat16);                  \
+        if (param_dtype == CGB200_F32) return CALL_(__half, float);                            \
+        return CALL_(__half, __half);                                                          \
+    } while (0)
+
+static int ln_check(int64_t rows, int64_t dim, int dtype, int param_dtype) {
+    CGB_REQUIRE(rows >= 0 && rows <= 0x7fffffff && dim > 0 && dim <= (1ll << 30), "layer norm: sizes out of range");
+    CGB_REQUIRE(dtype >= CGB200_F32 && dtype <= CGB200_F16, "layer norm: unknown type");
+    CGB_REQUIRE(param_dtype == dtype || param_dtype == CGB200_F32, "layer norm: weight and bias have the type of x or float32");
+    return CGB200_OK;
+}
+
+extern "C" {
+
+int cgb200_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps, void* y, float* stats,
+                          int64_t rows, int64_t dim, int dtype, int param_dtype, void* stream) {
+    if (int rc = ln_check(rows, dim, dtype, param_dtype)) return rc;
+    if (rows == 0) return CGB200_OK;
+    CGB_REQUIRE(x != nullptr && y != nullptr, "layer norm: null buffer");
+    CGB_REQUIRE(x_stride >= 0 && x_stride <= (1ll << 40), "layer norm: row stride out of range");
+    const LnArgs a{x, x_stride, weight, bias, eps, rows, dim};
+    cudaStream_t st = (cudaStream_t)stream;
+#define CGB_CALL(T_, P_) ln_fwd<T_, P_>(a, y, (float2*)stats, st)
+    CGB_LN_TYPES(CGB_CALL);
+#undef CGB_CALL
+}
+
+int64_t cgb200_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int dtype) {
+    if (ln_check(rows, dim, dtype, dtype) != CGB200_OK) return -1;
+    // whichever of the two access widths the buffers' alignment will allow
+    const int n = dtype == CGB200_F32 ? 4 : 8;
+    const int parts = std::max(ln_bwd_shape(rows, dim, 1).grid, dim % n == 0 ? ln_bwd_shape(rows, dim, n).grid : 0);
+    return (int64_t)parts * 2 * dim * (int64_t)sizeof(float);
+}
+
+int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight, const float* stats,
+                          void* dx, void* dweight, void* dbias, int64_t rows, int64_t dim, int dtype, int param_dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+    if (int rc = ln_check(rows, dim, dtype, param_dtype)) return rc;
+    const bool params = dweight != nullptr || dbias != nullptr;
+    if (!params && (dx == nullptr || rows == 0)) return CGB200_OK;
+    CGB_REQUIRE(rows == 0 || (x != nullptr && dy != nullptr && stats != nullptr), "layer norm: null buffer");
+    CGB_REQUIRE(x_stride >= 0 && x_stride <= (1ll << 40) && dy_stride >= 0 && dy_stride <= (1ll << 40), "layer norm: row stride out of range");
+    if (params) {
+        const int64_t need = cgb200_layer_norm_bwd_workspace_bytes(rows, dim, dtype);
+        if (workspace == nullptr || workspace_bytes < need) {
+            set_error("workspace too small: need " + std::to_string(need) + " bytes");
+            return CGB200_ERR_WORKSPACE;
+        }
+        CGB_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");
+    }
+    const LnBwdArgs a{x, x_stride, dy, dy_stride, weight, (const float2*)stats, dx, params ? (float*)workspace : nullptr, rows, dim};
+    cudaStream_t st = (cudaStream_t)stream;
+#define CGB_CALL(T_, P_) ln_bwd<T_, P_>(a, dweight, dbias, st)
+    CGB_LN_TYPES(CGB_CALL);
+#undef CGB_CALL
+}
+
+}  // extern "C"

@@ -33,7 +33,8 @@ static const char* kKernelNames[K_COUNT] = {"cg_table", "cg_product_fwd", "cg_pr
                                             "fused_grad_w", "fused_grad_f", "fused_grad_f_reduce",
                                             "fused_grad_w_reduce", "tc_pack_weights", "fused_fwd_tensor", "fused_grad_w_tensor", "fused_grad_f_tensor",
                                             "sh_pack", "sh_project_tensor", "raycast_pack", "raycast_sphere", "fused_fwd_tensor_reduce", "grad_mid_pack_weights",
-                                            "grad_mid_tensor"};
+                                            "grad_mid_tensor", "layer_norm_fwd", "layer_norm_bwd", "layer_norm_reduce", "log_probs_fwd", "log_probs_bwd",
+                                            "distill_fwd", "distill_bwd", "gated_ff_fwd", "gated_ff_bwd"};
 struct TimedLaunch {
     int kid;
     cudaEvent_t a, b;

@@ -1,0 +1,134 @@
+// Element access shared by the kernels that walk rows of a (rows, columns) matrix of float32, bfloat16 or float16 values:
+// 16-byte chunks that fall on 16-byte boundaries wherever the row starts, and sums over a warp or a block.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace cgb200 {
+
+constexpr int kNumSM = 148;   // streaming multiprocessors of a B200
+
+template <typename T>
+struct Chunk {
+    static constexpr int N = 16 / (int)sizeof(T);   // values of one 16-byte access
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ void unpack16(const uint4& u, float (&v)[4], const float*) {
+    v[0] = __uint_as_float(u.x);
+    v[1] = __uint_as_float(u.y);
+    v[2] = __uint_as_float(u.z);
+    v[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack16(const uint4& u, float (&v)[8], const __nv_bfloat16*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack16(const uint4& u, float (&v)[8], const __half*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __half2 h;
+        memcpy(&h, &w[i], 4);
+        const float2 f = __half22float2(h);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ uint4 pack16(const float (&v)[4], const float*) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint4 pack16(const float (&v)[8], const __nv_bfloat16*) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        memcpy(&w[i], &h, 4);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack16(const float (&v)[8], const __half*) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        memcpy(&w[i], &h, 4);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Values a row's first chunk lies before the row: chunk c of a row covers its values [c * N - phase, c * N - phase + N), so
+// that every chunk starts on a 16-byte boundary whatever the row's own address; values outside [0, n) are never touched.
+template <typename T>
+__device__ __forceinline__ int row_phase(const T* row) {
+    return (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % Chunk<T>::N);
+}
+// Chunk at value e0 (possibly negative) of a row of n values; values outside the row read as `fill`.
+template <typename T, int N = Chunk<T>::N>
+__device__ __forceinline__ void load_chunk(const T* row, int64_t e0, int64_t n, float fill, float (&v)[N]) {
+    if (e0 >= 0 && e0 + N <= n && aligned16(row + e0)) {
+        unpack16(*reinterpret_cast<const uint4*>(row + e0), v, (const T*)nullptr);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(row[e0 + i]) : fill;
+    }
+}
+template <typename T, int N = Chunk<T>::N>
+__device__ __forceinline__ void store_chunk(T* row, int64_t e0, int64_t n, const float (&v)[N]) {
+    if (e0 >= 0 && e0 + N <= n && aligned16(row + e0)) {
+        *reinterpret_cast<uint4*>(row + e0) = pack16(v, (const T*)nullptr);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = from_f32<T>(v[i]);
+    }
+}
+// N parameter values (of any of the three types) from value e0 on
+template <typename P, int N>
+__device__ __forceinline__ void load_params(const P* w, int64_t e0, int64_t n, float (&v)[N]) {
+    if (N * sizeof(P) % 16 == 0 && e0 >= 0 && e0 + N <= n && aligned16(w + e0)) {
+#pragma unroll
+        for (int c = 0; c < (int)(N * sizeof(P) / 16); ++c) {
+            float t[Chunk<P>::N];
+            unpack16(*(reinterpret_cast<const uint4*>(w + e0) + c), t, (const P*)nullptr);
+#pragma unroll
+            for (int i = 0; i < Chunk<P>::N; ++i) v[c * Chunk<P>::N + i] = t[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(w[e0 + i]) : 0.f;
+    }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Sum over the block in a fixed order, the same value in every thread.  `buf` holds 32 floats and may be reused by the next
+// call only after another barrier: callers alternate between two.
+__device__ __forceinline__ float block_sum(float v, float* buf) {
+    v = warp_sum(v);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = (int)(blockDim.x >> 5);
+    if (lane == 0) buf[warp] = v;
+    __syncthreads();
+    return warp_sum(lane < nw ? buf[lane] : 0.f);
+}
+
+}  // namespace cgb200

@@ -276,6 +276,83 @@ int cgb200_raycast_sphere(const float* vertices, int64_t n_vertices, const int32
                           int64_t n_points, float* image, void* workspace, int64_t workspace_bytes, int32_t* status_word,
                           void* stream);
 
+/*
+ * The operators between a network's invariant embedding and its answers (no counterpart in the reference's kernels, which
+ * leaves them to torch).  Matrices are row-major with the given number of values between rows (`stride`), values of one of
+ * three types; sums, norms and softmax statistics are held in float32 or more and every result is rounded once.  Pointers
+ * need the alignment of their type only.  Results do not depend on timing (no float atomics).
+ */
+#define CGB200_F32              0
+#define CGB200_BF16             1
+#define CGB200_F16              2
+
+/*
+ * Layer norm of each row:  y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps).
+ *   weight, bias   [dim] of type param_dtype (that of x, or CGB200_F32); NULL = 1 and 0
+ *   y              [rows][dim], contiguous
+ *   stats          float[rows][2] (mean, rstd) for the backward; NULL where none follows
+ * Backward: dx [rows][dim], dweight and dbias [dim] of type param_dtype, each NULL where it is not wanted.  With dweight or
+ * dbias it needs a workspace of cgb200_layer_norm_bwd_workspace_bytes (16-byte aligned, contents undefined); with 0 rows it
+ * writes zeros to them.
+ */
+int cgb200_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps, void* y, float* stats,
+                          int64_t rows, int64_t dim, int dtype, int param_dtype, void* stream);
+int64_t cgb200_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int dtype);
+int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight, const float* stats,
+                          void* dx, void* dweight, void* dbias, int64_t rows, int64_t dim, int dtype, int param_dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/*
+ * Gated feed-forward block:  h = act(x Wg^T) * (x Wu^T),  Wg and Wu [hidden][dim].
+ *   h         [rows][hidden], contiguous
+ *   gate_up   float[2][rows][hidden]: the two projections, for the backward; NULL where none follows
+ * Backward: dx [rows][dim], dw_gate and dw_up [hidden][dim], each NULL where it is not wanted; with 0 rows it writes zeros to
+ * the weights' gradients.  workspace: cgb200_gated_ff_workspace_bytes(..., backward = 0 or 1) bytes, 256-byte aligned, contents
+ * undefined; one workspace serves one call at a time.
+ */
+#define CGB200_ACT_SILU         0   /* g / (1 + exp(-g))                  */
+#define CGB200_ACT_GELU         1   /* g * (1 + erf(g / sqrt 2)) / 2      */
+#define CGB200_ACT_RELU         2   /* max(g, 0)                          */
+int64_t cgb200_gated_ff_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int dtype, int backward);
+int cgb200_gated_ff_fwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
+                        int activation, void* h, float* gate_up, int64_t rows, int64_t dim, int64_t hidden, int dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int cgb200_gated_ff_bwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
+                        int activation, const float* gate_up, const void* dh, int64_t dh_stride, void* dx, void* dw_gate, void* dw_up,
+                        int64_t rows, int64_t dim, int64_t hidden, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of given classes, the entropy and the `top` most probable classes of each row of logits.
+ *   targets         int64[rows]; a negative class marks a row without one (log probability 0, no gradient through it), one beyond
+ *                   the last gives NaN.  NULL: none wanted (log_prob unused)
+ *   top             0..128, at most `classes`; top_ids int64[rows][top] in order of score, equal scores by class, NaN first
+ *   stats           float[rows][2] for the backward, NULL where none follows
+ * A row of nothing but -inf has no distribution: log probabilities -inf, entropy 0, gradients 0.
+ * Backward: dlogits [rows][classes] = gradient through log_prob and entropy (g_* float[rows]; NULL = 0).
+ */
+int cgb200_log_probs_fwd(const void* logits, int64_t stride, const int64_t* targets, int top, float* log_prob, float* entropy,
+                         float* top_log_probs, int64_t* top_ids, float* stats, int64_t rows, int64_t classes, int dtype, void* stream);
+int cgb200_log_probs_bwd(const void* logits, int64_t stride, const int64_t* targets, const float* entropy, const float* stats,
+                         const float* g_log_prob, const float* g_entropy, void* dlogits, int64_t rows, int64_t classes, int dtype,
+                         void* stream);
+
+/*
+ * Distillation from a teacher's best scores:  loss = T^2 sum_k q_k (log q_k - log p(id_k)),  q = softmax over the row's entries of
+ * teacher_scores / T,  p = softmax of logits / T over all classes.
+ *   teacher_ids      int64[rows][n_teacher], contiguous; a negative class is an entry that is not there, one beyond the last makes
+ *                    the row NaN; a class named twice counts with both weights
+ *   teacher_scores   [rows][n_teacher] of type teacher_dtype, contiguous; -inf is an entry of weight 0
+ *   n_teacher        1..1024;  temperature 0.001..1000
+ * A row without entries has loss 0 and gradient 0; a row of logits that are all -inf has loss +inf and gradient 0.
+ */
+#define CGB200_MAX_TEACHER      1024
+int cgb200_distill_fwd(const void* logits, int64_t stride, const int64_t* teacher_ids, const void* teacher_scores, int n_teacher,
+                       int teacher_dtype, float temperature, float* loss, float* stats, int64_t rows, int64_t classes, int dtype,
+                       void* stream);
+int cgb200_distill_bwd(const void* logits, int64_t stride, const int64_t* teacher_ids, const void* teacher_scores, int n_teacher,
+                       int teacher_dtype, float temperature, const float* stats, const float* g_loss, void* dlogits, int64_t rows,
+                       int64_t classes, int dtype, void* stream);
+
 /* Number of kernels this library launched in this process since the last reset (bench accounting). */
 int64_t cgb200_launch_count(int reset);
 
