@@ -52,7 +52,7 @@ SIGNATURES = {
     "cgb200_layer_norm_fwd": (ctypes.c_int, [vp, i64, vp, vp, ctypes.c_float, vp, vp, i64, i64, ctypes.c_int, ctypes.c_int, vp]),
     "cgb200_layer_norm_bwd_workspace_bytes": (i64, [i64, i64, ctypes.c_int]),
     "cgb200_layer_norm_bwd": (ctypes.c_int, [vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, ctypes.c_int, ctypes.c_int, vp, i64, vp]),
-    "cgb200_gated_ff_workspace_bytes": (i64, [i64, i64, i64, ctypes.c_int, ctypes.c_int]),
+    "cgb200_gated_ff_workspace_bytes": (i64, [vp, i64, vp, i64, vp, i64, i64, i64, i64, ctypes.c_int, ctypes.c_int]),
     "cgb200_gated_ff_fwd": (ctypes.c_int, [vp, i64, vp, i64, vp, i64, ctypes.c_int, vp, vp, i64, i64, i64, ctypes.c_int, vp, i64, vp]),
     "cgb200_gated_ff_bwd": (ctypes.c_int, [vp, i64, vp, i64, vp, i64, ctypes.c_int, vp, vp, i64, vp, vp, vp, i64, i64, i64, ctypes.c_int,
                                            vp, i64, vp]),

@@ -1,0 +1,377 @@
+// Tensor-core products of the gated feed-forward block (gated_ff.cu): one persistent kernel for out[i][j] = sum_k A[i][k] B[j][k] over
+// a list of problems, with the gated epilogue or a plain one.
+//
+// Block: 128 rows i x BN columns j, 64 terms k per stage.  One thread issues the tiled bulk copies (64 x 64 boxes, 128-byte swizzle) of a
+// stage, one thread the tcgen05.mma of the stages before, eight warps read finished accumulators from tensor memory and write
+// them out while the next tile is multiplied into the other accumulator.  An operand may have its k axis (rows of the product in
+// memory) or its i / j axis contiguous; the copies are the same, only coordinates and descriptors differ, so no operand is ever
+// transposed in memory.
+//
+// float32 operands come as three bfloat16 planes (8 + 8 + 8 bits, together exact).  Of the nine plane products the six that reach
+// 2^-24 are taken; the leading one has its own accumulator, because the tensor core truncates each addition and the small
+// products would otherwise add steps to its long chain.  Every kFfFlush stages the accumulators are added, rounded, to sums in registers.
+#pragma once
+
+#include <cuda.h>
+
+#include "row_ops.cuh"
+#include "tc_ptx.cuh"
+
+namespace cgb200 {
+
+constexpr int kFfBM = 128, kFfBK = 64;
+constexpr int kFfThreads = 384;                // producer, issuer, allocator, idle; eight epilogue warps
+constexpr int kFfEpiWarps = 8;
+constexpr int kFfBox = 64 * 64 * 2;            // bytes of one copy
+constexpr int kFfStageBytes = 192 * 1024;      // all stages of a block
+constexpr int kFfFlush = 4;                    // stages between flushes of the three-plane form (16 truncating additions)
+constexpr int kFfStaging = 32 * 33;            // floats an epilogue warp turns rows into columns with
+constexpr size_t kFfSmem = 1024 + kFfStageBytes + kFfEpiWarps * kFfStaging * sizeof(float);
+static_assert(kFfSmem <= kMaxDynSmem, "stages and staging must fit a block's shared memory");
+
+struct FfProblem {
+    int a_map[2], b_map[2];     // tensor maps of A and B: by source of the contraction (dx), set of rows (dW: A), half of the columns (forward: B)
+    int a_mn, b_mn;             // 1: the operand's i / j axis is the contiguous one
+    int sources, kblk;          // the contraction runs over `sources` x kblk stages
+    int sets, tiles_i, tiles_j; // row tiles of each set of rows, column tiles
+    int splits, kper;           // the contraction in parts of kper stages
+    int unit0;                  // first work unit of this problem
+    int64_t n_i;                // rows of a set
+    int n_j;
+    void* out[2];               // per set; the forward: h, and g followed by u
+    float* part;                // [splits][sets * n_i][n_j] where splits > 1
+};
+struct FfGemmArgs {
+    CUtensorMap map[5];
+    FfProblem p[2];
+    int problems, units;
+    uint32_t idesc_type;        // operand format bits of the instruction descriptor
+    int act;
+    uint32_t polls;
+};
+
+__device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Descriptor of an operand tile made of 64 x 64 boxes in the 128-byte swizzle.  k contiguous: a box is 64 rows of 128 bytes, 8-row
+// groups 1024 bytes apart.  i / j contiguous: a box is 64 k-rows of 64 values; groups of 8 k are 1024 bytes apart (stride offset),
+// the next 64 values one box (leading offset).  [61,64) = 2 is the 128-byte swizzle.
+__device__ __forceinline__ uint64_t box_desc(uint32_t saddr, int mn) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(mn ? kFfBox >> 4 : 1) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+
+// act(g) and its derivative
+template <bool GRAD>
+__device__ __forceinline__ float2 activate(int act, float g) {
+    if (act == CGB200_ACT_RELU) return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);
+    if (act == CGB200_ACT_SILU) {
+        const float s = 1.f / (1.f + __expf(-g));
+        // where s is 0, g may be -inf
+        return s == 0.f ? make_float2(0.f, 0.f) : make_float2(g * s, GRAD ? s * (1.f + g * (1.f - s)) : 0.f);
+    }
+    const float c = 0.5f * erfcf(-0.70710678118654752f * g);
+    return make_float2(c == 0.f ? 0.f : g * c, GRAD ? c + (fabsf(g) > 20.f ? 0.f : g * __expf(-0.5f * g * g) * 0.39894228040143268f) : 0.f);
+}
+
+struct FfUnit {
+    const FfProblem* p;
+    int set, split, k0, k1;
+    int64_t i0;
+    int j0;        // in columns of the product's output
+};
+// Tiles in groups of eight row tiles, columns next: the blocks at work at one time share rows of A and of B in L2.
+__device__ __forceinline__ FfUnit ff_unit(const FfGemmArgs& a, int u, int jw) {
+    FfUnit t;
+    t.p = &a.p[a.problems > 1 && u >= a.p[1].unit0 ? 1 : 0];
+    const FfProblem& p = *t.p;
+    int v = u - p.unit0;
+    const int per_set = p.tiles_i * p.tiles_j, tiles = p.sets * per_set;
+    t.split = v / tiles;
+    v -= t.split * tiles;
+    t.set = v / per_set;
+    v -= t.set * per_set;
+    const int group = v / (8 * p.tiles_j), first = group * 8, height = min(8, p.tiles_i - first);
+    v -= first * p.tiles_j;
+    t.i0 = (int64_t)(first + v % height) * kFfBM;
+    t.j0 = v / height * jw;
+    t.k0 = t.split * p.kper;
+    t.k1 = min(p.sources * p.kblk, t.k0 + p.kper);
+    return t;
+}
+
+// 32 x 32 values, row = lane, to columns col0.. of rows row0.. of a row-major matrix: through shared memory, so that a warp
+// writes neighbouring columns.
+template <typename O>
+__device__ __forceinline__ void write_block(const float (&v)[32], float* st, O* out, int64_t row0, int64_t n_rows, int64_t ld, int col0, int n_cols) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 32; ++c) st[lane * 33 + c] = v[c];
+    __syncwarp();
+    if (col0 + lane < n_cols) {
+        const int n = (int)min((int64_t)32, n_rows - row0);
+        O* o = out + row0 * ld + col0 + lane;
+#pragma unroll 8
+        for (int r = 0; r < n; ++r) o[r * ld] = from_f32<O>(st[r * 33 + lane]);
+    }
+}
+
+
+template <int PLANES, int BN, typename T, bool FWD>
+__global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_constant__ FfGemmArgs a) {
+    constexpr int kStage = PLANES * (kFfBM + BN) * kFfBK * 2;
+    constexpr int kStages = kFfStageBytes / kStage;
+    constexpr int kAccCols = PLANES == 1 ? BN : 2 * BN;      // columns of one accumulator
+    constexpr int kTmemCols = 2 * kAccCols;
+    constexpr int JW = FWD ? BN / 2 : BN;                    // output columns of a tile
+    constexpr int kFlush = PLANES == 1 ? 1 << 30 : kFfFlush;
+    static_assert(kTmemCols <= 512, "two accumulators must fit the tensor memory");
+    extern __shared__ char dyn[];
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], stopped;
+    __shared__ uint32_t tmem_ptr;
+    __shared__ int failed_flag;
+    volatile int* failed = &failed_flag;
+    char* base = dyn + ((1024 - (smem_u32(dyn) & 1023)) & 1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        failed_flag = 0;
+        for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < 2; ++s) mbar_init(&acc_full[s], 1), mbar_init(&acc_empty[s], kFfEpiWarps);
+        mbar_init(&stopped, 1);
+        fence_mbar_init();
+    }
+    if (warp == 2) tmem_alloc(&tmem_ptr, kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_ptr;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, issued = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            for (int u = blockIdx.x; u < a.units && ok; u += gridDim.x) {
+                const FfUnit t = ff_unit(a, u, JW);
+                const FfProblem& p = *t.p;
+                for (int it = t.k0; it < t.k1; ++it) {
+                    if (!mbar_wait(&empty[s], ph, failed, a.polls)) {
+                        ok = false;
+                        break;
+                    }
+                    const int src = p.sources > 1 && it >= p.kblk ? 1 : 0, k = (it - src * p.kblk) * kFfBK;
+                    const CUtensorMap* am = &a.map[p.a_map[p.sets > 1 ? t.set : src]];
+                    char* d = base + s * kStage;
+                    mbar_arrive_expect_tx(&full[s], kStage);
+#pragma unroll
+                    for (int q = 0; q < PLANES; ++q) {
+#pragma unroll
+                        for (int b = 0; b < kFfBM / 64; ++b, d += kFfBox) {
+                            const int i = (int)t.i0 + 64 * b;
+                            tma_box(d, am, p.a_mn ? i : k, p.a_mn ? k : i, q, &full[s]);
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < PLANES; ++q) {
+#pragma unroll
+                        for (int b = 0; b < BN / 64; ++b, d += kFfBox) {
+                            const int second = FWD && b >= BN / 128;      // the up projection's half of the columns
+                            const CUtensorMap* bm = &a.map[p.b_map[FWD ? second : src]];
+                            const int j = t.j0 + 64 * (b - second * (BN / 128));
+                            tma_box(d, bm, p.b_mn ? j : k, p.b_mn ? k : j, q, &full[s]);
+                        }
+                    }
+                    ++issued;
+                    if (++s == kStages) s = 0, ph ^= 1;
+                }
+            }
+            if (!ok) {
+                // let the copies in flight land before the block gives up its shared memory: the last kStages issued ones
+                for (int n = max(0, issued - kStages); n < issued; ++n) mbar_drain(&full[n % kStages], (n / kStages) & 1, a.polls);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0, acc = 0;
+            uint32_t ph = 0, acc_ph = 1;
+            bool ok = true;
+            for (int u = blockIdx.x; u < a.units && ok; u += gridDim.x) {
+                const FfUnit t = ff_unit(a, u, JW);
+                const FfProblem& p = *t.p;
+                const uint32_t idesc = (1u << 4) | a.idesc_type | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
+                                       ((uint32_t)(kFfBM >> 4) << 24);
+                const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+                for (int it = t.k0; it < t.k1;) {
+                    if (!mbar_wait(&acc_empty[acc], acc_ph, failed, a.polls)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = tmem + acc * kAccCols;
+                    const int stop = min(t.k1 - it, kFlush) + it;
+                    bool first = true;
+                    for (; it < stop; ++it) {
+                        if (!mbar_wait(&full[s], ph, failed, a.polls)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t sa = smem_u32(base + s * kStage), sb = sa + PLANES * kFfBM * kFfBK * 2;
+                        const uint64_t da = box_desc(sa, p.a_mn), db = box_desc(sb, p.b_mn);
+                        if constexpr (PLANES == 1) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_16bit(d, desc_advance(da, k * a_step), desc_advance(db, k * b_step), idesc, !first || k > 0);
+                        } else {
+                            constexpr uint32_t pa = kFfBM * kFfBK * 2, pb = BN * kFfBK * 2;     // bytes of a plane
+                            constexpr int qa[5] = {0, 2, 1, 0, 1}, qb[5] = {2, 0, 1, 1, 0};
+#pragma unroll
+                            for (int x = 0; x < 5; ++x)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    mma_16bit(d + BN, desc_advance(da, qa[x] * pa + k * a_step), desc_advance(db, qb[x] * pb + k * b_step), idesc,
+                                              !first || x > 0 || k > 0);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_16bit(d, desc_advance(da, k * a_step), desc_advance(db, k * b_step), idesc, !first || k > 0);
+                        }
+                        first = false;
+                        tc_commit(&empty[s]);
+                        if (++s == kStages) s = 0, ph ^= 1;
+                    }
+                    if (!ok) break;
+                    tc_commit(&acc_full[acc]);
+                    if (++acc == 2) acc = 0, acc_ph ^= 1;
+                }
+            }
+            if (!ok) {      // the products issued so far end before the block gives up its memories
+                tc_commit(&stopped);
+                mbar_drain(&stopped, 0, a.polls);
+            }
+        }
+    } else if (warp >= 4) {
+        const int ew = warp - 4, quad = ew & 3, side = ew >> 2;      // 32 rows of the tile, half of its columns
+        float* st = (float*)(base + kFfStageBytes) + ew * kFfStaging;
+        int acc = 0;
+        uint32_t acc_ph = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
+            const FfUnit t = ff_unit(a, u, JW);
+            const FfProblem& p = *t.p;
+            const int64_t row0 = t.i0 + quad * 32;
+            const bool rows_here = row0 < p.n_i;
+            constexpr int kBlocks = JW / 64;                         // 32-column blocks of this warp's half
+            // what the block of output columns `c` of this warp is made of: accumulator columns `at` (and at + BN / 2 for the up half)
+            auto emit = [&](int c, float (&g)[32], float (&up)[32]) {
+                const int col0 = t.j0 + side * (JW / 2) + c * 32;
+                if (!rows_here || col0 >= p.n_j) return;
+                if constexpr (FWD) {
+                    if (p.out[1] != nullptr) {
+                        write_block(g, st, (float*)p.out[1], row0, p.n_i, p.n_j, col0, p.n_j);
+                        write_block(up, st, (float*)p.out[1] + p.n_i * p.n_j, row0, p.n_i, p.n_j, col0, p.n_j);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) g[i] = activate<false>(a.act, g[i]).x * up[i];
+                    write_block(g, st, (T*)p.out[0], row0, p.n_i, p.n_j, col0, p.n_j);
+                } else if (p.splits > 1) {
+                    float* part = p.part + ((int64_t)t.split * p.sets + t.set) * p.n_i * p.n_j;
+                    write_block(g, st, part, row0, p.n_i, p.n_j, col0, p.n_j);
+                } else if (p.out[t.set] != nullptr) {
+                    write_block(g, st, (T*)p.out[t.set], row0, p.n_i, p.n_j, col0, p.n_j);
+                }
+            };
+            const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+            if constexpr (PLANES == 1) {
+                ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, a.polls);
+                tc_fence_after();
+                const uint32_t d = lanes + acc * kAccCols + side * (JW / 2);
+#pragma unroll
+                for (int c = 0; c < kBlocks; ++c) {
+                    float g[32], up[32];
+                    if (ok) {
+                        tmem_ld32(d + c * 32, g);
+                        if (FWD) tmem_ld32(d + BN / 2 + c * 32, up);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) g[i] = up[i] = __uint_as_float(kNaNBits);
+                    }
+                    if (c == kBlocks - 1 && ok) {      // all of this accumulator is in registers or written
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+                    }
+                    emit(c, g, up);
+                }
+                if (++acc == 2) acc = 0, acc_ph ^= 1;
+            } else {
+                constexpr int kSums = FWD ? 2 * kBlocks : kBlocks;
+                float sum[kSums][32];
+#pragma unroll
+                for (int c = 0; c < kSums; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
+                for (int it = t.k0; it < t.k1; it += kFlush) {
+                    ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, a.polls);
+                    tc_fence_after();
+                    if (ok) {
+                        const uint32_t d = lanes + acc * kAccCols + side * (JW / 2);
+#pragma unroll
+                        for (int c = 0; c < kSums; ++c) {
+                            const uint32_t at = d + (FWD && c >= kBlocks ? BN / 2 + (c - kBlocks) * 32 : c * 32);
+                            float lead[32], rest[32];
+                            tmem_ld32(at, lead);
+                            tmem_ld32(at + BN, rest);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[c][i] += lead[i] + rest[i];
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+                    }
+                    if (++acc == 2) acc = 0, acc_ph ^= 1;
+                }
+                if (!ok) {
+#pragma unroll
+                    for (int c = 0; c < kSums; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[c][i] = __uint_as_float(kNaNBits);
+                }
+#pragma unroll
+                for (int c = 0; c < kBlocks; ++c) emit(c, sum[c], sum[FWD ? c + kBlocks : c]);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem, kTmemCols);
+}
+
+}  // namespace cgb200

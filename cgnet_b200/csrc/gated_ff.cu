@@ -9,8 +9,9 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
-#include "row_ops.cuh"
+#include "ff_gemm.cuh"
 
 namespace cgb200 {
 
@@ -25,19 +26,6 @@ struct FfArgs {
     int64_t dh_stride;
     void *dx, *dwg, *dwu;                      // each may be null
 };
-
-// act(g) and its derivative
-template <bool GRAD>
-__device__ __forceinline__ float2 activate(int act, float g) {
-    if (act == CGB200_ACT_RELU) return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);
-    if (act == CGB200_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-g));
-        // where s is 0, g may be -inf
-        return s == 0.f ? make_float2(0.f, 0.f) : make_float2(g * s, GRAD ? s * (1.f + g * (1.f - s)) : 0.f);
-    }
-    const float c = 0.5f * erfcf(-0.70710678118654752f * g);
-    return make_float2(c == 0.f ? 0.f : g * c, GRAD ? c + (fabsf(g) > 20.f ? 0.f : g * __expf(-0.5f * g * g) * 0.39894228040143268f) : 0.f);
-}
 
 // ---- a few rows: one warp per hidden unit, bound by reading the weights ------------------------------------------------
 constexpr int kFfFewRows = 4;
@@ -203,8 +191,324 @@ __global__ void __launch_bounds__(256) ff_tile_bwd_kernel(FfArgs a, int nx, int 
         }
 }
 
+// ---- operands of the tensor-core products ------------------------------------------------------------------------------
+// The tiled copies want rows on 16-byte boundaries and 16-bit values.  A 16-bit matrix that lies so is read where it is; other
+// ones are copied into the workspace first, float32 ones as three bfloat16 planes whose sum is the value.
+struct FfPackOp {
+    const void* src;
+    int64_t stride, rows;
+    int cols;
+    void* dst;             // [planes][rows][pitch]
+    int64_t pitch;
+};
+struct FfPackArgs {
+    FfPackOp op[3];
+};
+__device__ __forceinline__ void split3(float x, float& hi, float& mid, float& lo) {
+    hi = __bfloat162float(__float2bfloat16_rn(x));
+    if (isinf(hi) && !isinf(x)) hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);       // the largest values: rounded towards 0
+    const bool fine = fabsf(hi) < INFINITY;            // an infinity or NaN is its own first part
+    const float r = x - hi;
+    mid = fine ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;
+    lo = fine ? r - mid : 0.f;
+}
 template <typename T>
-static int ff_fwd(const FfArgs& a, cudaStream_t st) {
+__device__ __forceinline__ void store_operand(T* dst, int64_t plane, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(dst) = pack16(v, (const T*)nullptr);
+}
+// float32: dst holds bfloat16 planes
+template <>
+__device__ __forceinline__ void store_operand<float>(float* dst, int64_t plane, const float (&v)[8]) {
+    __nv_bfloat16* d = (__nv_bfloat16*)dst;
+    float hi[8], mid[8], lo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split3(v[i], hi[i], mid[i], lo[i]);
+    *reinterpret_cast<uint4*>(d) = pack16(hi, (const __nv_bfloat16*)nullptr);
+    *reinterpret_cast<uint4*>(d + plane) = pack16(mid, (const __nv_bfloat16*)nullptr);
+    *reinterpret_cast<uint4*>(d + 2 * plane) = pack16(lo, (const __nv_bfloat16*)nullptr);
+}
+// 2-byte slot `i` of an operand buffer, as the pointer type store_operand takes
+template <typename T>
+__device__ __forceinline__ T* operand_at(void* dst, int64_t i) {
+    return (T*)((uint16_t*)dst + i);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) ff_pack_kernel(FfPackArgs a) {
+    const FfPackOp& o = a.op[blockIdx.y];
+    const int64_t chunks = o.pitch / 8, n = o.rows * chunks;
+    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < n; c += (int64_t)gridDim.x * 256) {
+        const int64_t r = c / chunks;
+        const int e0 = (int)(c - r * chunks) * 8;
+        float v[8];
+        load_params<T, 8>((const T*)o.src + r * o.stride, e0, o.cols, v);
+        store_operand<T>(operand_at<T>(o.dst, r * o.pitch + e0), o.rows * o.pitch, v);
+    }
+}
+
+// dg and du, as operands of the products behind them
+template <typename T>
+__global__ void __launch_bounds__(256) ff_dgu_kernel(FfArgs a, void* dg, void* du, int64_t pitch) {
+    const int64_t chunks = pitch / 8, n = a.rows * chunks;
+    const float* g = a.gu;
+    const float* u = a.gu + a.rows * a.hidden;
+    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < n; c += (int64_t)gridDim.x * 256) {
+        const int64_t r = c / chunks;
+        const int e0 = (int)(c - r * chunks) * 8;
+        float gv[8], uv[8], dv[8];
+        load_params<float, 8>(g + r * a.hidden, e0, a.hidden, gv);
+        load_params<float, 8>(u + r * a.hidden, e0, a.hidden, uv);
+        load_params<T, 8>((const T*)a.dh + r * a.dh_stride, e0, a.hidden, dv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = activate<true>(a.act, gv[i]);
+            gv[i] = dv[i] * uv[i] * f.y;
+            uv[i] = dv[i] * f.x;
+        }
+        store_operand<T>(operand_at<T>(dg, r * pitch + e0), a.rows * pitch, gv);
+        store_operand<T>(operand_at<T>(du, r * pitch + e0), a.rows * pitch, uv);
+    }
+}
+
+// Parts of a split contraction, added in order: out[i] = sum over s of part[s][i].
+struct FfReduceArgs {
+    const float* part[2];
+    int splits[2], sets[2];
+    int64_t n[2];                 // values of a set
+    void* out[2][2];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) ff_reduce_kernel(FfReduceArgs a) {
+    const int p = blockIdx.y >> 1, set = blockIdx.y & 1;
+    if (a.splits[p] <= 1 || set >= a.sets[p] || a.out[p][set] == nullptr) return;
+    const float* src = a.part[p] + set * a.n[p];
+    const int64_t step = a.sets[p] * a.n[p];
+    T* out = (T*)a.out[p][set];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n[p]; i += (int64_t)gridDim.x * 256) {
+        float s = src[i];
+        for (int k = 1; k < a.splits[p]; ++k) s += src[k * step + i];
+        out[i] = from_f32<T>(s);
+    }
+}
+
+// ---- which path, and what it needs -------------------------------------------------------------------------------------
+constexpr int64_t kFfTensorWork = 4 << 20;      // rows x dim x hidden from which the tensor cores are used
+
+struct FfPlan {
+    bool tensor;
+    int planes, bn;
+    bool pack[3];                         // x, Wg, Wu
+    int64_t pitch_d, pitch_h;             // of packed operands (dim columns) and of dg, du (hidden columns)
+    int64_t off_pack[3], off_dg, off_du, off_part[2], bytes;
+    int n_problems;
+    FfProblem problem[2];
+};
+
+static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+static bool lies_aligned(const void* p, int64_t stride, int64_t rows, int cols) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows <= 1 ? true : stride >= cols && stride % 8 == 0 && rows * stride * 2 < (1ll << 39));
+}
+
+// `grads`: 0 for the forward, else the sum of 1 (dx), 2 (dWg), 4 (dWu).
+static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
+    FfPlan q{};
+    const bool fwd = grads == 0;
+    const int64_t work = a.rows * a.dim * (int64_t)a.hidden;
+    q.tensor = a.rows > 0 && work >= kFfTensorWork && !(fwd && a.rows <= kFfFewRows);
+    if (!q.tensor) return q;
+    q.planes = dtype == CGB200_F32 ? 3 : 1;
+    const bool need[3] = {true, fwd || (grads & 1), fwd || (grads & 1)};
+    const void* src[3] = {a.x, a.wg, a.wu};
+    const int64_t stride[3] = {a.x_stride, a.wg_stride, a.wu_stride}, rows[3] = {a.rows, a.hidden, a.hidden};
+    q.pitch_d = up(a.dim, 8), q.pitch_h = up(a.hidden, 8);
+    int64_t at = 0;
+    for (int i = 0; i < 3; ++i) {
+        q.pack[i] = need[i] && (i > 0 || fwd || (grads & 6)) && (q.planes == 3 || !lies_aligned(src[i], stride[i], rows[i], a.dim));
+        q.off_pack[i] = at;
+        if (q.pack[i]) at += up(q.planes * rows[i] * q.pitch_d * 2, 256);
+    }
+    if (!fwd) {
+        q.off_dg = at, at += up(q.planes * a.rows * q.pitch_h * 2, 256);
+        q.off_du = at, at += up(q.planes * a.rows * q.pitch_h * 2, 256);
+    }
+    const int64_t ti = (a.rows + kFfBM - 1) / kFfBM;
+    const int hk = (a.hidden + kFfBK - 1) / kFfBK, dk = (a.dim + kFfBK - 1) / kFfBK;
+    const int mk = (int)((a.rows + kFfBK - 1) / kFfBK), th = (a.hidden + kFfBM - 1) / kFfBM;
+    const int w_sets = ((grads & 2) ? 1 : 0) + ((grads & 4) ? 1 : 0);
+    auto units_at = [&](int bn) -> int64_t {
+        if (fwd) return ti * ((a.hidden + bn / 2 - 1) / (bn / 2));
+        const int64_t tj = (a.dim + bn - 1) / bn;
+        return ((grads & 1) ? ti * tj : 0) + (int64_t)w_sets * th * tj;
+    };
+    // wide tiles move less through shared memory; narrow ones fill the SMs where the wide ones do not
+    q.bn = q.planes == 3 || units_at(256) < kNumSM ? 128 : 256;
+    if (fwd) {
+        FfProblem& p = q.problem[q.n_problems++];
+        p.a_map[0] = 0, p.b_map[0] = 1, p.b_map[1] = 2;
+        p.sources = 1, p.kblk = dk, p.sets = 1;
+        p.tiles_i = (int)ti, p.tiles_j = (a.hidden + q.bn / 2 - 1) / (q.bn / 2);
+        p.n_i = a.rows, p.n_j = a.hidden;
+    }
+    if (grads & 1) {
+        FfProblem& p = q.problem[q.n_problems++];
+        p.a_map[0] = 3, p.a_map[1] = 4, p.b_map[0] = 1, p.b_map[1] = 2, p.b_mn = 1;
+        p.sources = 2, p.kblk = hk, p.sets = 1;
+        p.tiles_i = (int)ti, p.tiles_j = (a.dim + q.bn - 1) / q.bn;
+        p.n_i = a.rows, p.n_j = a.dim;
+        p.out[0] = a.dx;
+    }
+    if (w_sets > 0) {
+        FfProblem& p = q.problem[q.n_problems++];
+        p.a_map[0] = (grads & 2) ? 3 : 4, p.a_map[1] = 4, p.b_map[0] = 0, p.a_mn = p.b_mn = 1;
+        p.sources = 1, p.kblk = mk, p.sets = w_sets;
+        p.tiles_i = th, p.tiles_j = (a.dim + q.bn - 1) / q.bn;
+        p.n_i = a.hidden, p.n_j = a.dim;
+        p.out[0] = (grads & 2) ? a.dwg : a.dwu, p.out[1] = a.dwu;
+    }
+    const int64_t units = units_at(q.bn);
+    for (int i = 0; i < q.n_problems; ++i) {
+        FfProblem& p = q.problem[i];
+        const int stages = p.sources * p.kblk;
+        // fewer tiles than SMs: the contraction in parts of at least four stages, added in order afterwards
+        int splits = fwd || units >= kNumSM ? 1 : (int)std::min<int64_t>(8, kNumSM / units);
+        splits = std::max(1, std::min(splits, stages / 4));
+        p.kper = (stages + splits - 1) / splits;
+        p.splits = (stages + p.kper - 1) / p.kper;
+    }
+    if (q.n_problems == 2 && q.problem[1].kper > q.problem[0].kper) std::swap(q.problem[0], q.problem[1]);      // long units first
+    int64_t unit = 0;
+    for (int i = 0; i < q.n_problems; ++i) {
+        FfProblem& p = q.problem[i];
+        p.unit0 = (int)unit;
+        unit += (int64_t)p.sets * p.tiles_i * p.tiles_j * p.splits;
+        q.off_part[i] = at;
+        if (p.splits > 1) at += up((int64_t)p.splits * p.sets * p.n_i * p.n_j * 4, 256);
+    }
+    q.bytes = at;
+    return q;
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+    static std::atomic<void*> fn{nullptr};
+    void* f = fn.load();
+    if (f == nullptr) {
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            return nullptr;
+        fn.store(f);
+    }
+    return (EncodeTiled)f;
+}
+// [planes][rows][pitch] of 16-bit values, read in boxes of 64 rows x 64 columns; what lies outside reads as zero
+static bool ff_map(CUtensorMap* m, EncodeTiled enc, const void* p, int64_t pitch, int64_t rows, int cols, int planes, bool half) {
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)(pitch * 2), (cuuint64_t)((planes > 1 ? rows * pitch : pitch) * 2)};
+    const cuuint32_t box[3] = {64, 64, 1}, step[3] = {1, 1, 1};
+    return enc(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+           CUDA_SUCCESS;
+}
+
+template <int PLANES, int BN, typename T, bool FWD>
+static int ff_gemm_launch(const FfGemmArgs& g, int kid, cudaStream_t st) {
+    auto kern = ff_gemm_kernel<PLANES, BN, T, FWD>;
+    CGB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFfSmem));
+    launch_begin(kid, st);
+    kern<<<(unsigned)std::min(g.units, kNumSM), kFfThreads, kFfSmem, st>>>(g);
+    launch_end(kid, st);
+    CGB_CUDA(cudaGetLastError());
+    return CGB200_OK;
+}
+
+// The tensor-core path of the forward (grads = 0) and of the backward.
+template <typename T>
+static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cudaStream_t st) {
+    constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+    const bool fwd = grads == 0;
+    EncodeTiled enc = encode_tiled();
+    if (enc == nullptr) {
+        set_error("the driver has no cuTensorMapEncodeTiled");
+        return CGB200_ERR_CUDA;
+    }
+    const int kid = fwd ? K_FF_FWD : K_FF_BWD;
+    const void* src[3] = {a.x, a.wg, a.wu};
+    int64_t stride[3] = {a.x_stride, a.wg_stride, a.wu_stride};
+    const int64_t rows[3] = {a.rows, a.hidden, a.hidden};
+    FfPackArgs pack{};
+    int n_pack = 0;
+    int64_t most = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (!q.pack[i]) {
+            if (rows[i] == 1) stride[i] = up(a.dim, 8);       // one row: any distance to the next
+            continue;
+        }
+        pack.op[n_pack++] = FfPackOp{src[i], stride[i], rows[i], a.dim, ws + q.off_pack[i], q.pitch_d};
+        src[i] = ws + q.off_pack[i], stride[i] = q.pitch_d;
+        most = std::max(most, rows[i] * q.pitch_d / 8);
+    }
+    if (n_pack > 0) {
+        launch_begin(kid, st);
+        ff_pack_kernel<T><<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, kNumSM * 16), n_pack), 256, 0, st>>>(pack);
+        launch_end(kid, st);
+        CGB_CUDA(cudaGetLastError());
+    }
+    FfGemmArgs g{};
+    bool ok = true;
+    const bool half = std::is_same<T, __half>::value;
+    for (int i = 0; i < 3; ++i) {
+        const bool used = fwd || (i == 0 ? (grads & 6) != 0 : (grads & 1) != 0);
+        if (used) ok = ok && ff_map(&g.map[i], enc, src[i], stride[i], rows[i], a.dim, PLANES, half);
+    }
+    if (!fwd) {
+        void *dg = ws + q.off_dg, *du = ws + q.off_du;
+        launch_begin(kid, st);
+        ff_dgu_kernel<T><<<(unsigned)std::min<int64_t>((a.rows * q.pitch_h / 8 + 255) / 256, kNumSM * 16), 256, 0, st>>>(a, dg, du, q.pitch_h);
+        launch_end(kid, st);
+        CGB_CUDA(cudaGetLastError());
+        ok = ok && ff_map(&g.map[3], enc, dg, q.pitch_h, a.rows, a.hidden, PLANES, half);
+        ok = ok && ff_map(&g.map[4], enc, du, q.pitch_h, a.rows, a.hidden, PLANES, half);
+    }
+    if (!ok) {
+        set_error("gated feed-forward: an operand's layout was refused by the driver");
+        return CGB200_ERR_CUDA;
+    }
+    g.problems = q.n_problems;
+    for (int i = 0; i < q.n_problems; ++i) {
+        g.p[i] = q.problem[i];
+        g.p[i].part = (float*)(ws + q.off_part[i]);
+        g.units += g.p[i].sets * g.p[i].tiles_i * g.p[i].tiles_j * g.p[i].splits;
+    }
+    if (fwd) g.p[0].out[0] = a.h, g.p[0].out[1] = a.gu;
+    g.idesc_type = half ? 0u : (1u << 7) | (1u << 10);
+    g.act = a.act, g.polls = kDefaultWaitPolls;
+    int rc;
+    if constexpr (PLANES == 3) rc = fwd ? ff_gemm_launch<3, 128, T, true>(g, kid, st) : ff_gemm_launch<3, 128, T, false>(g, kid, st);
+    else if (q.bn == 256) rc = fwd ? ff_gemm_launch<1, 256, T, true>(g, kid, st) : ff_gemm_launch<1, 256, T, false>(g, kid, st);
+    else rc = fwd ? ff_gemm_launch<1, 128, T, true>(g, kid, st) : ff_gemm_launch<1, 128, T, false>(g, kid, st);
+    if (rc != CGB200_OK) return rc;
+    FfReduceArgs r{};
+    bool any = false;
+    int64_t n = 0;
+    for (int i = 0; i < g.problems; ++i) {
+        const FfProblem& p = g.p[i];
+        r.part[i] = p.part, r.splits[i] = p.splits, r.sets[i] = p.sets, r.n[i] = p.n_i * p.n_j;
+        r.out[i][0] = p.out[0], r.out[i][1] = p.out[1];
+        if (p.splits > 1) any = true, n = std::max(n, r.n[i]);
+    }
+    if (any && !fwd) {
+        launch_begin(kid, st);
+        ff_reduce_kernel<T><<<dim3((unsigned)std::min<int64_t>((n + 255) / 256, kNumSM * 8), 4), 256, 0, st>>>(r);
+        launch_end(kid, st);
+        CGB_CUDA(cudaGetLastError());
+    }
+    return CGB200_OK;
+}
+
+template <typename T>
+static int ff_fwd(const FfArgs& a, const FfPlan& q, char* ws, cudaStream_t st) {
+    if (q.tensor) return ff_tensor<T>(a, q, 0, ws, st);
     launch_begin(K_FF_FWD, st);
     if (a.rows <= kFfFewRows) {
         const unsigned grid = (unsigned)((a.hidden + 7) / 8);
@@ -223,7 +527,8 @@ static int ff_fwd(const FfArgs& a, cudaStream_t st) {
 }
 
 template <typename T>
-static int ff_bwd(const FfArgs& a, cudaStream_t st) {
+static int ff_bwd(const FfArgs& a, const FfPlan& q, int grads, char* ws, cudaStream_t st) {
+    if (q.tensor) return ff_tensor<T>(a, q, grads, ws, st);
     const int tiles_d = (a.dim + kFfTile - 1) / kFfTile;
     const int64_t nx = a.dx != nullptr ? (a.rows + kFfTile - 1) / kFfTile * tiles_d : 0;
     const int64_t nw = a.dwg != nullptr || a.dwu != nullptr ? (2 * (int64_t)a.hidden + kFfTile - 1) / kFfTile * tiles_d : 0;
@@ -247,35 +552,49 @@ static int ff_check(const FfArgs& a, int64_t rows, int64_t dim, int64_t hidden, 
     return CGB200_OK;
 }
 
+static int ff_workspace(const FfPlan& q, const void* ws, int64_t bytes) {
+    if (q.bytes > 0 && (ws == nullptr || bytes < q.bytes)) {
+        set_error("workspace too small: need " + std::to_string(q.bytes) + " bytes");
+        return CGB200_ERR_WORKSPACE;
+    }
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, "workspace must be 256-byte aligned");
+    return CGB200_OK;
+}
+
 }  // namespace cgb200
 
 using namespace cgb200;
 
 extern "C" {
 
-int64_t cgb200_gated_ff_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int dtype, int backward) {
-    (void)rows, (void)dim, (void)hidden, (void)dtype, (void)backward;
-    return 0;
+int64_t cgb200_gated_ff_workspace_bytes(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up,
+                                        int64_t w_up_stride, int64_t rows, int64_t dim, int64_t hidden, int dtype, int gradients) {
+    FfArgs a{};
+    a.x = x, a.wg = w_gate, a.wu = w_up, a.x_stride = x_stride, a.wg_stride = w_gate_stride, a.wu_stride = w_up_stride;
+    a.rows = rows, a.dim = (int)dim, a.hidden = (int)hidden;
+    if (ff_check(a, rows, dim, hidden, CGB200_ACT_SILU, dtype) != CGB200_OK) return -1;
+    return ff_plan(a, dtype, gradients & 7).bytes;
 }
 
 int cgb200_gated_ff_fwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
                         int activation, void* h, float* gate_up, int64_t rows, int64_t dim, int64_t hidden, int dtype, void* workspace,
                         int64_t workspace_bytes, void* stream) {
-    (void)workspace, (void)workspace_bytes;
     FfArgs a{};
     a.x = x, a.wg = w_gate, a.wu = w_up, a.x_stride = x_stride, a.wg_stride = w_gate_stride, a.wu_stride = w_up_stride;
     a.rows = rows, a.dim = (int)dim, a.hidden = (int)hidden, a.act = activation, a.h = h, a.gu = gate_up;
     if (int rc = ff_check(a, rows, dim, hidden, activation, dtype)) return rc;
     if (rows == 0) return CGB200_OK;
     CGB_REQUIRE(h != nullptr, "gated feed-forward: null buffer");
+    const FfPlan q = ff_plan(a, dtype, 0);
+    if (int rc = ff_workspace(q, workspace, workspace_bytes)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    return dtype == CGB200_F32 ? ff_fwd<float>(a, st) : dtype == CGB200_BF16 ? ff_fwd<__nv_bfloat16>(a, st) : ff_fwd<__half>(a, st);
+    char* ws = (char*)workspace;
+    return dtype == CGB200_F32 ? ff_fwd<float>(a, q, ws, st) : dtype == CGB200_BF16 ? ff_fwd<__nv_bfloat16>(a, q, ws, st) : ff_fwd<__half>(a, q, ws, st);
 }
 
 int cgb200_gated_ff_bwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
                         int activation, const float* gate_up, const void* dh, int64_t dh_stride, void* dx, void* dw_gate, void* dw_up,
                         int64_t rows, int64_t dim, int64_t hidden, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-    (void)workspace, (void)workspace_bytes;
     FfArgs a{};
     a.x = x, a.wg = w_gate, a.wu = w_up, a.x_stride = x_stride, a.wg_stride = w_gate_stride, a.wu_stride = w_up_stride;
     a.rows = rows, a.dim = (int)dim, a.hidden = (int)hidden, a.act = activation, a.gu = const_cast<float*>(gate_up);
@@ -283,8 +602,14 @@ int cgb200_gated_ff_bwd(const void* x, int64_t x_stride, const void* w_gate, int
     if (int rc = ff_check(a, rows, dim, hidden, activation, dtype)) return rc;
     CGB_REQUIRE(rows == 0 || (gate_up != nullptr && dh != nullptr), "gated feed-forward: null buffer");
     CGB_REQUIRE(dh_stride >= 0 && dh_stride <= (1ll << 32), "gated feed-forward: row stride out of range");
+    const int grads = (dx != nullptr && rows > 0 ? 1 : 0) | (dw_gate != nullptr ? 2 : 0) | (dw_up != nullptr ? 4 : 0);
+    if (grads == 0) return CGB200_OK;
+    const FfPlan q = ff_plan(a, dtype, grads);
+    if (int rc = ff_workspace(q, workspace, workspace_bytes)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    return dtype == CGB200_F32 ? ff_bwd<float>(a, st) : dtype == CGB200_BF16 ? ff_bwd<__nv_bfloat16>(a, st) : ff_bwd<__half>(a, st);
+    char* ws = (char*)workspace;
+    return dtype == CGB200_F32 ? ff_bwd<float>(a, q, grads, ws, st) : dtype == CGB200_BF16 ? ff_bwd<__nv_bfloat16>(a, q, grads, ws, st)
+                                                                                         : ff_bwd<__half>(a, q, grads, ws, st);
 }
 
 }  // extern "C"

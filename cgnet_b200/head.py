@@ -181,9 +181,10 @@ def _gated_ff_fwd(x2, wg, wu, act, keep):
     dev, dtype = x2.device, _DTYPES[x2.dtype]
     h = torch.empty(rows, hidden, dtype=x2.dtype, device=dev)
     gate_up = torch.empty(2, rows, hidden, dtype=torch.float32, device=dev) if keep else None
-    n = _lib.load().cgb200_gated_ff_workspace_bytes(rows, dim, hidden, dtype, 0)
+    operands = (x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
+    n = _lib.load().cgb200_gated_ff_workspace_bytes(*operands, rows, dim, hidden, dtype, 0)
     ws = _workspace(n, dev)
-    _call("cgb200_gated_ff_fwd", dev, x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), act, h.data_ptr(),
+    _call("cgb200_gated_ff_fwd", dev, *operands, act, h.data_ptr(),
           _ptr(gate_up), rows, dim, hidden, dtype, _ptr(ws), n)
     return h, gate_up
 
@@ -208,10 +209,10 @@ class _GatedFeedForward(torch.autograd.Function):
         dx = torch.empty(rows, dim, dtype=x2.dtype, device=dev) if need[0] else None
         dwg = torch.empty(hidden, dim, dtype=x2.dtype, device=dev) if need[1] else None
         dwu = torch.empty(hidden, dim, dtype=x2.dtype, device=dev) if need[2] else None
-        n = _lib.load().cgb200_gated_ff_workspace_bytes(rows, dim, hidden, dtype, 1)
+        operands = (x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
+        n = _lib.load().cgb200_gated_ff_workspace_bytes(*operands, rows, dim, hidden, dtype, bool(need[0]) + 2 * bool(need[1]) + 4 * bool(need[2]))
         ws = _workspace(n, dev)
-        _call("cgb200_gated_ff_bwd", dev, x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ctx.act,
-              gate_up.data_ptr(), dh.data_ptr(), dh.stride(0), _ptr(dx), _ptr(dwg), _ptr(dwu), rows, dim, hidden, dtype, _ptr(ws), n)
+        _call("cgb200_gated_ff_bwd", dev, *operands, ctx.act, gate_up.data_ptr(), dh.data_ptr(), dh.stride(0), _ptr(dx), _ptr(dwg), _ptr(dwu), rows, dim, hidden, dtype, _ptr(ws), n)
         return dx, dwg, dwu, None
 
 

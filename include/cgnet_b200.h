@@ -307,13 +307,17 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
  *   h         [rows][hidden], contiguous
  *   gate_up   float[2][rows][hidden]: the two projections, for the backward; NULL where none follows
  * Backward: dx [rows][dim], dw_gate and dw_up [hidden][dim], each NULL where it is not wanted; with 0 rows it writes zeros to
- * the weights' gradients.  workspace: cgb200_gated_ff_workspace_bytes(..., backward = 0 or 1) bytes, 256-byte aligned, contents
- * undefined; one workspace serves one call at a time.
+ * the weights' gradients.  workspace: cgb200_gated_ff_workspace_bytes bytes (`gradients` = 0 for the forward, else the sum of 1 for
+ * dx, 2 for dw_gate and 4 for dw_up, as the call asks for them; the operands' addresses and strides decide whether they have to
+ * be copied), 256-byte aligned, contents undefined; one workspace serves one call at a time.
+ * Small products run on the CUDA cores, others on the tensor cores (float32 in three bfloat16 parts, accurate to float32).  A row of
+ * x that is not finite spoils that row of h and dx; in float32 it may come out as NaN where the formula gives an infinity.
  */
 #define CGB200_ACT_SILU         0   /* g / (1 + exp(-g))                  */
 #define CGB200_ACT_GELU         1   /* g * (1 + erf(g / sqrt 2)) / 2      */
 #define CGB200_ACT_RELU         2   /* max(g, 0)                          */
-int64_t cgb200_gated_ff_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int dtype, int backward);
+int64_t cgb200_gated_ff_workspace_bytes(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up,
+                                        int64_t w_up_stride, int64_t rows, int64_t dim, int64_t hidden, int dtype, int gradients);
 int cgb200_gated_ff_fwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
                         int activation, void* h, float* gate_up, int64_t rows, int64_t dim, int64_t hidden, int dtype, void* workspace,
                         int64_t workspace_bytes, void* stream);
