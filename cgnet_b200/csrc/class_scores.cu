@@ -5,11 +5,14 @@
 // where a = (z - r) c, c = log2(e) / T.  From the joined (r, s, e) of a row
 //     log p(j) = ln 2 ((z_j - r) c - log2 s),     H = ln 2 (log2 s - e / s).
 // The difference is taken before the product: scores masked by the type's lowest value would overflow z c.  The backward passes
-// read (r, 1 / s): p = 2^((z - r) c) / s carries no rounding of a stored logarithm.
+// read (r, 1 / s): p = 2^((z - r) c) / s carries no rounding of a stored logarithm.  r follows the largest score only when that
+// is more than 2^kScMargin ahead: sums and products are in floating point, so a reference a little below the maximum is as exact,
+// and almost no chunk after the first has to rescale.
 #include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "row_ops.cuh"
 
@@ -22,6 +25,8 @@ constexpr int kScUnroll = 4;                     // chunks a thread has in fligh
 constexpr int kScCap = 4096;                     // candidates a block collects before it has to fall back
 constexpr int kScMaxTop = 128;                   // kScMaxTop threads' chunks of the first tile always fit the candidates
 constexpr int kScWarpValues = 32;                // values per lane of the kernel for short rows
+constexpr float kScMargin = 10.f;
+constexpr int kScPickKeys = 512;                 // candidates a warp searches in registers
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
 static_assert(kScMaxTop * kScUnroll * 8 <= kScCap, "the first tile's candidates must fit");
@@ -33,7 +38,7 @@ struct ScoreArgs {
     int64_t z_stride, rows;
     int classes;
     float scale;               // log2(e) / temperature
-    float2* stats;             // (r, 1 / s) per row; may be null
+    float2* stats;             // (r, 1 / s) per row, distillation: (r, 1 / s, tmax, 1 / sum of weights); may be null
     // log probabilities
     const int64_t* targets;    // may be null
     float *log_prob, *entropy;
@@ -45,6 +50,7 @@ struct ScoreArgs {
     const void* t_scores;      // [rows][n_t]
     int n_t, t_dtype;
     float temperature;
+    double inv_temperature;
     float* loss;
 };
 
@@ -61,77 +67,103 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
 
 // Order of the ranked classes as one integer: score, then index downwards.  NaN ranks highest, -0 equals +0.
 __device__ __forceinline__ uint32_t order_of(float z) {
-    if (z != z) return 0xffffffffu;
+    if (z != z) return 0xfffffffeu;        // below the largest integer, which no key may be
     const uint32_t b = __float_as_uint(z + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float score_of(uint32_t o) {
-    if (o == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+    if (o == 0xfffffffeu) return __uint_as_float(0x7fffffffu);
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ uint64_t key_of(float z, uint32_t idx) { return ((uint64_t)order_of(z) << 32) | (0xffffffffu - idx); }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
-// Running statistics of a row, or of a part of one.
+// Two float32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+// Statistics of a row, or of a part of one, joined: reference, sums relative to it; m is r, or -inf where there is no score yet.
 struct Stat {
-    float m, r, s, e;    // largest score, the reference (the same, but 0 while m is -inf), sums relative to r
-    __device__ __forceinline__ void clear() { m = -INFINITY, r = 0.f, s = 0.f, e = 0.f; }
+    float m, r, s, e;
+};
+// The running form of one thread: sums of even and odd places side by side.
+struct RunStat {
+    float r, limit, margin;      // a chunk whose largest score is above `limit` moves the reference
+    uint64_t s, e;
+    __device__ __forceinline__ explicit RunStat(float scale) : r(0.f), limit(-INFINITY), margin(kScMargin / scale), s(0), e(0) {}
     __device__ __forceinline__ void raise(float nm, float scale) {
-                if (m == -INFINITY) {
-            s *= 0.f, e *= 0.f;      // nothing so far, or a NaN, which stays
+        if (limit == -INFINITY) {
+            const uint64_t zero = pair(0.f, 0.f);
+            s = mul2(s, zero), e = mul2(e, zero);      // nothing so far, or a NaN, which stays
         } else {
             const float d = fmaxf((r - nm) * scale, -1e5f), f = ex2(d);
-            e = f * (e + s * d);
-            s *= f;
+            const uint64_t f2 = pair(f, f);
+            e = mul2(f2, fma2(s, pair(d, d), e));
+            s = mul2(f2, s);
         }
-        m = nm, r = nm;
+        r = nm, limit = nm + margin;
     }
     template <int N, bool ENT>
     __device__ __forceinline__ void add(const float (&v)[N], float cm, float scale) {
-        if (cm > m) raise(cm, scale);
+        if (cm > limit) raise(cm, scale);
+        const uint64_t r2 = pair(-r, -r), c2 = pair(scale, scale);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float a = (v[i] - r) * scale;
-            const float p = ex2(a);
-            s += p;
-            if (ENT) e = fmaf(p, fmaxf(a, -1e5f), e);     // p is 0 there: the bound keeps 0 * -inf out
+        for (int i = 0; i < N; i += 2) {
+            const float2 a = unpair(mul2(add2(pair(v[i], v[i + 1]), r2), c2));
+            const uint64_t p = pair(ex2(a.x), ex2(a.y));
+            s = add2(s, p);
+            if (ENT) e = fma2(p, pair(fmaxf(a.x, -1e5f), fmaxf(a.y, -1e5f)), e);     // p is 0 there: the bound keeps 0 * -inf out
         }
     }
-    __device__ __forceinline__ void join(const Stat& o, float scale) {
-        if (!(o.m > -INFINITY)) {             // nothing there, unless it holds a NaN
-            s += o.s, e += o.e;
-            return;
-        }
-        if (!(m > -INFINITY)) {
-            const float s0 = s, e0 = e;
-            *this = o;
-            s += s0, e += e0;
-            return;
-        }
-        const bool up = o.r > r;
-        const float nr = up ? o.r : r;
-        const float da = fmaxf((r - nr) * scale, -1e5f), db = fmaxf((o.r - nr) * scale, -1e5f), fa = ex2(da), fb = ex2(db);
-        e = fa * (e + s * da) + fb * (o.e + o.s * db);
-        s = fa * s + fb * o.s;
-        m = up ? o.m : m, r = nr;
-    }
-    __device__ __forceinline__ Stat shfl_xor(int o) const {
-        Stat x;
-        x.m = __shfl_xor_sync(0xffffffffu, m, o), x.r = __shfl_xor_sync(0xffffffffu, r, o);
-        x.s = __shfl_xor_sync(0xffffffffu, s, o), x.e = __shfl_xor_sync(0xffffffffu, e, o);
-        return x;
+    __device__ __forceinline__ Stat stat() const {
+        const float2 a = unpair(s), b = unpair(e);
+        return Stat{limit == -INFINITY ? -INFINITY : r, r, a.x + a.y, b.x + b.y};
     }
 };
+// Joined over a warp, the same bits in every lane: one common reference, each lane's sums rescaled to it once, then added.  A lane
+// without a score (m = -inf) has sums of 0, or NaN, which stays.
 __device__ __forceinline__ Stat warp_join(Stat a, float scale) {
+    float m = a.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stat b = a.shfl_xor(o);
-        // both lanes of a pair join in the same order, so that all lanes end with the same bits
-        Stat lo = (threadIdx.x & o) ? b : a;
-        lo.join((threadIdx.x & o) ? a : b, scale);
-        a = lo;
-    }
-    return a;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float r = m == -INFINITY ? 0.f : m;
+    const float d = a.m == -INFINITY ? 0.f : fmaxf((a.r - r) * scale, -1e5f), f = ex2(d);
+    return Stat{m, r, warp_sum(a.s * f), warp_sum(f * (a.e + a.s * d))};
+}
+// Largest value of a chunk, NaN if one is.
+__device__ __forceinline__ float chunk_max(const uint4& u, const float*) {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+template <typename T>
+__device__ __forceinline__ float chunk_max(const uint4& u, const T*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type h[4];
+    memcpy(h, w, 16);
+    const auto m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(to_f32(m.x), to_f32(m.y));
 }
 // A row of nothing but -inf has no distribution: log probabilities -inf, entropy 0, gradients 0.
 __device__ __forceinline__ bool empty_row(const Stat& a) { return a.m == -INFINITY && a.s == 0.f; }
@@ -147,7 +179,7 @@ __device__ __forceinline__ float load_score(const void* p, int dtype, int64_t i)
 }
 
 // ---- teacher's side of a row ---------------------------------------------------------------------------------------
-// Sums over the threads that share a row: a warp (buf unused) or the block.
+// Joined over the threads that share a row: a warp (buf unused) or the block.
 __device__ __forceinline__ double row_sum_d(double v, double* buf, bool whole_block) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -163,62 +195,74 @@ __device__ __forceinline__ float row_max_f(float v, double* buf, bool whole_bloc
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (!whole_block) return v;
+    float* f = (float*)buf;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) f[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (float)buf[0];
-    for (int i = 1; i < (int)(blockDim.x >> 5); ++i) v = fmaxf(v, (float)buf[i]);
+    v = f[0];
+    for (int i = 1; i < (int)(blockDim.x >> 5); ++i) v = fmaxf(v, f[i]);
     return v;
 }
-// Teacher's distribution over the classes it names: q(k) = exp(t_k / T - tmax / T) / sum.  Entries with a negative class are
-// not there; a class beyond the last makes the row NaN.
-struct Teacher {
-    float tmax;
-    double sum;
-    bool any;
+// One entry: class (-1: not there, or of weight 0 for lack of a class beyond the last, which `bad` tells), teacher's score and
+// student's score.
+struct Entry {
+    int id;
+    bool bad;
+    float t, z;
 };
-__device__ __forceinline__ Teacher teacher_of(const ScoreArgs& a, int64_t row, int t, int G, double* buf, bool whole_block) {
-    const int64_t at = row * a.n_t;
-    float mx = -INFINITY, some = 0.f;
-    for (int k = t; k < a.n_t; k += G) {
-        if (a.t_ids[at + k] < 0) continue;
-        const float v = load_score(a.t_scores, a.t_dtype, at + k);
+template <typename T>
+__device__ __forceinline__ Entry entry_of(const ScoreArgs& a, int64_t row, const T* zr, int k) {
+    Entry e{-1, false, -INFINITY, 0.f};
+    if (k >= a.n_t) return e;
+    const int64_t id = a.t_ids[row * a.n_t + k];
+    if (id < 0) return e;
+    e.t = load_score(a.t_scores, a.t_dtype, row * a.n_t + k);
+    e.bad = id >= a.classes;
+    if (!e.bad) e.id = (int)id, e.z = to_f32(zr[id]);
+    return e;
+}
+// Weight of an entry before the division by the sum of all: exp((t - tmax) / T).
+__device__ __forceinline__ float weight_of(const ScoreArgs& a, float t, float tmax) {
+    return expf((float)(((double)t - (double)tmax) * a.inv_temperature));
+}
+// Loss of a row from its statistics; `first` is this thread's first entry, fetched while the row was read.  Leaves what the
+// backward needs of the teacher, (tmax, 1 / sum of weights), 1 / sum = 0 for a row without entries.
+template <typename T>
+__device__ __forceinline__ float distill_loss(const ScoreArgs& a, int64_t row, const T* zr, const Stat& st, const Entry& first, int t, int G,
+                                              double* buf, bool whole_block, float2& teacher) {
+    float mx = first.t, some = first.t != -INFINITY ? 1.f : 0.f;      // a NaN counts as an entry
+    for (int k = t + G; k < a.n_t; k += G) {
+        const float v = a.t_ids[row * a.n_t + k] < 0 ? -INFINITY : load_score(a.t_scores, a.t_dtype, row * a.n_t + k);
         if (v != -INFINITY) some = 1.f;
         mx = fmaxf(mx, v);
     }
-    Teacher q;
-    q.any = row_max_f(some, buf, whole_block) > 0.f;
-    q.tmax = row_max_f(mx, buf, whole_block);
-    double s = 0.0;
-    for (int k = t; k < a.n_t; k += G) {
-        const int64_t id = a.t_ids[at + k];
-        if (id < 0) continue;
-        s += id < a.classes ? exp(((double)load_score(a.t_scores, a.t_dtype, at + k) - (double)q.tmax) / (double)a.temperature) : nan("");
+    const bool any = row_max_f(some, buf, whole_block) > 0.f;       // the same in all threads of the row
+    if (!any) {
+        teacher = make_float2(0.f, 0.f);
+        return 0.f;
     }
-    q.sum = q.any ? row_sum_d(s, buf, whole_block) : 1.0;     // `any` is the same in all threads of the row
-    return q;
-}
-template <typename T>
-__device__ __forceinline__ float distill_loss(const ScoreArgs& a, int64_t row, const T* zr, const Stat& st, int t, int G, double* buf,
-                                              bool whole_block) {
-    const Teacher q = teacher_of(a, row, t, G, buf, whole_block);
-    if (!q.any) return 0.f;
-    const int64_t at = row * a.n_t;
-    const double log_sum = log(q.sum), log2_s = log2((double)st.s);
-    double acc = 0.0;
-    for (int k = t; k < a.n_t; k += G) {
-        const int64_t id = a.t_ids[at + k];
-        if (id < 0 || id >= a.classes) continue;
-        const double lt = ((double)load_score(a.t_scores, a.t_dtype, at + k) - (double)q.tmax) / (double)a.temperature;
-        const double w = exp(lt) / q.sum;
-        if (w == 0.0) continue;
-        const double lp = empty_row(st) ? -INFINITY : kLn2 * (((double)to_f32(zr[id]) - (double)st.r) * (double)a.scale - log2_s);
-        acc += w * (lt - log_sum - lp);
+    const float tmax = row_max_f(mx, buf, whole_block);
+    // sum of w, and of w (log w - log p) with log p = ln 2 ((z - r) c - log2 s)
+    const double log2_s = log2((double)st.s);
+    const bool empty = empty_row(st);
+    double sum = 0.0, acc = 0.0;
+    Entry e = first;
+    for (int k = t;;) {
+        if (e.bad) sum += nan("");
+        if (e.id >= 0) {
+            const float w = weight_of(a, e.t, tmax);
+            const double lp = empty ? -INFINITY : kLn2 * (((double)e.z - (double)st.r) * (double)a.scale - log2_s);
+            sum += w;
+            if (w != 0.f) acc += (double)w * (((double)e.t - (double)tmax) * a.inv_temperature - lp);
+        }
+        k += G;
+        if (k >= a.n_t) break;
+        e = entry_of(a, row, zr, k);
     }
+    sum = row_sum_d(sum, buf, whole_block);
     acc = row_sum_d(acc, buf, whole_block);
-    // a NaN of the sum (a class beyond the last) is in log_sum even where no entry was added
-    if (q.sum != q.sum) acc = q.sum;
-    return (float)((double)a.temperature * (double)a.temperature * acc);
+    teacher = make_float2(tmax, (float)(1.0 / sum));
+    return (float)((double)a.temperature * (double)a.temperature * (acc / sum - log(sum)));
 }
 
 // ---- rows a warp holds in registers --------------------------------------------------------------------------------
@@ -230,25 +274,29 @@ __global__ void __launch_bounds__(kScThreads) scores_warp_kernel(ScoreArgs a) {
     if (row >= a.rows) return;       // whole warps leave; nothing below is wider than a warp
     const T* zr = (const T*)a.z + row * a.z_stride;
     const int ph = row_phase(zr);
+    uint4 raw[CH];
     float v[CH][N];
-    Stat st;
-    st.clear();
+#pragma unroll
+    for (int c = 0; c < CH; ++c) raw[c] = load_raw(zr, (lane + 32 * c) * N - ph, a.classes, -INFINITY);
+    Entry first{};
+    if (MODE == kDistill) first = entry_of(a, row, zr, lane);
+    RunStat run(a.scale);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e0 = (lane + 32 * c) * N - ph;
-        load_chunk(zr, e0, a.classes, -INFINITY, v[c]);
-        float cm = v[c][0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) cm = max_nan(cm, v[c][i]);
-        st.add<N, MODE == kLogProbs>(v[c], cm, a.scale);
+        unpack16(raw[c], v[c], (const T*)nullptr);
+        run.add<N, MODE == kLogProbs>(v[c], chunk_max(raw[c], (const T*)nullptr), a.scale);
     }
-    st = warp_join(st, a.scale);
-    if (a.stats != nullptr && lane == 0) a.stats[row] = make_float2(st.r, empty_row(st) ? 0.f : 1.f / st.s);
+    const Stat st = warp_join(run.stat(), a.scale);
     if (MODE == kDistill) {
-        const float loss = distill_loss(a, row, zr, st, lane, 32, nullptr, false);
-        if (lane == 0) a.loss[row] = loss;
+        float2 teacher;
+        const float loss = distill_loss(a, row, zr, st, first, lane, 32, nullptr, false, teacher);
+        if (lane == 0) {
+            a.loss[row] = loss;
+            if (a.stats != nullptr) ((float4*)a.stats)[row] = make_float4(st.r, empty_row(st) ? 0.f : 1.f / st.s, teacher.x, teacher.y);
+        }
         return;
     }
+    if (a.stats != nullptr && lane == 0) a.stats[row] = make_float2(st.r, empty_row(st) ? 0.f : 1.f / st.s);
     const double log2_s = log2((double)st.s);
     if (lane == 0) {
         a.entropy[row] = empty_row(st) ? 0.f : (float)(kLn2 * (log2_s - (double)st.e / (double)st.s));
@@ -284,18 +332,18 @@ __global__ void __launch_bounds__(kScThreads) scores_warp_kernel(ScoreArgs a) {
 }
 
 // ---- long rows: a block, or a cluster of blocks, per row -------------------------------------------------------------
-struct ScoreShared {
-    uint64_t buf[kScCap];          // candidates
-    uint64_t best[kScMaxTop];      // this block's best, in order
+struct ScoreBase {
     Stat part[kScThreads / 32];
     Stat stat;
-    float tmax[kScThreads];
+    double red[kScThreads / 32];
+};
+struct ScoreShared : ScoreBase {
+    uint64_t buf[kScCap];          // candidates
+    uint64_t best[kScMaxTop];      // this block's best, in order
     unsigned hist[256];
-    int count, n_best;
-    float thr;
+    int count, kept, n_best;
     uint64_t prefix;
     unsigned want;
-    double red[kScThreads / 32];
 };
 
 __device__ __forceinline__ void push(ScoreShared& sh, uint64_t key) {
@@ -303,14 +351,63 @@ __device__ __forceinline__ void push(ScoreShared& sh, uint64_t key) {
     if (at < kScCap) sh.buf[at] = key;
 }
 
+// The scores of a chunk that are not below thr (`strict`: above it) become candidates.  Rare and kept out of line: inlined into the
+// unrolled loop it outgrew the instruction cache.
+template <typename T>
+__device__ __noinline__ void push_chunk(ScoreShared& sh, uint4 raw, int e0, float thr, bool strict) {
+    constexpr int N = Chunk<T>::N;
+    float v[N];
+    unpack16(raw, v, (const T*)nullptr);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (!(v[i] < thr) && v[i] != -INFINITY && !(strict && v[i] == thr)) push(sh, key_of(v[i], (uint32_t)(e0 + i)));
+}
+
+// Largest t, in its upper 16 bits, that at least k of n <= kScPickKeys orders in shared memory (`step` words apart) reach; by the block's
+// first warp, 16 halvings on registers.  0 where n < k.
+__device__ __forceinline__ uint32_t kth_order(const uint32_t* v, int step, int n, int k) {
+    uint32_t own[kScPickKeys / 32];
+#pragma unroll
+    for (int j = 0; j < kScPickKeys / 32; ++j) {
+        const int i = threadIdx.x + 32 * j;
+        own[j] = i < n ? v[i * step] : 0u;
+    }
+    uint32_t t = 0;
+    const int groups = (n + 31) / 32;
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < kScPickKeys / 32; ++j)
+            if (j < groups) c += own[j] >= (t | bit);
+        if (__reduce_add_sync(0xffffffffu, c) >= k) t |= bit;
+    }
+    return t;
+}
 // The `k` highest of the first n candidates, in order, to sh.best (n_best of them).  All keys differ, so their order
 // does not depend on the order in which they were collected.
 __device__ void select_best(ScoreShared& sh, int n, int k) {
-    if (n <= 512) {
-        for (int i = threadIdx.x; i < n; i += kScThreads) {
-            const uint64_t key = sh.buf[i];
+    if (n <= kScPickKeys) {
+        uint64_t* keys = sh.buf;
+        int m = n;
+        if (n > 64 && n > k) {
+            // first down to those of the k-th one's order or above
+            if (threadIdx.x < 32) {
+                const uint32_t t = kth_order((const uint32_t*)sh.buf + 1, 2, n, k);
+                if (threadIdx.x == 0) sh.want = t, sh.kept = 0;
+            }
+            __syncthreads();
+            const uint32_t t = sh.want;
+            keys = sh.buf + kScPickKeys;
+            for (int i = threadIdx.x; i < n; i += kScThreads)
+                if ((uint32_t)(sh.buf[i] >> 32) >= t) keys[atomicAdd(&sh.kept, 1)] = sh.buf[i];
+            __syncthreads();
+            m = sh.kept;
+        }
+        for (int i = threadIdx.x; i < m; i += kScThreads) {
+            const uint64_t key = keys[i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += sh.buf[j] > key;
+#pragma unroll 4
+            for (int j = 0; j < m; ++j) rank += keys[j] > key;
             if (rank < k) sh.best[rank] = key;
         }
     } else {
@@ -388,10 +485,11 @@ __device__ void radix_collect(ScoreShared& sh, const T* zr, int ph, int c0, int 
 }
 
 template <typename T, int MODE, bool CLUSTER>
-__global__ void __launch_bounds__(kScThreads) scores_row_kernel(ScoreArgs a, int blocks_per_row) {
+__global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_row_kernel(ScoreArgs a, int blocks_per_row) {
     constexpr int N = Chunk<T>::N;
     constexpr bool ENT = MODE == kLogProbs;
-    __shared__ ScoreShared sh;
+    constexpr int kTile = kScThreads * kScUnroll;
+    __shared__ typename std::conditional<ENT, ScoreShared, ScoreBase>::type sh;
     const int part = CLUSTER ? (int)(blockIdx.x % (unsigned)blocks_per_row) : 0;
     const int64_t row = CLUSTER ? (int64_t)(blockIdx.x / (unsigned)blocks_per_row) : (int64_t)blockIdx.x;
     const T* zr = (const T*)a.z + row * a.z_stride;
@@ -399,140 +497,166 @@ __global__ void __launch_bounds__(kScThreads) scores_row_kernel(ScoreArgs a, int
     const int nc = (a.classes + ph + N - 1) / N;
     const int per = CLUSTER ? (nc + blocks_per_row - 1) / blocks_per_row : nc;
     const int c0 = min(nc, part * per), c1 = min(nc, c0 + per);
-    const int full0 = ph > 0 ? 1 : 0, full1 = (a.classes + ph) / N;     // chunks [full0, full1) lie inside the row
     const int first = max(0, c0 * N - ph), behind = min(a.classes, c1 * N - ph);   // this block's classes
     const bool tops = ENT && a.top > 0;
     const int want = tops ? min(a.top, max(0, behind - first)) : 0;      // entries it has to offer
-    if (threadIdx.x == 0) sh.count = 0;
-    Stat st;
-    st.clear();
-    float thr = INFINITY;
-    for (int base = c0; base < c1; base += kScThreads * kScUnroll) {
+    if constexpr (ENT) {
+        if (threadIdx.x == 0) sh.count = 0;
+    }
+    RunStat run(a.scale);
+    float thr = -INFINITY;
+    // Chunks [f0, f1) lie inside the row; what is left at its two ends is one chunk each.
+    const int f0 = c0 == 0 && ph > 0 ? 1 : c0, f1 = max(f0, min(c1, (a.classes + ph) / N));
+    const uint4* src = reinterpret_cast<const uint4*>(zr - ph) + f0 + threadIdx.x;
+    const uint4 none = load_raw(zr, 0, 0, -INFINITY);
+    Entry entry{};
+    if (!ENT && part == 0) entry = entry_of(a, row, zr, (int)threadIdx.x);
+    for (int base = f0; base < f1; base += kTile) {
         uint4 raw[kScUnroll];
-        const bool inside = base >= full0 && base + kScThreads * kScUnroll <= min(c1, full1);
-        if (inside) {
+        if (base + kTile <= f1) {
 #pragma unroll
-            for (int u = 0; u < kScUnroll; ++u)
-                raw[u] = *reinterpret_cast<const uint4*>(zr + ((int64_t)(base + u * kScThreads + (int)threadIdx.x) * N - ph));
+            for (int u = 0; u < kScUnroll; ++u) raw[u] = src[u * kScThreads];
         } else {
 #pragma unroll
-            for (int u = 0; u < kScUnroll; ++u) {
-                const int c = base + u * kScThreads + (int)threadIdx.x;
-                float v[N];
-                load_chunk(zr, (int64_t)c * N - ph, c < c1 ? a.classes : 0, -INFINITY, v);
-                raw[u] = pack16(v, (const T*)nullptr);       // the values came from this type: nothing is rounded
-            }
+            for (int u = 0; u < kScUnroll; ++u) raw[u] = base + u * kScThreads + (int)threadIdx.x < f1 ? src[u * kScThreads] : none;
         }
+        src += kTile;
         float tm = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kScUnroll; ++u) {
             float v[N];
             unpack16(raw[u], v, (const T*)nullptr);
-            float cm = v[0];
-#pragma unroll
-            for (int i = 1; i < N; ++i) cm = max_nan(cm, v[i]);
-            st.add<N, ENT>(v, cm, a.scale);
-            tm = fmaxf(tm, cm);
-            if (tops && base != c0 && !(cm <= thr)) {
-                const int e0 = (base + u * kScThreads + (int)threadIdx.x) * N - ph;
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (!(v[i] <= thr)) push(sh, key_of(v[i], (uint32_t)(e0 + i)));
+            const float cm = chunk_max(raw[u], (const T*)nullptr);
+            run.add<N, ENT>(v, cm, a.scale);
+            if constexpr (ENT) {
+                tm = fmaxf(tm, cm);
+                if (tops && base != f0 && !(cm <= thr)) push_chunk<T>(sh, raw[u], (base + u * kScThreads + (int)threadIdx.x) * N - ph, thr, true);
             }
         }
-        if (tops && base == c0) {
-            // Threshold: at least `top` threads of the first tile hold a score of at least the top-th highest of the threads'
-            // maxima, so nothing below it can rank, and nothing equal to it further right.
-            sh.tmax[threadIdx.x] = tm;
-            __syncthreads();
-            int above = 0, same = 0;
-            for (int j = 0; j < kScThreads; ++j) {
-                const float o = sh.tmax[j];
-                above += o > tm;
-                same += o == tm && j < (int)threadIdx.x;
-            }
-            if (above + same == a.top - 1) sh.thr = tm;
-            __syncthreads();
-            thr = sh.thr;
+        if constexpr (ENT) {
+            if (tops && base == f0) {
+                // Threshold: the largest value (to the upper 16 bits of its order) that at least `top` threads' maxima of the first
+                // tile reach: nothing below it can rank, and nothing equal to it further right.
+                uint32_t* maxima = (uint32_t*)sh.hist;
+                maxima[threadIdx.x] = order_of(tm);
+                __syncthreads();
+                if (threadIdx.x < 32) {
+                    const uint32_t t = kth_order(maxima, 1, kScThreads, a.top);
+                    if (threadIdx.x == 0) sh.want = t;
+                }
+                __syncthreads();
+                const uint32_t t = sh.want;
+                thr = t <= order_of(-INFINITY) ? -INFINITY : score_of(t);
 #pragma unroll
-            for (int u = 0; u < kScUnroll; ++u) {
-                const int e0 = (base + u * kScThreads + (int)threadIdx.x) * N - ph;
-                float v[N];
-                unpack16(raw[u], v, (const T*)nullptr);
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (!(v[i] < thr) && v[i] != -INFINITY) push(sh, key_of(v[i], (uint32_t)(e0 + i)));
+                for (int u = 0; u < kScUnroll; ++u)
+                    if (!(chunk_max(raw[u], (const T*)nullptr) < thr))
+                        push_chunk<T>(sh, raw[u], (base + u * kScThreads + (int)threadIdx.x) * N - ph, thr, false);
             }
         }
     }
+    if (threadIdx.x < 2) {
+        // the ends: thread 0 the first chunk, thread 1 the last
+        const int c = threadIdx.x == 0 ? c0 : f1;
+        if (threadIdx.x == 0 ? c0 < f0 : f1 < c1) {
+            const uint4 end = load_raw(zr, (int64_t)c * N - ph, a.classes, -INFINITY);
+            float v[N];
+            unpack16(end, v, (const T*)nullptr);
+            run.add<N, ENT>(v, chunk_max(end, (const T*)nullptr), a.scale);
+            if constexpr (ENT) {
+                if (tops) push_chunk<T>(sh, end, c * N - ph, thr, false);
+            }
+        }
+    }
+    Stat st = run.stat();
     st = warp_join(st, a.scale);
     if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = st;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kScThreads / 32; ++w) st.join(sh.part[w], a.scale);
-        sh.stat = st;
+    if (threadIdx.x < 32) {
+        st = warp_join(threadIdx.x < kScThreads / 32 ? sh.part[threadIdx.x] : Stat{-INFINITY, 0.f, 0.f, 0.f}, a.scale);
+        if (threadIdx.x == 0) sh.stat = st;
     }
-    if (tops) {
-        int n = sh.count;
-        if (n > kScCap) {
-            radix_collect(sh, zr, ph, c0, c1, a.classes, want);
-            n = sh.count;
-        } else if (n < want) {
-            // fewer scores than places: masked classes follow, lowest index first
-            if (threadIdx.x == 0)
-                for (int e = first; e < behind && n < want; ++e)
-                    if (to_f32(zr[e]) == -INFINITY) sh.buf[n++] = key_of(-INFINITY, (uint32_t)e);
-            n = want;
-            __syncthreads();
+    if constexpr (ENT) {
+        if (tops) {
+            int n = sh.count;
+            if (n > kScCap) {
+                radix_collect(sh, zr, ph, c0, c1, a.classes, want);
+                n = sh.count;
+            } else if (n < want) {
+                // fewer scores than places: masked classes follow, lowest index first
+                if (threadIdx.x < 32) {
+                    int have = n;
+                    for (int e = first; e < behind && have < want; e += 32) {
+                        const int at = e + (int)threadIdx.x;
+                        const bool masked = at < behind && to_f32(zr[at]) == -INFINITY;
+                        const unsigned votes = __ballot_sync(0xffffffffu, masked);
+                        const int place = have + __popc(votes & ((1u << threadIdx.x) - 1u));
+                        if (masked && place < want) sh.buf[place] = key_of(-INFINITY, (uint32_t)at);
+                        have += __popc(votes);
+                    }
+                }
+                n = want;
+                __syncthreads();
+            }
+            select_best(sh, n, want);
         }
-        select_best(sh, n, want);
     }
     if (CLUSTER) {
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         if (part == 0) {
-            if (threadIdx.x == 0) {
-                st = sh.stat;
-                for (int p = 1; p < blocks_per_row; ++p) st.join(cluster.map_shared_rank(&sh, p)->stat, a.scale);
-                sh.stat = st;
-                sh.count = 0;
+            if (threadIdx.x < 32) {
+                Stat mine = (int)threadIdx.x < blocks_per_row ? cluster.map_shared_rank(&sh, (int)threadIdx.x)->stat : Stat{-INFINITY, 0.f, 0.f, 0.f};
+                mine = warp_join(mine, a.scale);
+                if (threadIdx.x == 0) sh.part[0] = mine;       // sh.stat is still being read
+            }
+            if constexpr (ENT) {
+                if (tops) {
+                    if (threadIdx.x == 0) sh.count = 0;
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < blocks_per_row * a.top; i += kScThreads) {
+                        const ScoreShared* o = cluster.map_shared_rank(&sh, i / a.top);
+                        if (i % a.top < o->n_best) push(sh, o->best[i % a.top]);
+                    }
+                    __syncthreads();
+                    const int n = sh.count;
+                    __syncthreads();          // the lists, this block's own among them, have been read
+                    select_best(sh, n, a.top);
+                }
             }
             __syncthreads();
-            if (tops) {
-                for (int i = threadIdx.x; i < blocks_per_row * kScMaxTop; i += kScThreads) {
-                    const ScoreShared* o = cluster.map_shared_rank(&sh, i / kScMaxTop);
-                    if (i % kScMaxTop < o->n_best) push(sh, o->best[i % kScMaxTop]);
-                }
-                __syncthreads();
-                const int n = sh.count;
-                __syncthreads();          // the remote lists, block 0's own among them, have been read
-                select_best(sh, n, a.top);
-            }
+            st = sh.part[0];
         }
-        cluster.sync();                   // no block leaves while its lists are read
+        cluster.sync();                   // no block leaves while its part is read
         if (part != 0) return;
     } else {
         __syncthreads();
+        st = sh.stat;
     }
-    st = sh.stat;
-    if (a.stats != nullptr && threadIdx.x == 0) a.stats[row] = make_float2(st.r, empty_row(st) ? 0.f : 1.f / st.s);
-    if (MODE == kDistill) {
-        const float loss = distill_loss(a, row, zr, st, (int)threadIdx.x, kScThreads, sh.red, true);
-        if (threadIdx.x == 0) a.loss[row] = loss;
-        return;
-    }
-    const double log2_s = log2((double)st.s);
-    if (threadIdx.x == 0) {
-        a.entropy[row] = empty_row(st) ? 0.f : (float)(kLn2 * (log2_s - (double)st.e / (double)st.s));
-        if (a.targets != nullptr) {
-            const int64_t t = a.targets[row];
-            a.log_prob[row] = t < 0 ? 0.f : t >= a.classes ? __uint_as_float(0x7fffffffu) : log_prob_of(st, log2_s, to_f32(zr[t]), a.scale);
+    if constexpr (!ENT) {
+        // few entries are the first warp's work, the other warps are done
+        const bool whole = a.n_t > 128;
+        if (!whole && threadIdx.x >= 32) return;
+        float2 teacher;
+        const float loss = distill_loss(a, row, zr, st, entry, (int)threadIdx.x, whole ? kScThreads : 32, sh.red, whole, teacher);
+        if (threadIdx.x == 0) {
+            a.loss[row] = loss;
+            if (a.stats != nullptr) ((float4*)a.stats)[row] = make_float4(st.r, empty_row(st) ? 0.f : 1.f / st.s, teacher.x, teacher.y);
         }
-    }
-    for (int k = threadIdx.x; k < a.top; k += kScThreads) {
-        const uint64_t key = sh.best[k];
-        a.top_ids[row * a.top + k] = index_of(key);
-        a.top_lp[row * a.top + k] = log_prob_of(st, log2_s, score_of((uint32_t)(key >> 32)), a.scale);
+    } else {
+        const double log2_s = log2((double)st.s);
+        if (threadIdx.x == 0) {
+            if (a.stats != nullptr) a.stats[row] = make_float2(st.r, empty_row(st) ? 0.f : 1.f / st.s);
+            a.entropy[row] = empty_row(st) ? 0.f : (float)(kLn2 * (log2_s - (double)st.e / (double)st.s));
+            if (a.targets != nullptr) {
+                const int64_t t = a.targets[row];
+                a.log_prob[row] = t < 0 ? 0.f : t >= a.classes ? __uint_as_float(0x7fffffffu) : log_prob_of(st, log2_s, to_f32(zr[t]), a.scale);
+            }
+        }
+        for (int k = threadIdx.x; k < a.top; k += kScThreads) {
+            const uint64_t key = sh.best[k];
+            a.top_ids[row * a.top + k] = index_of(key);
+            a.top_lp[row * a.top + k] = log_prob_of(st, log2_s, score_of((uint32_t)(key >> 32)), a.scale);
+        }
     }
 }
 
@@ -543,14 +667,53 @@ struct ScoreGradArgs {
     const float *g_lp, *g_ent, *g_loss;    // per row; g_lp or g_ent may be null
 };
 
+// Chunks [c_begin, c_end) of a row, dealt out to `step` threads, through `f` to the same places of another row.  f(e0, v, j) gets the
+// first class of a chunk and the chunk's number among those that lie inside the row, counted from the block's first (-1 for
+// the ones at the row's ends).  Five blocks of these loops per SM keep enough loads in flight; fetching the next chunks ahead in
+// registers instead cost a block and was slower (201 against 190 us at 4096 x 50000 bf16).
+template <typename T, typename F>
+__device__ __forceinline__ void stream_chunks(const T* zr, T* dr, int n, int ph, int c_begin, int c_end, int t, int step, F f) {
+    constexpr int N = Chunk<T>::N;
+    float v[N];
+    const int f0 = c_begin == 0 && ph > 0 ? 1 : c_begin, f1 = max(f0, min(c_end, (n + ph) / N)), inner = f1 - f0;
+    const uint4* src = reinterpret_cast<const uint4*>(zr - ph) + f0;
+    int j = t;
+    if (aligned16(dr - ph)) {
+        uint4* dst = reinterpret_cast<uint4*>(dr - ph) + f0;
+        for (; j + (kScUnroll - 1) * step < inner; j += kScUnroll * step) {
+            uint4 raw[kScUnroll];
+#pragma unroll
+            for (int u = 0; u < kScUnroll; ++u) raw[u] = src[j + u * step];
+#pragma unroll
+            for (int u = 0; u < kScUnroll; ++u) {
+                unpack16(raw[u], v, (const T*)nullptr);
+                f((f0 + j + u * step) * N - ph, v, j + u * step);
+                dst[j + u * step] = pack16(v, (const T*)nullptr);
+            }
+        }
+    }
+    for (; j < inner; j += step) {
+        unpack16(src[j], v, (const T*)nullptr);
+        f((f0 + j) * N - ph, v, j);
+        store_chunk(dr, (f0 + j) * N - ph, n, v);
+    }
+    if (t < 2 && (t == 0 ? c_begin < f0 : f1 < c_end)) {
+        const int e0 = (t == 0 ? c_begin : f1) * N - ph;
+        load_chunk(zr, e0, n, 0.f, v);
+        f(e0, v, -1);
+        store_chunk(dr, e0, n, v);
+    }
+}
+
 // kScThreads / G rows of a block, G threads a row and `run` chunks of it per block.  log_probs:
 //     dz_j = g_lp (1[j = t] - p_j) - g_H p_j (log p_j + H)
-// distillation:  dz_j = g T (p_j - sum_k q_k 1[id_k = j]); the named classes are written a second time, each by its first entry.
+// distillation:  dz_j = g T (p_j - sum_k q_k 1[id_k = j]).  The named classes are sorted first, with the place in that order where
+// each run of 32 chunks begins, so that a warp knows the few entries of its chunks; writing them in a second step behind a
+// barrier took a third as long again (190 against 141 us of streaming at 4096 x 50000 bf16).
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kScThreads) scores_grad_kernel(ScoreGradArgs a, int G, int run, int runs) {
+__global__ void __launch_bounds__(kScThreads, 5) scores_grad_kernel(ScoreGradArgs a, int G, int run, int runs) {
     constexpr int N = Chunk<T>::N;
-    __shared__ double red[kScThreads / 32];
-    extern __shared__ int sids[];                       // distillation: classes of this block's rows
+    extern __shared__ int dyn[];
     const int t = (int)threadIdx.x % G, sub = (int)threadIdx.x / G, rows_here = kScThreads / G;
     const int64_t row = (int64_t)(blockIdx.x / (unsigned)runs) * rows_here + sub;
     const bool on = row < a.f.rows;
@@ -558,75 +721,91 @@ __global__ void __launch_bounds__(kScThreads) scores_grad_kernel(ScoreGradArgs a
     const T* zr = (const T*)a.f.z + (on ? row : 0) * a.f.z_stride;
     T* dr = (T*)a.dz + (on ? row : 0) * a.f.classes;
     const int V = a.f.classes, ph = row_phase(zr);
-    const float2 st = on ? a.f.stats[row] : make_float2(0.f, 0.f);
     const float scale = a.f.scale;
     const int c_end = min(c_begin + run, (V + ph + N - 1) / N);
-    if (MODE == kLogProbs) {
+    if constexpr (MODE == kLogProbs) {
         if (!on) return;
+        const float2 st = a.f.stats[row];
         const int64_t tgt = a.f.targets != nullptr ? a.f.targets[row] : -1;
         const bool dead = st.y == 0.f;                                          // a row without a distribution
         float g_lp = a.g_lp != nullptr && tgt >= 0 && !dead ? a.g_lp[row] : 0.f;
         if (tgt >= V) g_lp = __uint_as_float(0x7fffffffu);
         const float g_ent = a.g_ent != nullptr && !dead ? a.g_ent[row] : 0.f;
-        const float H = a.g_ent != nullptr ? a.f.entropy[row] : 0.f;
-        const float ln2 = (float)kLn2, lg = log2f(st.y);
-        for (int c = c_begin + t; c < c_end; c += G) {
-            const int64_t e0 = (int64_t)c * N - ph;
-            float v[N];
-            load_chunk(zr, e0, V, 0.f, v);
+        // -p (g_lp + g_H (ln 2 a + log(1 / s) + H)),  p = 2^a / s
+        const float base = g_ent == 0.f ? g_lp : g_lp + g_ent * (logf(st.y) + a.f.entropy[row]), slope = g_ent * (float)kLn2;
+        const int at = tgt >= V ? -1 : (int)tgt;
+        stream_chunks(zr, dr, V, ph, c_begin, c_end, t, G, [&](int e0, float (&v)[N], int) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float y = (v[i] - st.x) * scale;
-                const float p = ex2(y) * st.y;
-                float d = -g_lp * p;
-                if (g_ent != 0.f) d -= g_ent * p * (ln2 * (fmaxf(y, -1e5f) + lg) + H);
-                if (dead) d = 0.f;
-                if (e0 + i == tgt) d += g_lp;
-                v[i] = d;
+                v[i] = dead ? 0.f : -(ex2(y) * st.y) * fmaf(slope, fmaxf(y, -1e5f), base);
             }
-            store_chunk(dr, e0, V, v);
-        }
+            if (at >= e0 && at < e0 + N) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (e0 + i == at) v[i] += g_lp;
+            }
+        });
         return;
     }
-    const bool whole = G > 32;       // then the block has one row
-    Teacher q{};
-    if (on) q = teacher_of(a.f, row, t, G, red, whole);
-    const bool dead = !on || !q.any || st.y == 0.f;
-    const float g = dead ? 0.f : a.g_loss[row] * a.f.temperature;
-    if (on) {
-        for (int c = c_begin + t; c < c_end; c += G) {
-            const int64_t e0 = (int64_t)c * N - ph;
-            float v[N];
-            load_chunk(zr, e0, V, 0.f, v);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = dead ? 0.f : g * (ex2((v[i] - st.x) * scale) * st.y);
-            store_chunk(dr, e0, V, v);
+    const int K = a.f.n_t, groups = (run + 31) / 32 + 1;
+    int* named = dyn + sub * (3 * K + groups);           // as given, -1 for an entry that is not there
+    int* ids = named + K;                                // in order
+    float* wts = (float*)(ids + K);
+    int* start = (int*)(wts + K);
+    const float4 st = on ? ((const float4*)a.f.stats)[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool dead = st.y == 0.f || st.w == 0.f;       // no row, no distribution, or no teacher
+    const float g = dead ? 0.f : a.g_loss[row] * a.f.temperature, gp = g * st.y;
+    if (!dead)
+        for (int k = t; k < K; k += G) {
+            const int64_t id = a.f.t_ids[row * K + k];
+            named[k] = id >= 0 && id < V ? (int)id : -1;
         }
-    }
-    int* ids = sids + sub * a.f.n_t;
-    if (on && !dead)
-        for (int k = t; k < a.f.n_t; k += G) {
-            const int64_t id = a.f.t_ids[row * a.f.n_t + k];
-            ids[k] = id >= 0 && id < V ? (int)id : -1;
+    __syncthreads();
+    if (!dead)
+        for (int k = t; k < K; k += G) {
+            const int id = named[k];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < K; ++j) rank += named[j] < id || (named[j] == id && j < k);
+            ids[rank] = id;
+            wts[rank] = id < 0 ? 0.f : g * (weight_of(a.f, load_score(a.f.t_scores, a.f.t_dtype, row * K + k), st.z) * st.w);
         }
-    __syncthreads();                 // the list is there, and what the block wrote above is in order before what follows
-    if (dead) return;
-    const int e_lo = c_begin * N - ph, e_hi = c_end * N - ph;
-    for (int k = t; k < a.f.n_t; k += G) {
-        const int id = ids[k];
-        if (id < e_lo || id >= e_hi || id < 0) continue;
-        double w = 0.0;
-        bool mine = true;
-        for (int j = 0; j < a.f.n_t; ++j) {
-            if (ids[j] != id) continue;
-            if (j < k) {
-                mine = false;
-                break;
+    __syncthreads();
+    if (!dead) {
+        const int first = (c_begin == 0 && ph > 0 ? 1 : c_begin) * N - ph;
+        for (int i = t; i < groups; i += G) {
+            const int from = first + i * 32 * N;         // entries below this class lie before group i
+            int lo = 0, hi = K;
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (ids[mid] < from) lo = mid + 1;
+                else hi = mid;
             }
-            w += exp(((double)load_score(a.f.t_scores, a.f.t_dtype, row * a.f.n_t + j) - (double)q.tmax) / (double)a.f.temperature) / q.sum;
+            start[i] = lo;
         }
-        if (mine) dr[id] = from_f32<T>(g * (float)((double)(ex2((to_f32(zr[id]) - st.x) * scale) * st.y) - w));
     }
+    __syncthreads();
+    if (!on) return;
+    stream_chunks(zr, dr, V, ph, c_begin, c_end, t, G, [&](int e0, float (&v)[N], int j) {
+        if (dead) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = 0.f;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = gp * ex2((v[i] - st.x) * scale);
+        const int k1 = j < 0 ? K : start[j / 32 + 1];
+        for (int k = j < 0 ? 0 : start[j / 32]; k < k1; ++k) {
+            const int at = ids[k] - e0;
+            if (at >= 0 && at < N) {
+                const float w = wts[k];
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (i == at) v[i] -= w;
+            }
+        }
+    });
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
@@ -679,14 +858,21 @@ static int scores_bwd(const ScoreGradArgs& a, cudaStream_t st) {
     constexpr int N = Chunk<T>::N;
     const int kid = MODE == kLogProbs ? K_LOGP_BWD : K_DISTILL_BWD;
     const int64_t chunks = ((int64_t)a.f.classes + 2 * N - 2) / N;
-    const int G = chunks <= 32 ? 32 : kScThreads;
-    const int run = kScThreads * kScUnroll;
-    const int runs = G == 32 ? 1 : (int)((chunks + run - 1) / run);
+    int G = 32;
+    while (G < kScThreads && G * kScUnroll < chunks) G *= 2;
+    // whole rows, or parts of them where the rows alone would not keep the SMs busy
+    const int64_t groups = (a.f.rows + kScThreads / G - 1) / (kScThreads / G), tile = (int64_t)G * kScUnroll;
+    const int64_t tiles = (chunks + tile - 1) / tile;
+    const int64_t cut = std::max<int64_t>(1, std::min(tiles, (kNumSM * 8 + groups - 1) / groups));
+    const int run = (int)std::min<int64_t>((tiles + cut - 1) / cut * tile, 1 << 15);      // bounds the table of starts
+    const int runs = (int)((chunks + run - 1) / run);
     const int64_t blocks = (a.f.rows + kScThreads / G - 1) / (kScThreads / G) * runs;
     CGB_REQUIRE(blocks <= 0x7fffffff, "class scores: too many blocks for one launch");
-    const size_t smem = MODE == kDistill ? (size_t)(kScThreads / G) * a.f.n_t * sizeof(int) : 0;
+    const size_t smem = MODE == kDistill ? (size_t)(kScThreads / G) * (3 * a.f.n_t + (run + 31) / 32 + 1) * sizeof(int) : 0;
+    auto kern = scores_grad_kernel<T, MODE>;
+    if (smem > 48 * 1024) CGB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     launch_begin(kid, st);
-    scores_grad_kernel<T, MODE><<<(unsigned)blocks, kScThreads, smem, st>>>(a, G, run, runs);
+    kern<<<(unsigned)blocks, kScThreads, smem, st>>>(a, G, run, runs);
     launch_end(kid, st);
     CGB_CUDA(cudaGetLastError());
     return CGB200_OK;
@@ -751,9 +937,11 @@ int cgb200_distill_fwd(const void* logits, int64_t stride, const int64_t* teache
     if (rows == 0) return CGB200_OK;
     if (int rc = teacher_check(teacher_ids, teacher_scores, n_teacher, teacher_dtype, temperature)) return rc;
     CGB_REQUIRE(loss != nullptr, "distillation: null buffer");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "distillation: stats must be 16-byte aligned");
     ScoreArgs a{};
     a.z = logits, a.z_stride = stride, a.rows = rows, a.classes = (int)classes, a.scale = kLog2e / temperature, a.stats = (float2*)stats;
     a.t_ids = teacher_ids, a.t_scores = teacher_scores, a.n_t = n_teacher, a.t_dtype = teacher_dtype, a.temperature = temperature, a.loss = loss;
+    a.inv_temperature = 1.0 / (double)temperature;
     CGB_SCORE_TYPES(scores_fwd, kDistill, a, (cudaStream_t)stream);
 }
 
@@ -764,9 +952,11 @@ int cgb200_distill_bwd(const void* logits, int64_t stride, const int64_t* teache
     if (rows == 0) return CGB200_OK;
     if (int rc = teacher_check(teacher_ids, teacher_scores, n_teacher, teacher_dtype, temperature)) return rc;
     CGB_REQUIRE(stats != nullptr && g_loss != nullptr && dlogits != nullptr, "distillation: null buffer");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "distillation: stats must be 16-byte aligned");
     ScoreGradArgs a{};
     a.f.z = logits, a.f.z_stride = stride, a.f.rows = rows, a.f.classes = (int)classes, a.f.scale = kLog2e / temperature, a.f.stats = (float2*)stats;
     a.f.t_ids = teacher_ids, a.f.t_scores = teacher_scores, a.f.n_t = n_teacher, a.f.t_dtype = teacher_dtype, a.f.temperature = temperature;
+    a.f.inv_temperature = 1.0 / (double)temperature;
     a.dz = dlogits, a.g_loss = g_loss;
     CGB_SCORE_TYPES(scores_bwd, kDistill, a, (cudaStream_t)stream);
 }

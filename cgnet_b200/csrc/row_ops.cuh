@@ -79,15 +79,25 @@ template <typename T>
 __device__ __forceinline__ int row_phase(const T* row) {
     return (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % Chunk<T>::N);
 }
-// Chunk at value e0 (possibly negative) of a row of n values; values outside the row read as `fill`.
-template <typename T, int N = Chunk<T>::N>
-__device__ __forceinline__ void load_chunk(const T* row, int64_t e0, int64_t n, float fill, float (&v)[N]) {
+// The 16 bytes of the chunk at value e0 (possibly negative) of a row of n values; values outside the row read as `fill`.  Kept apart
+// from the conversion to float32, so that a thread's chunks are all on their way before the first is waited for.
+template <typename T>
+__device__ __forceinline__ uint4 load_raw(const T* row, int64_t e0, int64_t n, float fill) {
+    constexpr int N = Chunk<T>::N;
+    uint4 u;
     if (e0 >= 0 && e0 + N <= n && aligned16(row + e0)) {
-        unpack16(*reinterpret_cast<const uint4*>(row + e0), v, (const T*)nullptr);
+        u = *reinterpret_cast<const uint4*>(row + e0);
     } else {
+        float v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(row[e0 + i]) : fill;
+        u = pack16(v, (const T*)nullptr);      // the values came from this type: nothing is rounded
     }
+    return u;
+}
+template <typename T, int N = Chunk<T>::N>
+__device__ __forceinline__ void load_chunk(const T* row, int64_t e0, int64_t n, float fill, float (&v)[N]) {
+    unpack16(load_raw(row, e0, n, fill), v, (const T*)nullptr);
 }
 template <typename T, int N = Chunk<T>::N>
 __device__ __forceinline__ void store_chunk(T* row, int64_t e0, int64_t n, const float (&v)[N]) {

@@ -314,7 +314,7 @@ def _distill_fwd(z2, ids, scores, temperature, keep):
     rows, classes = z2.shape
     dev = z2.device
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if keep else None
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if keep else None
     _call("cgb200_distill_fwd", dev, z2.data_ptr(), z2.stride(0), ids.data_ptr(), scores.data_ptr(), ids.shape[1], _DTYPES[scores.dtype],
           temperature, loss.data_ptr(), _ptr(stats), rows, classes, _DTYPES[z2.dtype])
     return loss, stats

@@ -347,6 +347,7 @@ int cgb200_log_probs_bwd(const void* logits, int64_t stride, const int64_t* targ
  *                    the row NaN; a class named twice counts with both weights
  *   teacher_scores   [rows][n_teacher] of type teacher_dtype, contiguous; -inf is an entry of weight 0
  *   n_teacher        1..1024;  temperature 0.001..1000
+ *   stats            float[rows][4] for the backward, 16-byte aligned, NULL where none follows
  * A row without entries has loss 0 and gradient 0; a row of logits that are all -inf has loss +inf and gradient 0.
  */
 #define CGB200_MAX_TEACHER      1024

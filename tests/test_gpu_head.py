@@ -384,6 +384,7 @@ def test_log_probs_nan_infinity_and_bad_targets(classes):
     z[1, 7], z[2, classes - 1], z[3, 11] = float("nan"), float("nan"), float("inf")
     z[4] = float("-inf")
     z[4, 20] = float("nan")
+    z[5, 0], z[5, 1] = float("nan"), float("nan")
     target = torch.tensor([classes, 3, 4, 11, 5, -100], device=cuda())
     check_log_probs(z, target, 9, randn(g, 6), None)
     for row in range(6):
