@@ -23,13 +23,14 @@ namespace cg = cooperative_groups;
 constexpr int kScThreads = 256;
 constexpr int kScUnroll = 4;                     // chunks a thread has in flight
 constexpr int kScCap = 4096;                     // candidates a block collects before it has to fall back
-constexpr int kScMaxTop = 128;                   // kScMaxTop threads' chunks of the first tile always fit the candidates
+constexpr int kScChunks = kScCap / 8;            // chunks they come from
+constexpr int kScMaxTop = 128;                   // kScMaxTop threads' chunks of the first tile always fit
 constexpr int kScWarpValues = 32;                // values per lane of the kernel for short rows
 constexpr float kScMargin = 10.f;
 constexpr int kScPickKeys = 512;                 // candidates a warp searches in registers
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
-static_assert(kScMaxTop * kScUnroll * 8 <= kScCap, "the first tile's candidates must fit");
+static_assert(kScMaxTop * kScUnroll <= kScChunks, "the first tile's candidates must fit");
 
 enum ScoreMode { kLogProbs = 0, kDistill = 1 };
 
@@ -341,26 +342,36 @@ struct ScoreShared : ScoreBase {
     uint64_t buf[kScCap];          // candidates
     uint64_t best[kScMaxTop];      // this block's best, in order
     unsigned hist[256];
-    int count, kept, n_best;
+    int count, kept, n_best, chunks;
+    int chunk[kScChunks];          // chunks with a score that may rank
     uint64_t prefix;
     unsigned want;
 };
 
 __device__ __forceinline__ void push(ScoreShared& sh, uint64_t key) {
     const int at = atomicAdd(&sh.count, 1);
-    if (at < kScCap) sh.buf[at] = key;
+    if (at < kScCap) sh.buf[at] = key;       // the counts that decide what is pushed keep it within; the bound makes sure
 }
 
-// The scores of a chunk that are not below thr (`strict`: above it) become candidates.  Rare and kept out of line: inlined into the
-// unrolled loop it outgrew the instruction cache.
+// A chunk with a score that may rank: only its number is noted in the loop over the row, by what is usually one lane of a warp;
+// its scores are looked at afterwards, chunk by thread (expand_chunks).  Doing that in the loop took half of its instructions.
+__device__ __forceinline__ void note_chunk(ScoreShared& sh, int c) {
+    const int at = atomicAdd(&sh.chunks, 1);
+    if (at < kScChunks) sh.chunk[at] = c;
+}
+// The scores of the noted chunks from thr on become candidates (each chunk is noted once, and kScChunks of them fit).
 template <typename T>
-__device__ __noinline__ void push_chunk(ScoreShared& sh, uint4 raw, int e0, float thr, bool strict) {
+__device__ __forceinline__ void expand_chunks(ScoreShared& sh, const T* zr, int ph, int classes, float thr) {
     constexpr int N = Chunk<T>::N;
-    float v[N];
-    unpack16(raw, v, (const T*)nullptr);
+    for (int i = threadIdx.x; i < sh.chunks; i += kScThreads) {
+        const int e0 = sh.chunk[i] * N - ph;
+        float v[N];
+        load_chunk(zr, e0, classes, -INFINITY, v);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (!(v[i] < thr) && v[i] != -INFINITY && !(strict && v[i] == thr)) push(sh, key_of(v[i], (uint32_t)(e0 + i)));
+        for (int j = 0; j < N; ++j)
+            if (!(v[j] < thr) && v[j] != -INFINITY) push(sh, key_of(v[j], (uint32_t)(e0 + j)));
+    }
+    __syncthreads();
 }
 
 // Largest t, in its upper 16 bits, that at least k of n <= kScPickKeys orders in shared memory (`step` words apart) reach; by the block's
@@ -501,7 +512,7 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
     const bool tops = ENT && a.top > 0;
     const int want = tops ? min(a.top, max(0, behind - first)) : 0;      // entries it has to offer
     if constexpr (ENT) {
-        if (threadIdx.x == 0) sh.count = 0;
+        if (threadIdx.x == 0) sh.count = 0, sh.chunks = 0;
     }
     RunStat run(a.scale);
     float thr = -INFINITY;
@@ -530,7 +541,7 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
             run.add<N, ENT>(v, cm, a.scale);
             if constexpr (ENT) {
                 tm = fmaxf(tm, cm);
-                if (tops && base != f0 && !(cm <= thr)) push_chunk<T>(sh, raw[u], (base + u * kScThreads + (int)threadIdx.x) * N - ph, thr, true);
+                if (tops && base != f0 && !(cm <= thr)) note_chunk(sh, base + u * kScThreads + (int)threadIdx.x);
             }
         }
         if constexpr (ENT) {
@@ -548,9 +559,10 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
                 const uint32_t t = sh.want;
                 thr = t <= order_of(-INFINITY) ? -INFINITY : score_of(t);
 #pragma unroll
-                for (int u = 0; u < kScUnroll; ++u)
-                    if (!(chunk_max(raw[u], (const T*)nullptr) < thr))
-                        push_chunk<T>(sh, raw[u], (base + u * kScThreads + (int)threadIdx.x) * N - ph, thr, false);
+                for (int u = 0; u < kScUnroll; ++u) {
+                    const float cm = chunk_max(raw[u], (const T*)nullptr);
+                    if (!(cm < thr) && cm != -INFINITY) note_chunk(sh, base + u * kScThreads + (int)threadIdx.x);
+                }
             }
         }
     }
@@ -563,7 +575,7 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
             unpack16(end, v, (const T*)nullptr);
             run.add<N, ENT>(v, chunk_max(end, (const T*)nullptr), a.scale);
             if constexpr (ENT) {
-                if (tops) push_chunk<T>(sh, end, c * N - ph, thr, false);
+                if (tops) note_chunk(sh, c);
             }
         }
     }
@@ -577,8 +589,12 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
     }
     if constexpr (ENT) {
         if (tops) {
-            int n = sh.count;
-            if (n > kScCap) {
+            int n = 0;
+            if (sh.chunks <= kScChunks) {
+                expand_chunks(sh, zr, ph, a.classes, thr);
+                n = sh.count;
+            }
+            if (sh.chunks > kScChunks) {
                 radix_collect(sh, zr, ph, c0, c1, a.classes, want);
                 n = sh.count;
             } else if (n < want) {
