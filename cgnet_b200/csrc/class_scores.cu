@@ -22,15 +22,16 @@ namespace cg = cooperative_groups;
 
 constexpr int kScThreads = 256;
 constexpr int kScUnroll = 4;                     // chunks a thread has in flight
-constexpr int kScCap = 4096;                     // candidates a block collects before it has to fall back
-constexpr int kScChunks = kScCap / 8;            // chunks they come from
-constexpr int kScMaxTop = 128;                   // kScMaxTop threads' chunks of the first tile always fit
+constexpr int kScPickKeys = 512;                 // candidates a warp searches in registers
+constexpr int kScCap = 2 * kScPickKeys;          // candidates a block keeps: two lists, one is sifted into the other
+constexpr int kScChunks = 512;                   // chunks with a score that may rank, noted between two looks at them
+constexpr int kScNewKeys = 256;                  // candidates expected between two looks
+constexpr int kScMaxTop = 128;
 constexpr int kScWarpValues = 32;                // values per lane of the kernel for short rows
 constexpr float kScMargin = 10.f;
-constexpr int kScPickKeys = 512;                 // candidates a warp searches in registers
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
-static_assert(kScMaxTop * kScUnroll <= kScChunks, "the first tile's candidates must fit");
+static_assert(kScMaxTop + kScNewKeys <= kScPickKeys * 3 / 4, "candidates between two looks should fit a list");
 
 enum ScoreMode { kLogProbs = 0, kDistill = 1 };
 
@@ -348,32 +349,12 @@ struct ScoreShared : ScoreBase {
     unsigned want;
 };
 
-__device__ __forceinline__ void push(ScoreShared& sh, uint64_t key) {
-    const int at = atomicAdd(&sh.count, 1);
-    if (at < kScCap) sh.buf[at] = key;       // the counts that decide what is pushed keep it within; the bound makes sure
-}
-
 // A chunk with a score that may rank: only its number is noted in the loop over the row, by what is usually one lane of a warp;
 // its scores are looked at afterwards, chunk by thread (expand_chunks).  Doing that in the loop took half of its instructions.
 __device__ __forceinline__ void note_chunk(ScoreShared& sh, int c) {
     const int at = atomicAdd(&sh.chunks, 1);
     if (at < kScChunks) sh.chunk[at] = c;
 }
-// The scores of the noted chunks from thr on become candidates (each chunk is noted once, and kScChunks of them fit).
-template <typename T>
-__device__ __forceinline__ void expand_chunks(ScoreShared& sh, const T* zr, int ph, int classes, float thr) {
-    constexpr int N = Chunk<T>::N;
-    for (int i = threadIdx.x; i < sh.chunks; i += kScThreads) {
-        const int e0 = sh.chunk[i] * N - ph;
-        float v[N];
-        load_chunk(zr, e0, classes, -INFINITY, v);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (!(v[j] < thr) && v[j] != -INFINITY) push(sh, key_of(v[j], (uint32_t)(e0 + j)));
-    }
-    __syncthreads();
-}
-
 // Largest t, in its upper 16 bits, that at least k of n <= kScPickKeys orders in shared memory (`step` words apart) reach; by the block's
 // first warp, 16 halvings on registers.  0 where n < k.
 __device__ __forceinline__ uint32_t kth_order(const uint32_t* v, int step, int n, int k) {
@@ -394,24 +375,51 @@ __device__ __forceinline__ uint32_t kth_order(const uint32_t* v, int step, int n
     }
     return t;
 }
+__device__ __forceinline__ void push(ScoreShared& sh, uint64_t key) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < kScCap) sh.buf[at] = key;
+}
+// The scores of the noted chunks from thr on become candidates.  False where either did not fit: the row is then searched
+// by radix_collect.  Ends behind a barrier; sh.count is the number of candidates.
+template <typename T>
+__device__ __forceinline__ bool expand_chunks(ScoreShared& sh, const T* zr, int ph, int classes, float thr) {
+    constexpr int N = Chunk<T>::N;
+    __syncthreads();
+    const int n = sh.chunks;
+    for (int i = threadIdx.x; i < min(n, kScChunks); i += kScThreads) {
+        const int e0 = sh.chunk[i] * N - ph;
+        float v[N];
+        load_chunk(zr, e0, classes, -INFINITY, v);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (!(v[j] < thr) && v[j] != -INFINITY) push(sh, key_of(v[j], (uint32_t)(e0 + j)));
+    }
+    __syncthreads();
+    return n <= kScChunks && sh.count <= kScCap;
+}
+// Of n <= kScPickKeys candidates those whose order is at least the k-th highest's (in its upper 16 bits), which is returned:
+// moved to the list's second half, sh.kept of them.  Ends behind a barrier.
+__device__ __forceinline__ uint32_t sift(ScoreShared& sh, int n, int k) {
+    if (threadIdx.x < 32) {
+        const uint32_t t = kth_order((const uint32_t*)sh.buf + 1, 2, n, k);
+        if (threadIdx.x == 0) sh.want = t, sh.kept = 0;
+    }
+    __syncthreads();
+    const uint32_t t = sh.want;
+    for (int i = threadIdx.x; i < n; i += kScThreads)
+        if ((uint32_t)(sh.buf[i] >> 32) >= t) sh.buf[kScPickKeys + atomicAdd(&sh.kept, 1)] = sh.buf[i];
+    __syncthreads();
+    return t;
+}
 // The `k` highest of the first n candidates, in order, to sh.best (n_best of them).  All keys differ, so their order
 // does not depend on the order in which they were collected.
 __device__ void select_best(ScoreShared& sh, int n, int k) {
     if (n <= kScPickKeys) {
-        uint64_t* keys = sh.buf;
+        const uint64_t* keys = sh.buf;
         int m = n;
         if (n > 64 && n > k) {
-            // first down to those of the k-th one's order or above
-            if (threadIdx.x < 32) {
-                const uint32_t t = kth_order((const uint32_t*)sh.buf + 1, 2, n, k);
-                if (threadIdx.x == 0) sh.want = t, sh.kept = 0;
-            }
-            __syncthreads();
-            const uint32_t t = sh.want;
+            sift(sh, n, k);
             keys = sh.buf + kScPickKeys;
-            for (int i = threadIdx.x; i < n; i += kScThreads)
-                if ((uint32_t)(sh.buf[i] >> 32) >= t) keys[atomicAdd(&sh.kept, 1)] = sh.buf[i];
-            __syncthreads();
             m = sh.kept;
         }
         for (int i = threadIdx.x; i < m; i += kScThreads) {
@@ -422,13 +430,11 @@ __device__ void select_best(ScoreShared& sh, int n, int k) {
             if (rank < k) sh.best[rank] = key;
         }
     } else {
-        int p = 1024;
-        while (p < n) p *= 2;
-        for (int i = n + threadIdx.x; i < p; i += kScThreads) sh.buf[i] = 0;
-        for (int size = 2; size <= p; size *= 2)
+        for (int i = n + threadIdx.x; i < kScCap; i += kScThreads) sh.buf[i] = 0;
+        for (int size = 2; size <= kScCap; size *= 2)
             for (int d = size / 2; d > 0; d /= 2) {
                 __syncthreads();
-                for (int i = threadIdx.x; i < p / 2; i += kScThreads) {
+                for (int i = threadIdx.x; i < kScCap / 2; i += kScThreads) {
                     const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
                     const uint64_t x = sh.buf[lo], y = sh.buf[hi];
                     if ((x < y) == ((lo & size) == 0)) sh.buf[lo] = y, sh.buf[hi] = x;    // descending
@@ -440,6 +446,8 @@ __device__ void select_best(ScoreShared& sh, int n, int k) {
     if (threadIdx.x == 0) sh.n_best = min(n, k);
     __syncthreads();
 }
+
+__device__ __forceinline__ float threshold_of(uint32_t order) { return order <= order_of(-INFINITY) ? -INFINITY : score_of(order); }
 
 // Too many candidates (long runs of equal or rising scores): the k-th highest key by radix, most significant byte first, until
 // what lies above the byte found fits the candidates.  Keys differ, so eight bytes always do.
@@ -516,12 +524,16 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
     }
     RunStat run(a.scale);
     float thr = -INFINITY;
+    // a row of random scores adds `top` candidates whenever what has been read of it doubles
+    const int grow = tops ? 1 + kScNewKeys / a.top : 1;
+    bool fits = true;
     // Chunks [f0, f1) lie inside the row; what is left at its two ends is one chunk each.
     const int f0 = c0 == 0 && ph > 0 ? 1 : c0, f1 = max(f0, min(c1, (a.classes + ph) / N));
     const uint4* src = reinterpret_cast<const uint4*>(zr - ph) + f0 + threadIdx.x;
     const uint4 none = load_raw(zr, 0, 0, -INFINITY);
     Entry entry{};
     if (!ENT && part == 0) entry = entry_of(a, row, zr, (int)threadIdx.x);
+    int look = f0 + kTile * (grow - 1);       // chunk behind which the candidates are looked at
     for (int base = f0; base < f1; base += kTile) {
         uint4 raw[kScUnroll];
         if (base + kTile <= f1) {
@@ -532,7 +544,7 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
             for (int u = 0; u < kScUnroll; ++u) raw[u] = base + u * kScThreads + (int)threadIdx.x < f1 ? src[u * kScThreads] : none;
         }
         src += kTile;
-        float tm = -INFINITY;
+        float cms[kScUnroll];
 #pragma unroll
         for (int u = 0; u < kScUnroll; ++u) {
             float v[N];
@@ -540,29 +552,41 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
             const float cm = chunk_max(raw[u], (const T*)nullptr);
             run.add<N, ENT>(v, cm, a.scale);
             if constexpr (ENT) {
-                tm = fmaxf(tm, cm);
+                cms[u] = cm;
                 if (tops && base != f0 && !(cm <= thr)) note_chunk(sh, base + u * kScThreads + (int)threadIdx.x);
             }
         }
         if constexpr (ENT) {
             if (tops && base == f0) {
-                // Threshold: the largest value (to the upper 16 bits of its order) that at least `top` threads' maxima of the first
-                // tile reach: nothing below it can rank, and nothing equal to it further right.
-                uint32_t* maxima = (uint32_t*)sh.hist;
-                maxima[threadIdx.x] = order_of(tm);
+                // Threshold: the largest value (to the upper 16 bits of its order) that at least `top` chunks of the first tile reach:
+                // nothing below it can rank, and nothing equal to it further right.  Chunk maxima are counted per pair of chunks.
+                uint32_t* maxima = (uint32_t*)sh.buf;
+#pragma unroll
+                for (int u = 0; u < kScUnroll; u += 2)
+                    maxima[u / 2 * kScThreads + threadIdx.x] = order_of(cms[u] > cms[u + 1] || !(cms[u + 1] == cms[u + 1]) ? cms[u] : cms[u + 1]);
                 __syncthreads();
                 if (threadIdx.x < 32) {
-                    const uint32_t t = kth_order(maxima, 1, kScThreads, a.top);
+                    const uint32_t t = kth_order(maxima, 1, kScThreads * kScUnroll / 2, a.top);
                     if (threadIdx.x == 0) sh.want = t;
                 }
                 __syncthreads();
-                const uint32_t t = sh.want;
-                thr = t <= order_of(-INFINITY) ? -INFINITY : score_of(t);
+                thr = threshold_of(sh.want);
 #pragma unroll
-                for (int u = 0; u < kScUnroll; ++u) {
-                    const float cm = chunk_max(raw[u], (const T*)nullptr);
-                    if (!(cm < thr) && cm != -INFINITY) note_chunk(sh, base + u * kScThreads + (int)threadIdx.x);
+                for (int u = 0; u < kScUnroll; ++u)
+                    if (!(cms[u] < thr) && cms[u] != -INFINITY) note_chunk(sh, base + u * kScThreads + (int)threadIdx.x);
+            } else if (tops && base >= look) {
+                // about as many candidates as a list holds by now: sift them, and raise the threshold to the k-th of them
+                fits = expand_chunks(sh, zr, ph, a.classes, thr) && sh.count <= kScPickKeys && fits;
+                const int n = sh.count;
+                if (fits && n > a.top) {
+                    thr = fmaxf(thr, threshold_of(sift(sh, n, a.top)));
+                    const int kept = sh.kept;
+                    for (int i = threadIdx.x; i < min(kept, kScPickKeys); i += kScThreads) sh.buf[i] = sh.buf[kScPickKeys + i];
+                    if (threadIdx.x == 0) sh.count = kept;
                 }
+                if (threadIdx.x == 0) sh.chunks = 0;
+                look = f0 + (int)min((int64_t)(base - f0 + kTile) * grow, (int64_t)1 << 30) - kTile;
+                __syncthreads();
             }
         }
     }
@@ -589,12 +613,9 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
     }
     if constexpr (ENT) {
         if (tops) {
-            int n = 0;
-            if (sh.chunks <= kScChunks) {
-                expand_chunks(sh, zr, ph, a.classes, thr);
-                n = sh.count;
-            }
-            if (sh.chunks > kScChunks) {
+            fits = expand_chunks(sh, zr, ph, a.classes, thr) && fits;
+            int n = sh.count;
+            if (!fits) {
                 radix_collect(sh, zr, ph, c0, c1, a.classes, want);
                 n = sh.count;
             } else if (n < want) {
@@ -627,16 +648,21 @@ __global__ void __launch_bounds__(kScThreads, MODE == kDistill ? 6 : 5) scores_r
             }
             if constexpr (ENT) {
                 if (tops) {
-                    if (threadIdx.x == 0) sh.count = 0;
-                    __syncthreads();
-                    for (int i = threadIdx.x; i < blocks_per_row * a.top; i += kScThreads) {
-                        const ScoreShared* o = cluster.map_shared_rank(&sh, i / a.top);
-                        if (i % a.top < o->n_best) push(sh, o->best[i % a.top]);
+                    // the blocks' lists, as many at a time as fit beside the best so far
+                    const int lists = kScCap / a.top - 1;
+                    for (int p0 = 0; p0 < blocks_per_row; p0 += lists) {
+                        if (threadIdx.x == 0) sh.count = 0;
+                        __syncthreads();
+                        for (int i = threadIdx.x; i < min(lists, blocks_per_row - p0) * a.top; i += kScThreads) {
+                            const ScoreShared* o = cluster.map_shared_rank(&sh, p0 + i / a.top);
+                            if (i % a.top < o->n_best) push(sh, o->best[i % a.top]);
+                        }
+                        if (p0 > 0 && (int)threadIdx.x < sh.n_best) push(sh, sh.best[threadIdx.x]);
+                        __syncthreads();
+                        const int n = sh.count;
+                        __syncthreads();          // the lists, this block's own among them, have been read
+                        select_best(sh, n, a.top);
                     }
-                    __syncthreads();
-                    const int n = sh.count;
-                    __syncthreads();          // the lists, this block's own among them, have been read
-                    select_best(sh, n, a.top);
                 }
             }
             __syncthreads();
