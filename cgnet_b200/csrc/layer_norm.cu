@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "row_ops.cuh"
+#include "tc_ptx.cuh"
 
 namespace cgb200 {
 
@@ -43,11 +44,23 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, T* 
     const T* xr = (const T*)a.x + row * a.x_stride;
     T* yr = y + row * a.dim;
     const int ph = row_phase(xr);
+    // everything the row needs is on its way before the first value is waited for
+    uint4 raw[CH];
+    Params<P, N> w[CH], b[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) raw[c] = load_raw(xr, (t + c * G) * N - ph, a.dim, 0.f);
+    if (CH <= 2) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (a.w != nullptr) w[c].load((const P*)a.w, (t + c * G) * N - ph, a.dim);
+            if (a.b != nullptr) b[c].load((const P*)a.b, (t + c * G) * N - ph, a.dim);
+        }
+    }
     float v[CH][N];
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        load_chunk(xr, (int64_t)(t + c * G) * N - ph, a.dim, 0.f, v[c]);
+        unpack16(raw[c], v[c], (const T*)nullptr);
 #pragma unroll
         for (int i = 0; i < N; ++i) s += v[c][i];
     }
@@ -65,18 +78,25 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, T* 
     }
     const float rstd = 1.f / sqrtf(row_sum<WARP>(q, red[1]) / (float)a.dim + a.eps);
     if (stats != nullptr && t == 0) stats[row] = make_float2(mean, rstd);
+    if (CH > 2) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (a.w != nullptr) w[c].load((const P*)a.w, (t + c * G) * N - ph, a.dim);
+            if (a.b != nullptr) b[c].load((const P*)a.b, (t + c * G) * N - ph, a.dim);
+        }
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int64_t e0 = (int64_t)(t + c * G) * N - ph;
+        const int e0 = (t + c * G) * N - ph;
         if (e0 >= a.dim) continue;
-        float w[N], b[N];
-        if (a.w != nullptr) load_params((const P*)a.w, e0, a.dim, w);
-        if (a.b != nullptr) load_params((const P*)a.b, e0, a.dim, b);
+        float wv[N], bv[N];
+        if (a.w != nullptr) w[c].get(wv);
+        if (a.b != nullptr) b[c].get(bv);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float o = v[c][i] * rstd;
-            if (a.w != nullptr) o *= w[i];
-            if (a.b != nullptr) o += b[i];
+            if (a.w != nullptr) o *= wv[i];
+            if (a.b != nullptr) o += bv[i];
             v[c][i] = o;
         }
         store_chunk(yr, e0, a.dim, v[c]);
@@ -272,6 +292,122 @@ __global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(L
     }
 }
 
+// The same for aligned rows of a block, which come through shared memory: a ring of `stages` rows of x and dy, filled by the
+// bulk copies of one thread, keeps reads in flight across the two barriers of a row.
+constexpr size_t kLnRingBytes = 200 * 1024;     // of the blocks of an SM together
+constexpr int kLnRingStages = 8;
+constexpr int kLnBwdThreadsPerSM = 512;         // of these kernels: 128 registers a thread
+
+template <typename T, typename P, int NC>
+__global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs a, int stages, uint32_t polls) {
+    constexpr int VE = Chunk<T>::N;
+    extern __shared__ __align__(128) char ring[];
+    __shared__ float red[4][32];
+    __shared__ uint64_t full[kLnRingStages];
+    __shared__ int failed_flag;
+    volatile int* failed = &failed_flag;
+    const int G = (int)blockDim.x, t = (int)threadIdx.x, warp = t >> 5, lane = t & 31, nwarps = G >> 5;
+    const uint32_t row_bytes = (uint32_t)(a.dim * sizeof(T));
+    const float inv_n = 1.f / (float)a.dim;
+    const int64_t n_here = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;      // rows blockIdx.x, + gridDim.x, ...
+    auto fetch = [&](int64_t i, int s) {
+        const int64_t row = blockIdx.x + i * gridDim.x;
+        mbar_arrive_expect_tx(&full[s], 2 * row_bytes);
+        bulk_g2s(ring + (size_t)s * 2 * row_bytes, (const T*)a.x + row * a.x_stride, row_bytes, &full[s]);
+        bulk_g2s(ring + (size_t)s * 2 * row_bytes + row_bytes, (const T*)a.dy + row * a.dy_stride, row_bytes, &full[s]);
+    };
+    if (t == 0) {
+        failed_flag = 0;
+        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+        for (int s = 0; s < stages && s < n_here; ++s) fetch(s, s);
+    }
+    float w[NC][VE], dw[NC][VE], db[NC][VE];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int e0 = (t + c * G) * VE;
+        if (a.w != nullptr) {
+            load_params<P, VE>((const P*)a.w, e0, a.dim, w[c]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) w[c][i] = 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) dw[c][i] = db[c][i] = 0.f;
+    }
+    __syncthreads();
+    int s = 0, flip = 0;
+    uint32_t phase = 0;
+    float2 st = a.stats[blockIdx.x];
+    for (int64_t i = 0; i < n_here; ++i) {
+        const int64_t row = blockIdx.x + i * gridDim.x;
+        const float2 now = st;
+        if (i + 1 < n_here) st = a.stats[row + gridDim.x];
+        // a wait that ran out (it cannot, short of a broken copy) makes this row and the sums NaN and goes on
+        const float ok = mbar_wait(&full[s], phase, failed, polls) ? 0.f : __uint_as_float(kNaNBits);
+        const uint4* sx = (const uint4*)(ring + (size_t)s * 2 * row_bytes);
+        const uint4* sg = (const uint4*)(ring + (size_t)s * 2 * row_bytes + row_bytes);
+        float xh[NC][VE], g[NC][VE];
+        float s1 = ok, s2 = ok;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = t + c * G;
+            if (at * VE < a.dim) {
+                unpack16(sx[at], xh[c], (const T*)nullptr);
+                unpack16(sg[at], g[c], (const T*)nullptr);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; ++k) xh[c][k] = g[c][k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                xh[c][k] = (xh[c][k] - now.x) * now.y;       // beyond the row g is 0, so xh there counts for nothing
+                dw[c][k] += g[c][k] * xh[c][k] + ok;
+                db[c][k] += g[c][k] + ok;
+                g[c][k] *= w[c][k];
+                s1 += g[c][k];
+                s2 += g[c][k] * xh[c][k];
+            }
+        }
+        s1 = warp_sum(s1);
+        s2 = warp_sum(s2);
+        float *r1 = red[flip], *r2 = red[flip + 2];
+        flip ^= 1;
+        if (lane == 0) r1[warp] = s1, r2[warp] = s2;
+        __syncthreads();
+        // every thread has this stage in registers
+        if (t == 0 && i + stages < n_here) fetch(i + stages, s);
+        const float m1 = warp_sum(lane < nwarps ? r1[lane] : 0.f) * inv_n, m2 = warp_sum(lane < nwarps ? r2[lane] : 0.f) * inv_n;
+        if (a.dx != nullptr) {
+            T* dxr = (T*)a.dx + row * a.dim;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float o[VE];
+#pragma unroll
+                for (int k = 0; k < VE; ++k) o[k] = now.y * (g[c][k] - m1 - xh[c][k] * m2);
+                store_values<T, VE>(dxr, (t + c * G) * VE, a.dim, o);
+            }
+        }
+        if (++s == stages) s = 0, phase ^= 1;
+    }
+    if (failed_flag && t == 0) {
+        // let the copies still on their way land before the block gives up its shared memory
+        for (int64_t i = max((int64_t)0, n_here - stages); i < n_here; ++i) mbar_drain(&full[i % stages], (uint32_t)(i / stages) & 1, polls);
+    }
+    if (a.part == nullptr) return;
+    float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int e0 = (t + c * G) * VE;
+        if (e0 >= a.dim) continue;
+#pragma unroll
+        for (int k = 0; k < VE; k += 4) {
+            *(float4*)(out + e0 + k) = make_float4(dw[c][k], dw[c][k + 1], dw[c][k + 2], dw[c][k + 3]);
+            *(float4*)(out + a.dim + e0 + k) = make_float4(db[c][k], db[c][k + 1], db[c][k + 2], db[c][k + 3]);
+        }
+    }
+}
+
 // Rows too long for registers: dx alone, one block per row.
 template <typename T, typename P>
 __global__ void ln_bwd_long_kernel(LnBwdArgs a) {
@@ -325,24 +461,34 @@ __global__ void ln_bwd_cols_kernel(LnBwdArgs a, int64_t rows_per_part) {
     a.part[(int64_t)blockIdx.y * 2 * a.dim + a.dim + e] = db;
 }
 
-// Partial sums [parts][2][dim] -> dw, db: 32 columns per block, thread row y adds parts y, y + 8, ... and the eight sums are
-// added in order.
+// Partial sums [parts][2][dim] -> dw, db: 32 columns per block, thread row y adds parts y, y + 32, ... and the sums of the thread
+// rows are added by a tree.
 template <typename P>
-__global__ void ln_param_reduce_kernel(const float* __restrict__ part, int parts, int64_t dim, P* __restrict__ dw, P* __restrict__ db) {
-    __shared__ float sm[8][33];
+__global__ void __launch_bounds__(1024) ln_param_reduce_kernel(const float* __restrict__ part, int parts, int64_t dim, P* __restrict__ dw,
+                                                               P* __restrict__ db) {
+    __shared__ float sm[32][33];
     const int64_t e = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
-    if (e < 2 * dim)
-        for (int p = threadIdx.y; p < parts; p += 8) s += part[(int64_t)p * 2 * dim + e];
+    if (e < 2 * dim) {
+        const float* src = part + e;
+        const int64_t step = 2 * dim;
+        int p = threadIdx.y;
+        for (; p + 96 < parts; p += 128) {
+            const float a = src[p * step], b = src[(p + 32) * step], c = src[(p + 64) * step], d = src[(p + 96) * step];
+            s += a, s += b, s += c, s += d;
+        }
+        for (; p < parts; p += 32) s += src[p * step];
+    }
     sm[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && e < 2 * dim) {
-#pragma unroll
-        for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
-        if (e < dim) {
-            if (dw != nullptr) dw[e] = from_f32<P>(s);
+    // thread row y has column y of the 32 x 32 sums, one per lane
+    s = warp_sum(sm[threadIdx.x][threadIdx.y]);
+    const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && col < 2 * dim) {
+        if (col < dim) {
+            if (dw != nullptr) dw[col] = from_f32<P>(s);
         } else if (db != nullptr) {
-            db[e - dim] = from_f32<P>(s);
+            db[col - dim] = from_f32<P>(s);
         }
     }
 }
@@ -385,7 +531,7 @@ static int ln_fwd(const LnArgs& a, void* y, float2* stats, cudaStream_t st) {
 // Blocks of the backward kernel (= partial sums) for rows a thread can hold, and threads per block.
 struct LnBwdShape {
     bool fits, warp;
-    int nc, threads, grid;
+    int nc, threads, grid, stages;
 };
 static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int ve) {
     LnBwdShape s{};
@@ -406,7 +552,11 @@ static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int ve) {
     } else {
         s.threads = (int)std::min<int64_t>(kLnBwdMaxThreads, std::max(64, pow2_at_least((acc + ncmax - 1) / ncmax)));
         s.nc = pow2_at_least((acc + s.threads - 1) / s.threads);
-        s.grid = (int)std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)kNumSM * (1024 / s.threads)));
+        const int per_sm = std::max(1, kLnBwdThreadsPerSM / s.threads);
+        // a block has eight rows or more, so that its partial sums are a small part of its traffic
+        s.grid = (int)std::max<int64_t>(std::min<int64_t>(rows, kNumSM), std::min<int64_t>((rows + 7) / 8, (int64_t)kNumSM * per_sm));
+        s.grid = std::max(1, s.grid);
+        if (ve > 1) s.stages = (int)std::min<int64_t>(kLnRingStages, kLnRingBytes / per_sm / (2 * acc * 16));
     }
     return s;
 }
@@ -427,6 +577,15 @@ static void ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t 
 #undef CGB_LN_BWD
 }
 
+template <typename T, typename P, int NC>
+static int ln_bwd_ring(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
+    const size_t smem = (size_t)s.stages * 2 * a.dim * sizeof(T);
+    auto kern = ln_bwd_ring_kernel<T, P, NC>;
+    CGB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kern<<<s.grid, s.threads, smem, st>>>(a, s.stages, kDefaultWaitPolls);
+    return CGB200_OK;
+}
+
 template <typename T, typename P>
 static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
     constexpr int N = Chunk<T>::N;
@@ -437,7 +596,13 @@ static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
         if (s.fits) {
             launch_begin(K_LN_BWD, st);
             if (vec && s.warp) ln_bwd_launch<T, P, N, true>(s, a, st);
-            else if (vec) ln_bwd_launch<T, P, N, false>(s, a, st);
+            else if (vec) {
+                int rc = CGB200_OK;
+                if (s.nc == 1) rc = ln_bwd_ring<T, P, 1>(s, a, st);
+                else if (s.nc == 2) rc = ln_bwd_ring<T, P, 2>(s, a, st);
+                else if constexpr (N == 4) rc = ln_bwd_ring<T, P, 4>(s, a, st);
+                if (rc != CGB200_OK) return rc;
+            }
             else if (s.warp) ln_bwd_launch<T, P, 1, true>(s, a, st);
             else ln_bwd_launch<T, P, 1, false>(s, a, st);
             launch_end(K_LN_BWD, st);
@@ -457,7 +622,7 @@ static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
     }
     if (a.part != nullptr) {
         launch_begin(K_LN_REDUCE, st);
-        ln_param_reduce_kernel<P><<<(unsigned)((2 * a.dim + 31) / 32), dim3(32, 8), 0, st>>>(a.part, a.rows > 0 ? s.grid : 0, a.dim, (P*)dw, (P*)db);
+        ln_param_reduce_kernel<P><<<(unsigned)((2 * a.dim + 31) / 32), dim3(32, 32), 0, st>>>(a.part, a.rows > 0 ? s.grid : 0, a.dim, (P*)dw, (P*)db);
         launch_end(K_LN_REDUCE, st);
         CGB_CUDA(cudaGetLastError());
     }

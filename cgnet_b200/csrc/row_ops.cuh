@@ -109,17 +109,44 @@ __device__ __forceinline__ void store_chunk(T* row, int64_t e0, int64_t n, const
             if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = from_f32<T>(v[i]);
     }
 }
-// N parameter values (of any of the three types) from value e0 on
+// N parameter values (of any of the three types) from value e0 on, as they lie in memory (zeros outside [0, n)), and as float32.
 template <typename P, int N>
-__device__ __forceinline__ void load_params(const P* w, int64_t e0, int64_t n, float (&v)[N]) {
-    if (N * sizeof(P) % 16 == 0 && e0 >= 0 && e0 + N <= n && aligned16(w + e0)) {
+struct Params {
+    static constexpr int W = N * (int)sizeof(P) / 16;
+    uint4 u[W];
+    __device__ __forceinline__ void load(const P* w, int64_t e0, int64_t n) {
+        if (e0 >= 0 && e0 + N <= n && aligned16(w + e0)) {
 #pragma unroll
-        for (int c = 0; c < (int)(N * sizeof(P) / 16); ++c) {
+            for (int c = 0; c < W; ++c) u[c] = *(reinterpret_cast<const uint4*>(w + e0) + c);
+        } else {
+#pragma unroll
+            for (int c = 0; c < W; ++c) {
+                float t[Chunk<P>::N];
+#pragma unroll
+                for (int i = 0; i < Chunk<P>::N; ++i) {
+                    const int64_t e = e0 + c * Chunk<P>::N + i;
+                    t[i] = e >= 0 && e < n ? to_f32(w[e]) : 0.f;
+                }
+                u[c] = pack16(t, (const P*)nullptr);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
             float t[Chunk<P>::N];
-            unpack16(*(reinterpret_cast<const uint4*>(w + e0) + c), t, (const P*)nullptr);
+            unpack16(u[c], t, (const P*)nullptr);
 #pragma unroll
             for (int i = 0; i < Chunk<P>::N; ++i) v[c * Chunk<P>::N + i] = t[i];
         }
+    }
+};
+template <typename P, int N>
+__device__ __forceinline__ void load_params(const P* w, int64_t e0, int64_t n, float (&v)[N]) {
+    if constexpr (N * sizeof(P) % 16 == 0) {
+        Params<P, N> p;
+        p.load(w, e0, n);
+        p.get(v);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(w[e0 + i]) : 0.f;
