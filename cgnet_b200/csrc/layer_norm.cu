@@ -32,30 +32,42 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
     return WARP ? warp_sum(v) : block_sum(v, buf);
 }
 
-// One row per warp (WARP) or per block; its values stay in registers between the three steps, so x is read once.
-template <typename T, typename P, int CH, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, T* __restrict__ y, float2* __restrict__ stats) {
+// One row per warp (WARP) or per block; its values stay in registers between the three steps, so x is read once, and everything
+// the row needs is on its way before the first value is waited for.  EDGE: rows (or weight and bias) that do not start on 16-byte
+// boundaries or do not end on them; without it every chunk is inside the row or behind it.
+template <typename T, typename P, int CH, bool WARP, bool EDGE>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, float inv_n, T* __restrict__ y, float2* __restrict__ stats) {
     constexpr int N = Chunk<T>::N;
     __shared__ float red[2][32];
-    const int G = WARP ? 32 : (int)blockDim.x;
-    const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-    const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    __shared__ uint4 last[EDGE && !WARP ? 32 : 1];     // each warp's last chunk, for the next warp
+    const int lane = threadIdx.x & 31, warp = (int)(threadIdx.x >> 5), n = (int)a.dim;
+    const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
     if (row >= a.rows) return;               // whole warps or whole blocks leave
     const T* xr = (const T*)a.x + row * a.x_stride;
     T* yr = y + row * a.dim;
-    const int ph = row_phase(xr);
-    // everything the row needs is on its way before the first value is waited for
+    const int k0 = WARP ? 0 : warp * 32 * CH, k = k0 + lane;       // this thread's first chunk, the next ones are 32 further
     uint4 raw[CH];
     Params<P, N> w[CH], b[CH];
-#pragma unroll
-    for (int c = 0; c < CH; ++c) raw[c] = load_raw(xr, (t + c * G) * N - ph, a.dim, 0.f);
-    if (CH <= 2) {
+    auto load_wb = [&]() {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (a.w != nullptr) w[c].load((const P*)a.w, (t + c * G) * N - ph, a.dim);
-            if (a.b != nullptr) b[c].load((const P*)a.b, (t + c * G) * N - ph, a.dim);
+            const int e0 = (k + 32 * c) * N;
+            if (EDGE) {
+                if (a.w != nullptr) w[c].load((const P*)a.w, e0, n);
+                if (a.b != nullptr) b[c].load((const P*)a.b, e0, n);
+            } else if (e0 < n) {
+                if (a.w != nullptr) w[c].load_aligned((const P*)a.w + e0);
+                if (a.b != nullptr) b[c].load_aligned((const P*)a.b + e0);
+            }
         }
+    };
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e0 = (k + 32 * c) * N;
+        if (EDGE) raw[c] = load_at(xr, row_phase(xr), k + 32 * c, n);
+        else raw[c] = e0 < n ? *reinterpret_cast<const uint4*>(xr + e0) : make_uint4(0, 0, 0, 0);
     }
+    if (CH <= 2) load_wb();
     float v[CH][N];
     float s = 0.f;
 #pragma unroll
@@ -64,42 +76,57 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, T* 
 #pragma unroll
         for (int i = 0; i < N; ++i) s += v[c][i];
     }
-    const float mean = row_sum<WARP>(s, red[0]) / (float)a.dim;
+    const float mean = row_sum<WARP>(s, red[0]) * inv_n;
     float q = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int64_t e0 = (int64_t)(t + c * G) * N - ph;
-        const bool full = e0 >= 0 && e0 + N <= a.dim;
+        const int e0 = (k + 32 * c) * N;
+        if (EDGE ? e0 + N > n : e0 >= n) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[c][i] = EDGE && e0 + i < n ? v[c][i] : mean;     // counts for nothing
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             v[c][i] -= mean;
-            if (full || (e0 + i >= 0 && e0 + i < a.dim)) q += v[c][i] * v[c][i];
+            q = fmaf(v[c][i], v[c][i], q);
         }
     }
-    const float rstd = 1.f / sqrtf(row_sum<WARP>(q, red[1]) / (float)a.dim + a.eps);
-    if (stats != nullptr && t == 0) stats[row] = make_float2(mean, rstd);
-    if (CH > 2) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            if (a.w != nullptr) w[c].load((const P*)a.w, (t + c * G) * N - ph, a.dim);
-            if (a.b != nullptr) b[c].load((const P*)a.b, (t + c * G) * N - ph, a.dim);
-        }
-    }
+    const float rstd = 1.f / sqrtf(row_sum<WARP>(q, red[1]) * inv_n + a.eps);
+    if (stats != nullptr && (WARP ? lane : (int)threadIdx.x) == 0) stats[row] = make_float2(mean, rstd);
+    if (CH > 2) load_wb();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e0 = (t + c * G) * N - ph;
-        if (e0 >= a.dim) continue;
+        const int e0 = (k + 32 * c) * N;
         float wv[N], bv[N];
-        if (a.w != nullptr) w[c].get(wv);
-        if (a.b != nullptr) b[c].get(bv);
+        if (a.w != nullptr) {
+            w[c].get(wv);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float o = v[c][i] * rstd;
-            if (a.w != nullptr) o *= wv[i];
-            if (a.b != nullptr) o += bv[i];
-            v[c][i] = o;
+            for (int i = 0; i < N; ++i) v[c][i] *= rstd * wv[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[c][i] *= rstd;
         }
-        store_chunk(yr, e0, a.dim, v[c]);
+        if (a.b != nullptr) {
+            b[c].get(bv);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[c][i] += bv[i];
+        }
+        raw[c] = pack16(v[c], (const T*)nullptr);
+        if (!EDGE && e0 < n) *reinterpret_cast<uint4*>(yr + e0) = raw[c];
+    }
+    if (EDGE) {
+        uint4 before = raw[0];
+        if (!WARP) {
+            if (lane == 31) last[warp] = raw[CH - 1];
+            __syncthreads();
+            if (warp > 0) before = last[warp - 1];
+        }
+        store_groups<T, CH>(yr, row_phase(yr), k0, n, raw, before);
+        // the row's last values, where they are this warp's last chunk's and the group behind it is no one's
+        if (lane == 31 && (WARP || warp == (int)(blockDim.x >> 5) - 1)) {
+            const int tail = (k0 + 32 * CH) * N - row_phase(yr);
+            if (tail < n) store_pieces(yr, tail, n, shifted(raw[CH - 1], raw[CH - 1], (N - row_phase(yr)) * (int)sizeof(T)));
+        }
     }
 }
 
@@ -185,24 +212,19 @@ __device__ __forceinline__ void store_values(T* p, int64_t e0, int64_t n, const 
     }
 }
 
-// A thread owns the same columns of every row its warp (WARP) or block visits, so the sums over rows stay in registers
-// until the end: x and dy are read once for all three gradients.  VE values per access (16 bytes, or one value where rows do
-// not start on 16-byte boundaries), NC accesses.  Each block leaves one partial sum per column; ln_param_reduce_kernel
-// adds them in block order, so the result does not depend on timing.
-template <typename T, typename P, int VE, int NC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(LnBwdArgs a) {
+// A lane owns the same columns of every row its warp visits, so the sums over rows stay in registers until the end: x and dy are
+// read once for all three gradients.  VE values per access (16 bytes, or one value where rows do not start on 16-byte
+// boundaries), NC accesses.  Each block leaves one partial sum per column; ln_param_reduce_kernel adds them, so the result does
+// not depend on timing.
+template <typename T, typename P, int VE, int NC>
+__global__ void __launch_bounds__(256) ln_bwd_kernel(LnBwdArgs a) {
     extern __shared__ float sm[];
-    __shared__ float red[4][32];
-    const int G = WARP ? 32 : (int)blockDim.x;
-    const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-    const int warp = threadIdx.x >> 5, nwarps = (int)(blockDim.x >> 5);
-    const int64_t row0 = WARP ? (int64_t)blockIdx.x * nwarps + warp : (int64_t)blockIdx.x;
-    const int64_t step = WARP ? (int64_t)gridDim.x * nwarps : (int64_t)gridDim.x;
+    const int t = (int)(threadIdx.x & 31), warp = threadIdx.x >> 5, nwarps = (int)(blockDim.x >> 5);
     const float inv_n = 1.f / (float)a.dim;
     float w[NC][VE], dw[NC][VE], db[NC][VE];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int64_t e0 = (int64_t)(t + c * G) * VE;
+        const int64_t e0 = (int64_t)(t + c * 32) * VE;
         if (a.w != nullptr) {
             load_params<P, VE>((const P*)a.w, e0, a.dim, w[c]);
         } else {
@@ -212,8 +234,7 @@ __global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(L
 #pragma unroll
         for (int i = 0; i < VE; ++i) dw[c][i] = db[c][i] = 0.f;
     }
-    int flip = 0;
-    for (int64_t row = row0; row < a.rows; row += step) {
+    for (int64_t row = (int64_t)blockIdx.x * nwarps + warp; row < a.rows; row += (int64_t)gridDim.x * nwarps) {
         const T* xr = (const T*)a.x + row * a.x_stride;
         const T* gr = (const T*)a.dy + row * a.dy_stride;
         const float2 st = a.stats[row];
@@ -221,7 +242,7 @@ __global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(L
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int64_t e0 = (int64_t)(t + c * G) * VE;
+            const int64_t e0 = (int64_t)(t + c * 32) * VE;
             load_values<T, VE>(xr, e0, a.dim, xh[c]);
             load_values<T, VE>(gr, e0, a.dim, g[c]);
         }
@@ -230,58 +251,34 @@ __global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(L
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
                 xh[c][i] = (xh[c][i] - st.x) * st.y;     // beyond the row g is 0, so xh there counts for nothing
-                dw[c][i] += g[c][i] * xh[c][i];
+                dw[c][i] = fmaf(g[c][i], xh[c][i], dw[c][i]);
                 db[c][i] += g[c][i];
                 g[c][i] *= w[c][i];
                 s1 += g[c][i];
-                s2 += g[c][i] * xh[c][i];
+                s2 = fmaf(g[c][i], xh[c][i], s2);
             }
         }
         if (a.dx != nullptr) {
-            float m1, m2;
-            if (WARP) {
-                m1 = warp_sum(s1) * inv_n;
-                m2 = warp_sum(s2) * inv_n;
-            } else {
-                s1 = warp_sum(s1);
-                s2 = warp_sum(s2);
-                float* r1 = red[flip], *r2 = red[flip + 2];
-                flip ^= 1;
-                if ((threadIdx.x & 31) == 0) r1[warp] = s1, r2[warp] = s2;
-                __syncthreads();
-                const int lane = threadIdx.x & 31;
-                m1 = warp_sum(lane < nwarps ? r1[lane] : 0.f) * inv_n;
-                m2 = warp_sum(lane < nwarps ? r2[lane] : 0.f) * inv_n;
-            }
+            const float m1 = warp_sum(s1) * inv_n, m2 = warp_sum(s2) * inv_n;
             T* dxr = (T*)a.dx + row * a.dim;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 float o[VE];
 #pragma unroll
                 for (int i = 0; i < VE; ++i) o[i] = st.y * (g[c][i] - m1 - xh[c][i] * m2);
-                store_values<T, VE>(dxr, (int64_t)(t + c * G) * VE, a.dim, o);
+                store_values<T, VE>(dxr, (int64_t)(t + c * 32) * VE, a.dim, o);
             }
         }
     }
     if (a.part == nullptr) return;
     float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
-    if (!WARP) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const int64_t e = (int64_t)(t + c * G) * VE + i;
-                if (e < a.dim) out[e] = dw[c][i], out[a.dim + e] = db[c][i];
-            }
-        return;
-    }
     // the block's warps, in order
     const int n2 = 2 * (int)a.dim;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-            const int e = (t + c * G) * VE + i;
+            const int e = (t + c * 32) * VE + i;
             if (e < a.dim) sm[warp * n2 + e] = dw[c][i], sm[warp * n2 + (int)a.dim + e] = db[c][i];
         }
     __syncthreads();
@@ -292,29 +289,66 @@ __global__ void __launch_bounds__(WARP ? 256 : kLnBwdMaxThreads) ln_bwd_kernel(L
     }
 }
 
-// The same for aligned rows of a block, which come through shared memory: a ring of `stages` rows of x and dy, filled by the
-// bulk copies of one thread, keeps reads in flight across the two barriers of a row.
+// The same for rows of a block, which come through shared memory: a ring of `stages` rows of x and dy, filled by the bulk copies of
+// one thread, keeps reads in flight across the barriers of a row.  Bulk copies move whole 16-byte groups.  EDGE: rows start
+// anywhere; a copy then takes the groups the row lies in, with values of its neighbours at both ends, except for the matrix's
+// first and last row (and rows that overlap), where the groups at the ends are read value by value.
 constexpr size_t kLnRingBytes = 200 * 1024;     // of the blocks of an SM together
 constexpr int kLnRingStages = 8;
 constexpr int kLnBwdThreadsPerSM = 512;         // of these kernels: 128 registers a thread
 
-template <typename T, typename P, int NC>
+// Groups a row of n values can touch, wherever it starts
+template <typename T>
+static __host__ __device__ int ring_groups(int64_t n, bool edge) {
+    constexpr int N = Chunk<T>::N;
+    return (int)((n + (edge ? N - 1 : 0) + N - 1) / N);
+}
+// What the ring holds of a row, and where: groups [g0, g1) of those that start `ph` values before it.
+struct RingRow {
+    int ph, g0, g1;
+};
+template <typename T, bool EDGE>
+__device__ __forceinline__ RingRow ring_row(const T* r, int64_t row, int64_t rows, int64_t stride, int n) {
+    constexpr int N = Chunk<T>::N;
+    if (!EDGE) return RingRow{0, 0, n / N};
+    const int ph = row_phase(r);
+    return RingRow{ph, ph > 0 && (row == 0 || stride < n) ? 1 : 0, row == rows - 1 || stride < n ? (ph + n) / N : (ph + n + N - 1) / N};
+}
+template <typename T, bool EDGE>
+__device__ __forceinline__ uint4 ring_at(const uint4* slot, const RingRow& q, const T* r, int k, int n) {
+    constexpr int N = Chunk<T>::N;
+    if (!EDGE) return slot[k];
+    const uint4 lo = k >= q.g0 && k < q.g1 ? slot[k] : load_group(r, q.ph, k, n);
+    if (q.ph == 0) return lo;
+    const int j = k + 1;
+    const uint4 hi = j >= q.g0 && j < q.g1 ? slot[j] : load_group(r, q.ph, j, n);
+    return shifted(lo, hi, q.ph * (int)sizeof(T));
+}
+
+template <typename T, typename P, int NC, bool EDGE>
 __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs a, int stages, uint32_t polls) {
     constexpr int VE = Chunk<T>::N;
     extern __shared__ __align__(128) char ring[];
     __shared__ float red[4][32];
+    __shared__ uint4 last[EDGE ? kLnBwdMaxThreads / 32 : 1];
     __shared__ uint64_t full[kLnRingStages];
     __shared__ int failed_flag;
     volatile int* failed = &failed_flag;
-    const int G = (int)blockDim.x, t = (int)threadIdx.x, warp = t >> 5, lane = t & 31, nwarps = G >> 5;
-    const uint32_t row_bytes = (uint32_t)(a.dim * sizeof(T));
+    const int t = (int)threadIdx.x, warp = t >> 5, lane = t & 31, nwarps = (int)(blockDim.x >> 5), n = (int)a.dim;
+    const int k0 = warp * 32 * NC, k = k0 + lane;          // this thread's first chunk, the next ones are 32 further
+    const int slot = ring_groups<T>(a.dim, EDGE);           // groups of a row in the ring
     const float inv_n = 1.f / (float)a.dim;
     const int64_t n_here = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;      // rows blockIdx.x, + gridDim.x, ...
+    auto place = [&](int s) { return (uint4*)ring + (size_t)s * 2 * slot; };
     auto fetch = [&](int64_t i, int s) {
         const int64_t row = blockIdx.x + i * gridDim.x;
-        mbar_arrive_expect_tx(&full[s], 2 * row_bytes);
-        bulk_g2s(ring + (size_t)s * 2 * row_bytes, (const T*)a.x + row * a.x_stride, row_bytes, &full[s]);
-        bulk_g2s(ring + (size_t)s * 2 * row_bytes + row_bytes, (const T*)a.dy + row * a.dy_stride, row_bytes, &full[s]);
+        const T* xr = (const T*)a.x + row * a.x_stride;
+        const T* gr = (const T*)a.dy + row * a.dy_stride;
+        const RingRow qx = ring_row<T, EDGE>(xr, row, a.rows, a.x_stride, n), qg = ring_row<T, EDGE>(gr, row, a.rows, a.dy_stride, n);
+        const uint32_t bx = (uint32_t)max(0, qx.g1 - qx.g0) * 16, bg = (uint32_t)max(0, qg.g1 - qg.g0) * 16;
+        mbar_arrive_expect_tx(&full[s], bx + bg);
+        if (bx > 0) bulk_g2s(place(s) + qx.g0, xr + (qx.g0 * VE - qx.ph), bx, &full[s]);
+        if (bg > 0) bulk_g2s(place(s) + slot + qg.g0, gr + (qg.g0 * VE - qg.ph), bg, &full[s]);
     };
     if (t == 0) {
         failed_flag = 0;
@@ -325,7 +359,7 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
     float w[NC][VE], dw[NC][VE], db[NC][VE];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int e0 = (t + c * G) * VE;
+        const int e0 = (k + 32 * c) * VE;
         if (a.w != nullptr) {
             load_params<P, VE>((const P*)a.w, e0, a.dim, w[c]);
         } else {
@@ -345,29 +379,36 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         if (i + 1 < n_here) st = a.stats[row + gridDim.x];
         // a wait that ran out (it cannot, short of a broken copy) makes this row and the sums NaN and goes on
         const float ok = mbar_wait(&full[s], phase, failed, polls) ? 0.f : __uint_as_float(kNaNBits);
-        const uint4* sx = (const uint4*)(ring + (size_t)s * 2 * row_bytes);
-        const uint4* sg = (const uint4*)(ring + (size_t)s * 2 * row_bytes + row_bytes);
+        const T* xr = (const T*)a.x + row * a.x_stride;
+        const T* gr = (const T*)a.dy + row * a.dy_stride;
+        const RingRow qx = ring_row<T, EDGE>(xr, row, a.rows, a.x_stride, n), qg = ring_row<T, EDGE>(gr, row, a.rows, a.dy_stride, n);
         float xh[NC][VE], g[NC][VE];
         float s1 = ok, s2 = ok;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int at = t + c * G;
-            if (at * VE < a.dim) {
-                unpack16(sx[at], xh[c], (const T*)nullptr);
-                unpack16(sg[at], g[c], (const T*)nullptr);
+            const int at = k + 32 * c;
+            if (at * VE < n) {
+                unpack16(ring_at<T, EDGE>(place(s), qx, xr, at, n), xh[c], (const T*)nullptr);
+                unpack16(ring_at<T, EDGE>(place(s) + slot, qg, gr, at, n), g[c], (const T*)nullptr);
+                if (EDGE && (at + 1) * VE > n) {
+#pragma unroll
+                    for (int j = 0; j < VE; ++j)
+                        if (at * VE + j >= n) xh[c][j] = g[c][j] = 0.f;
+                }
             } else {
 #pragma unroll
-                for (int k = 0; k < VE; ++k) xh[c][k] = g[c][k] = 0.f;
+                for (int j = 0; j < VE; ++j) xh[c][j] = g[c][j] = 0.f;
             }
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                xh[c][k] = (xh[c][k] - now.x) * now.y;       // beyond the row g is 0, so xh there counts for nothing
-                dw[c][k] += g[c][k] * xh[c][k] + ok;
-                db[c][k] += g[c][k] + ok;
-                g[c][k] *= w[c][k];
-                s1 += g[c][k];
-                s2 += g[c][k] * xh[c][k];
+            for (int j = 0; j < VE; ++j) {
+                xh[c][j] = (xh[c][j] - now.x) * now.y;       // beyond the row g is 0, so xh there counts for nothing
+                dw[c][j] = fmaf(g[c][j], xh[c][j], dw[c][j]);
+                db[c][j] += g[c][j];
+                g[c][j] *= w[c][j];
+                s1 += g[c][j];
+                s2 = fmaf(g[c][j], xh[c][j], s2);
             }
+            dw[c][0] += ok, db[c][0] += ok;
         }
         s1 = warp_sum(s1);
         s2 = warp_sum(s2);
@@ -380,12 +421,22 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         const float m1 = warp_sum(lane < nwarps ? r1[lane] : 0.f) * inv_n, m2 = warp_sum(lane < nwarps ? r2[lane] : 0.f) * inv_n;
         if (a.dx != nullptr) {
             T* dxr = (T*)a.dx + row * a.dim;
+            uint4 out[NC];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 float o[VE];
 #pragma unroll
-                for (int k = 0; k < VE; ++k) o[k] = now.y * (g[c][k] - m1 - xh[c][k] * m2);
-                store_values<T, VE>(dxr, (t + c * G) * VE, a.dim, o);
+                for (int j = 0; j < VE; ++j) o[j] = now.y * (g[c][j] - m1 - xh[c][j] * m2);
+                out[c] = pack16(o, (const T*)nullptr);
+                if (!EDGE && (k + 32 * c) * VE < n) *reinterpret_cast<uint4*>(dxr + (k + 32 * c) * VE) = out[c];
+            }
+            if (EDGE) {
+                const int ph = row_phase(dxr);
+                if (lane == 31) last[warp] = out[NC - 1];
+                __syncthreads();          // before the next row's barrier, behind which `last` is written again
+                store_groups<T, NC>(dxr, ph, k0, n, out, warp > 0 ? last[warp - 1] : out[0]);
+                const int tail = (k0 + 32 * NC) * VE - ph;
+                if (lane == 31 && warp == nwarps - 1 && tail < n) store_pieces(dxr, tail, n, shifted(out[NC - 1], out[NC - 1], (VE - ph) * (int)sizeof(T)));
             }
         }
         if (++s == stages) s = 0, phase ^= 1;
@@ -398,13 +449,10 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
     float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int e0 = (t + c * G) * VE;
-        if (e0 >= a.dim) continue;
+        const int e0 = (k + 32 * c) * VE;
 #pragma unroll
-        for (int k = 0; k < VE; k += 4) {
-            *(float4*)(out + e0 + k) = make_float4(dw[c][k], dw[c][k + 1], dw[c][k + 2], dw[c][k + 3]);
-            *(float4*)(out + a.dim + e0 + k) = make_float4(db[c][k], db[c][k + 1], db[c][k + 2], db[c][k + 3]);
-        }
+        for (int j = 0; j < VE; ++j)
+            if (e0 + j < n) out[e0 + j] = dw[c][j], out[a.dim + e0 + j] = db[c][j];
     }
 }
 
@@ -494,12 +542,13 @@ __global__ void __launch_bounds__(1024) ln_param_reduce_kernel(const float* __re
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
-template <typename T, typename P, bool WARP>
+template <typename T, typename P, bool WARP, bool EDGE>
 static void ln_fwd_launch(int ch, unsigned grid, int threads, const LnArgs& a, T* y, float2* stats, cudaStream_t st) {
+    const float inv_n = 1.f / (float)a.dim;
     switch (ch) {
-        case 1: ln_fwd_kernel<T, P, 1, WARP><<<grid, threads, 0, st>>>(a, y, stats); break;
-        case 2: ln_fwd_kernel<T, P, 2, WARP><<<grid, threads, 0, st>>>(a, y, stats); break;
-        default: ln_fwd_kernel<T, P, 4, WARP><<<grid, threads, 0, st>>>(a, y, stats); break;
+        case 1: ln_fwd_kernel<T, P, 1, WARP, EDGE><<<grid, threads, 0, st>>>(a, inv_n, y, stats); break;
+        case 2: ln_fwd_kernel<T, P, 2, WARP, EDGE><<<grid, threads, 0, st>>>(a, inv_n, y, stats); break;
+        default: ln_fwd_kernel<T, P, 4, WARP, EDGE><<<grid, threads, 0, st>>>(a, inv_n, y, stats); break;
     }
 }
 static int pow2_at_least(int64_t n) {
@@ -511,15 +560,20 @@ static int pow2_at_least(int64_t n) {
 template <typename T, typename P>
 static int ln_fwd(const LnArgs& a, void* y, float2* stats, cudaStream_t st) {
     constexpr int N = Chunk<T>::N;
-    const int64_t chunks = (a.dim + N - 1 + N - 1) / N;    // with any phase
+    auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    const bool edge = a.dim % N != 0 || a.x_stride % N != 0 || !at16(a.x) || !at16(y) || !at16(a.w) || !at16(a.b);
+    const int64_t chunks = (a.dim + N - 1) / N;
     launch_begin(K_LN_FWD, st);
     if (chunks <= 32 * kLnMaxChunks) {
         const int ch = pow2_at_least((chunks + 31) / 32);
-        ln_fwd_launch<T, P, true>(ch, (unsigned)((a.rows + 7) / 8), 256, a, (T*)y, stats, st);
+        const unsigned grid = (unsigned)((a.rows + 7) / 8);
+        if (edge) ln_fwd_launch<T, P, true, true>(ch, grid, 256, a, (T*)y, stats, st);
+        else ln_fwd_launch<T, P, true, false>(ch, grid, 256, a, (T*)y, stats, st);
     } else if (chunks <= 1024 * kLnMaxChunks) {
-        // two chunks a thread, four from 2048 chunks on
-        const int threads = (int)std::min<int64_t>(1024, std::max(64, pow2_at_least((chunks + 1) / 2)));
-        ln_fwd_launch<T, P, false>(pow2_at_least((chunks + threads - 1) / threads), (unsigned)a.rows, threads, a, (T*)y, stats, st);
+        // four chunks a thread; two and twice the threads took 39 instead of 31 us at 8192 x 4096 bf16
+        const int ch = kLnMaxChunks, threads = (int)((chunks + 32 * ch - 1) / (32 * ch)) * 32;
+        if (edge) ln_fwd_launch<T, P, false, true>(ch, (unsigned)a.rows, threads, a, (T*)y, stats, st);
+        else ln_fwd_launch<T, P, false, false>(ch, (unsigned)a.rows, threads, a, (T*)y, stats, st);
     } else {
         ln_fwd_long_kernel<T, P><<<(unsigned)a.rows, 1024, 0, st>>>(a, (T*)y, stats);
     }
@@ -531,41 +585,37 @@ static int ln_fwd(const LnArgs& a, void* y, float2* stats, cudaStream_t st) {
 // Blocks of the backward kernel (= partial sums) for rows a thread can hold, and threads per block.
 struct LnBwdShape {
     bool fits, warp;
-    int nc, threads, grid, stages;
+    int nc, threads, grid;
 };
-static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int ve) {
+// N: values of a 16-byte group; vec: rows start and end on those
+static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int N, bool vec) {
     LnBwdShape s{};
-    const int64_t acc = (dim + ve - 1) / ve;      // accesses per row
-    const int ncmax = kLnBwdValues / ve;
-    s.fits = acc <= (int64_t)ncmax * kLnBwdMaxThreads;
-    s.warp = acc <= 32 * ncmax;
+    const int64_t chunks = (dim + N - 1) / N;
+    s.fits = chunks <= (int64_t)kLnBwdValues / N * kLnBwdMaxThreads;
+    s.warp = dim <= 32 * kLnBwdValues;
     if (!s.fits) {
         // column kernel: runs of rows such that about 2048 threads per SM are busy
         const int64_t cols = (dim + 255) / 256;
         s.grid = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(rows, 256), (kNumSM * 8 + cols - 1) / cols));
-        return s;
-    }
-    if (s.warp) {
+    } else if (s.warp) {
         s.threads = 256;
-        s.nc = pow2_at_least((acc + 31) / 32);
+        s.nc = pow2_at_least(((vec ? chunks : dim) + 31) / 32);
         s.grid = (int)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, kNumSM * 4));
     } else {
-        s.threads = (int)std::min<int64_t>(kLnBwdMaxThreads, std::max(64, pow2_at_least((acc + ncmax - 1) / ncmax)));
-        s.nc = pow2_at_least((acc + s.threads - 1) / s.threads);
+        s.threads = (int)((chunks + 32 * (kLnBwdValues / N) - 1) / (32 * (kLnBwdValues / N))) * 32;
         const int per_sm = std::max(1, kLnBwdThreadsPerSM / s.threads);
         // a block has eight rows or more, so that its partial sums are a small part of its traffic
         s.grid = (int)std::max<int64_t>(std::min<int64_t>(rows, kNumSM), std::min<int64_t>((rows + 7) / 8, (int64_t)kNumSM * per_sm));
         s.grid = std::max(1, s.grid);
-        if (ve > 1) s.stages = (int)std::min<int64_t>(kLnRingStages, kLnRingBytes / per_sm / (2 * acc * 16));
     }
     return s;
 }
-template <typename T, typename P, int VE, bool WARP>
+template <typename T, typename P, int VE>
 static void ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
-    const size_t smem = WARP ? (size_t)(s.threads / 32) * 2 * a.dim * sizeof(float) : 0;
-#define CGB_LN_BWD(NC_)                                                                              \
-    if constexpr (NC_ * VE <= kLnBwdValues) {                                                        \
-        ln_bwd_kernel<T, P, VE, NC_, WARP><<<s.grid, s.threads, smem, st>>>(a);                      \
+    const size_t smem = (size_t)(s.threads / 32) * 2 * a.dim * sizeof(float);
+#define CGB_LN_BWD(NC_)                                                                        \
+    if constexpr (NC_ * VE <= kLnBwdValues) {                                                  \
+        ln_bwd_kernel<T, P, VE, NC_><<<s.grid, s.threads, smem, st>>>(a);                      \
     }
     switch (s.nc) {
         case 1: CGB_LN_BWD(1) break;
@@ -577,12 +627,16 @@ static void ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t 
 #undef CGB_LN_BWD
 }
 
-template <typename T, typename P, int NC>
+template <typename T, typename P, bool EDGE>
 static int ln_bwd_ring(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
-    const size_t smem = (size_t)s.stages * 2 * a.dim * sizeof(T);
-    auto kern = ln_bwd_ring_kernel<T, P, NC>;
+    constexpr int NC = kLnBwdValues / Chunk<T>::N;
+    const size_t slots = (size_t)2 * ring_groups<T>(a.dim, EDGE) * 16;
+    const int per_sm = std::max(1, kLnBwdThreadsPerSM / s.threads);
+    const int stages = (int)std::max<size_t>(2, std::min<size_t>(kLnRingStages, kLnRingBytes / per_sm / slots));
+    const size_t smem = stages * slots;
+    auto kern = ln_bwd_ring_kernel<T, P, NC, EDGE>;
     CGB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<s.grid, s.threads, smem, st>>>(a, s.stages, kDefaultWaitPolls);
+    kern<<<s.grid, s.threads, smem, st>>>(a, stages, kDefaultWaitPolls);
     return CGB200_OK;
 }
 
@@ -591,21 +645,17 @@ static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
     constexpr int N = Chunk<T>::N;
     auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     const bool vec = a.dim % N == 0 && a.x_stride % N == 0 && a.dy_stride % N == 0 && at16(a.x) && at16(a.dy) && at16(a.dx);
-    const LnBwdShape s = ln_bwd_shape(a.rows, a.dim, vec ? N : 1);
+    const LnBwdShape s = ln_bwd_shape(a.rows, a.dim, N, vec);
     if (a.rows > 0) {
         if (s.fits) {
+            int rc = CGB200_OK;
             launch_begin(K_LN_BWD, st);
-            if (vec && s.warp) ln_bwd_launch<T, P, N, true>(s, a, st);
-            else if (vec) {
-                int rc = CGB200_OK;
-                if (s.nc == 1) rc = ln_bwd_ring<T, P, 1>(s, a, st);
-                else if (s.nc == 2) rc = ln_bwd_ring<T, P, 2>(s, a, st);
-                else if constexpr (N == 4) rc = ln_bwd_ring<T, P, 4>(s, a, st);
-                if (rc != CGB200_OK) return rc;
-            }
-            else if (s.warp) ln_bwd_launch<T, P, 1, true>(s, a, st);
-            else ln_bwd_launch<T, P, 1, false>(s, a, st);
+            if (vec && s.warp) ln_bwd_launch<T, P, N>(s, a, st);
+            else if (s.warp) ln_bwd_launch<T, P, 1>(s, a, st);
+            else if (vec) rc = ln_bwd_ring<T, P, false>(s, a, st);
+            else rc = ln_bwd_ring<T, P, true>(s, a, st);
             launch_end(K_LN_BWD, st);
+            if (rc != CGB200_OK) return rc;
         } else {
             if (a.dx != nullptr) {
                 launch_begin(K_LN_BWD, st);
@@ -666,9 +716,8 @@ int cgb200_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, c
 
 int64_t cgb200_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int dtype) {
     if (ln_check(rows, dim, dtype, dtype) != CGB200_OK) return -1;
-    // whichever of the two access widths the buffers' alignment will allow
     const int n = dtype == CGB200_F32 ? 4 : 8;
-    const int parts = std::max(ln_bwd_shape(rows, dim, 1).grid, dim % n == 0 ? ln_bwd_shape(rows, dim, n).grid : 0);
+    const int parts = ln_bwd_shape(rows, dim, n, false).grid;
     return (int64_t)parts * 2 * dim * (int64_t)sizeof(float);
 }
 

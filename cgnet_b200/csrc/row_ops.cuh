@@ -81,19 +81,30 @@ __device__ __forceinline__ int row_phase(const T* row) {
 }
 // The 16 bytes of the chunk at value e0 (possibly negative) of a row of n values; values outside the row read as `fill`.  Kept apart
 // from the conversion to float32, so that a thread's chunks are all on their way before the first is waited for.
+//
+// The value-by-value forms are kept out of line: inlined they are predicated, not branched around, and a layer norm whose rows are
+// all aligned issued 640 instructions a chunk because of them (8192 x 4096 bf16: 92 us).
+template <typename T>
+__device__ __noinline__ uint4 load_pieces(const T* row, int64_t e0, int64_t n, float fill) {
+    constexpr int N = Chunk<T>::N;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(row[e0 + i]) : fill;
+    return pack16(v, (const T*)nullptr);      // the values came from this type: nothing is rounded
+}
+template <typename T>
+__device__ __noinline__ void store_pieces(T* row, int64_t e0, int64_t n, uint4 u) {
+    constexpr int N = Chunk<T>::N;
+    T v[N];
+    memcpy(v, &u, 16);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = v[i];
+}
 template <typename T>
 __device__ __forceinline__ uint4 load_raw(const T* row, int64_t e0, int64_t n, float fill) {
-    constexpr int N = Chunk<T>::N;
-    uint4 u;
-    if (e0 >= 0 && e0 + N <= n && aligned16(row + e0)) {
-        u = *reinterpret_cast<const uint4*>(row + e0);
-    } else {
-        float v[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = e0 + i >= 0 && e0 + i < n ? to_f32(row[e0 + i]) : fill;
-        u = pack16(v, (const T*)nullptr);      // the values came from this type: nothing is rounded
-    }
-    return u;
+    if (e0 >= 0 && e0 + Chunk<T>::N <= n && aligned16(row + e0)) return *reinterpret_cast<const uint4*>(row + e0);
+    return load_pieces(row, e0, n, fill);
 }
 template <typename T, int N = Chunk<T>::N>
 __device__ __forceinline__ void load_chunk(const T* row, int64_t e0, int64_t n, float fill, float (&v)[N]) {
@@ -104,31 +115,82 @@ __device__ __forceinline__ void store_chunk(T* row, int64_t e0, int64_t n, const
     if (e0 >= 0 && e0 + N <= n && aligned16(row + e0)) {
         *reinterpret_cast<uint4*>(row + e0) = pack16(v, (const T*)nullptr);
     } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = from_f32<T>(v[i]);
+        store_pieces(row, e0, n, pack16(v, (const T*)nullptr));
     }
 }
+// Columns of rows that start anywhere: a thread owns chunk k = values [k N, k N + N) of every row, and moves them with 16-byte
+// accesses all the same.  To read them it takes the two aligned groups they lie in and shifts; to write them, each thread puts
+// together the aligned group that ends in its chunk, from its neighbour's values and its own.
+
+// 16 bytes from byte `bytes` (0..15, a multiple of 2, the same in the whole warp) of the 32 of lo and hi.
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int bytes) {
+    uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 6; ++j) x[j] = bytes & 8 ? x[j + 2] : x[j];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) x[j] = bytes & 4 ? x[j + 1] : x[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = bytes & 2 ? __funnelshift_r(x[j], x[j + 1], 16) : x[j];
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+// Group g of a row of n values whose aligned groups start `ph` values before it; zeros outside the row.
+template <typename T>
+__device__ __forceinline__ uint4 load_group(const T* row, int ph, int g, int n) {
+    constexpr int N = Chunk<T>::N;
+    const int e0 = g * N - ph;
+    if (e0 >= 0 && e0 + N <= n) return *reinterpret_cast<const uint4*>(row + e0);
+    if (e0 < n) return load_pieces(row, e0, n, 0.f);
+    return make_uint4(0, 0, 0, 0);
+}
+// Chunk k of such a row.
+template <typename T>
+__device__ __forceinline__ uint4 load_at(const T* row, int ph, int k, int n) {
+    const uint4 lo = load_group(row, ph, k, n);
+    if (ph == 0) return lo;
+    return shifted(lo, load_group(row, ph, k + 1, n), ph * (int)sizeof(T));
+}
+// Writes the groups of a row of n values that end in this warp's chunks k0 + lane, k0 + 32 + lane, ... (CH of them, in `u`), `ph` as
+// above.  `before` is the last chunk before this warp's (any value where there is none).  The values of the warp's last
+// chunk that lie in the group behind it are the next warp's, except at the end of the row.
+template <typename T, int CH>
+__device__ __forceinline__ void store_groups(T* row, int ph, int k0, int n, const uint4 (&u)[CH], const uint4& before) {
+    constexpr int N = Chunk<T>::N;
+    const int lane = threadIdx.x & 31;
+    uint4 old = before;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e0 = (k0 + 32 * c + lane) * N - ph;      // first value of the group
+        uint4 out = u[c];
+        if (ph != 0) {
+            // lane 31 hands on what it had one step earlier: that is lane 0's neighbour
+            const uint4 give = lane == 31 ? old : u[c];
+            const int from = (lane + 31) & 31;
+            const uint4 prev = make_uint4(__shfl_sync(0xffffffffu, give.x, from), __shfl_sync(0xffffffffu, give.y, from),
+                                          __shfl_sync(0xffffffffu, give.z, from), __shfl_sync(0xffffffffu, give.w, from));
+            out = shifted(c == 0 && lane == 0 ? before : prev, u[c], (N - ph) * (int)sizeof(T));
+            old = u[c];
+        }
+        if (e0 >= 0 && e0 + N <= n) *reinterpret_cast<uint4*>(row + e0) = out;
+        else if (e0 < n && e0 + N > 0) store_pieces(row, e0, n, out);
+    }
+}
+
 // N parameter values (of any of the three types) from value e0 on, as they lie in memory (zeros outside [0, n)), and as float32.
 template <typename P, int N>
 struct Params {
     static constexpr int W = N * (int)sizeof(P) / 16;
     uint4 u[W];
+    __device__ __forceinline__ void load_aligned(const P* w) {
+#pragma unroll
+        for (int c = 0; c < W; ++c) u[c] = *(reinterpret_cast<const uint4*>(w) + c);
+    }
     __device__ __forceinline__ void load(const P* w, int64_t e0, int64_t n) {
         if (e0 >= 0 && e0 + N <= n && aligned16(w + e0)) {
 #pragma unroll
             for (int c = 0; c < W; ++c) u[c] = *(reinterpret_cast<const uint4*>(w + e0) + c);
         } else {
 #pragma unroll
-            for (int c = 0; c < W; ++c) {
-                float t[Chunk<P>::N];
-#pragma unroll
-                for (int i = 0; i < Chunk<P>::N; ++i) {
-                    const int64_t e = e0 + c * Chunk<P>::N + i;
-                    t[i] = e >= 0 && e < n ? to_f32(w[e]) : 0.f;
-                }
-                u[c] = pack16(t, (const P*)nullptr);
-            }
+            for (int c = 0; c < W; ++c) u[c] = load_pieces(w, e0 + c * Chunk<P>::N, n, 0.f);
         }
     }
     __device__ __forceinline__ void get(float (&v)[N]) const {
