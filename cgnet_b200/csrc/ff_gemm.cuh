@@ -101,6 +101,9 @@ __device__ __forceinline__ float2 activate(int act, float g) {
     return make_float2(c == 0.f ? 0.f : g * c, GRAD ? c + (fabsf(g) > 20.f ? 0.f : g * __expf(-0.5f * g * g) * 0.39894228040143268f) : 0.f);
 }
 
+// The same, one copy of it, for kernels that want short code
+__device__ __noinline__ float2 activate_shared(int act, float g) { return activate<true>(act, g); }
+
 struct FfUnit {
     const FfProblem* p;
     int set, split, k0, k1;

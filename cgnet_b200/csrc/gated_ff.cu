@@ -30,34 +30,50 @@ struct FfArgs {
 // ---- a few rows: one warp per hidden unit, bound by reading the weights ------------------------------------------------
 constexpr int kFfFewRows = 4;
 
-template <typename T, int M>
-__global__ void __launch_bounds__(256) ff_few_rows_kernel(FfArgs a) {
-    constexpr int N = Chunk<T>::N;
+// Four chunks of either weight row are on their way at a time.  EDGE: rows that do not start or end on 16-byte boundaries.
+template <typename T, int M, bool EDGE>
+__global__ void __launch_bounds__(128) ff_few_rows_kernel(FfArgs a) {
+    constexpr int N = Chunk<T>::N, U = 4;
     const int lane = threadIdx.x & 31;
     const int64_t j = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (j >= a.hidden) return;
     const T* wg = (const T*)a.wg + j * a.wg_stride;
     const T* wu = (const T*)a.wu + j * a.wu_stride;
-    const int ph = row_phase(wg);
+    const int pg = EDGE ? row_phase(wg) : 0, pu = EDGE ? row_phase(wu) : 0;
     float g[M], u[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) g[m] = u[m] = 0.f;
-#pragma unroll 4
-    for (int e0 = lane * N - ph; e0 < a.dim; e0 += 32 * N) {
+    auto multiply = [&](const uint4& rg, const uint4& ru, int k) {
         float vg[N], vu[N];
-        load_chunk(wg, e0, a.dim, 0.f, vg);
-        load_chunk(wu, e0, a.dim, 0.f, vu);
+        unpack16(rg, vg, (const T*)nullptr);
+        unpack16(ru, vu, (const T*)nullptr);
 #pragma unroll
         for (int m = 0; m < M; ++m) {
+            const T* x = (const T*)a.x + m * a.x_stride;
             float vx[N];
-            load_chunk((const T*)a.x + m * a.x_stride, e0, a.dim, 0.f, vx);
+            unpack16(EDGE ? load_at(x, row_phase(x), k, a.dim) : *reinterpret_cast<const uint4*>(x + k * N), vx, (const T*)nullptr);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 g[m] = fmaf(vg[i], vx[i], g[m]);
                 u[m] = fmaf(vu[i], vx[i], u[m]);
             }
         }
+    };
+    const int chunks = (a.dim + N - 1) / N;
+    int k = lane;
+    if (!EDGE) {
+        for (; k + (U - 1) * 32 < chunks; k += U * 32) {
+            uint4 rg[U], ru[U];
+#pragma unroll
+            for (int c = 0; c < U; ++c) {
+                rg[c] = __ldcs(reinterpret_cast<const uint4*>(wg) + k + c * 32);
+                ru[c] = __ldcs(reinterpret_cast<const uint4*>(wu) + k + c * 32);
+            }
+#pragma unroll
+            for (int c = 0; c < U; ++c) multiply(rg[c], ru[c], k + c * 32);
+        }
     }
+    for (; k < chunks; k += 32) multiply(load_at(wg, pg, k, a.dim), load_at(wu, pu, k, a.dim), k);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
         g[m] = warp_sum(g[m]);
@@ -72,123 +88,180 @@ __global__ void __launch_bounds__(256) ff_few_rows_kernel(FfArgs a) {
     }
 }
 
-// ---- CUDA-core tiles ---------------------------------------------------------------------------------------------------
-// 64 x 64 outputs per block, 16 terms of the contraction at a time, 4 x 4 outputs per thread; operands of any alignment.
-constexpr int kFfTile = 64, kFfK = 16;
+// ---- CUDA-core tiles: small products, where the time is one chain of loads ----------------------------------------------
+// A block has 32 x 32 outputs.  Its warps share the contraction: each takes a part of it, in slabs of eight terms that it fetches while it
+// multiplies the slab before and keeps in shared memory of its own, so no barrier stands between them; their sums are added in a fixed
+// order at the end, by all threads.  Lane (ly, lx) has outputs 8 ly .. 8 ly + 7 x 4 lx .. 4 lx + 3 of its warp's sums.  Operands
+// of any alignment.  The code is kept short: run once by a few blocks, it is bound by fetching its instructions (unrolled
+// to 16 terms, with the results written by one warp, 52 -> 256 at 100 rows took 12 + 38 us).
+constexpr int kFfTile = 32, kFfSlab = 8, kFfPitch = kFfTile + 4, kFfFwdWarps = 8, kFfBwdWarps = 16;
+constexpr int kFfSumPitch = kFfTile + 1, kFfSums = kFfFwdWarps * kFfTile * kFfSumPitch;      // floats of eight warps' sums
 
-template <typename T>
-__global__ void __launch_bounds__(256) ff_tile_fwd_kernel(FfArgs a) {
-    __shared__ float sx[kFfK][kFfTile + 4], sg[kFfK][kFfTile + 4], su[kFfK][kFfTile + 4];
-    const int64_t m0 = (int64_t)blockIdx.x * kFfTile;
-    const int j0 = blockIdx.y * kFfTile;
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    float g[4][4] = {}, u[4][4] = {};
-    for (int k0 = 0; k0 < a.dim; k0 += kFfK) {
-        const int k = threadIdx.x & 15;
+// acc += slab
+__device__ __forceinline__ void ff_slab(const float (*a)[kFfPitch], const float (*b)[kFfPitch], int ly, int lx, float (&acc)[8][4]) {
+#pragma unroll 4
+    for (int k = 0; k < kFfSlab; ++k) {
+        const float4 a0 = *(const float4*)&a[k][ly * 8], a1 = *(const float4*)&a[k][ly * 8 + 4], b0 = *(const float4*)&b[k][lx * 4];
+        const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, bv[4] = {b0.x, b0.y, b0.z, b0.w};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = (threadIdx.x >> 4) + 16 * r;
-            const bool kin = k0 + k < a.dim;
-            sx[k][i] = kin && m0 + i < a.rows ? to_f32(((const T*)a.x)[(m0 + i) * a.x_stride + k0 + k]) : 0.f;
-            const bool jin = kin && j0 + i < a.hidden;
-            sg[k][i] = jin ? to_f32(((const T*)a.wg)[(int64_t)(j0 + i) * a.wg_stride + k0 + k]) : 0.f;
-            su[k][i] = jin ? to_f32(((const T*)a.wu)[(int64_t)(j0 + i) * a.wu_stride + k0 + k]) : 0.f;
-        }
-        __syncthreads();
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int kk = 0; kk < kFfK; ++kk) {
-            const float4 x = *(const float4*)&sx[kk][ty * 4], wg = *(const float4*)&sg[kk][tx * 4], wu = *(const float4*)&su[kk][tx * 4];
-            const float xv[4] = {x.x, x.y, x.z, x.w}, gv[4] = {wg.x, wg.y, wg.z, wg.w}, uv[4] = {wu.x, wu.y, wu.z, wu.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    g[i][j] = fmaf(xv[i], gv[j], g[i][j]);
-                    u[i][j] = fmaf(xv[i], uv[j], u[i][j]);
-                }
-        }
-        __syncthreads();
+            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
     }
+}
+__device__ __forceinline__ void ff_leave(const float (&acc)[8][4], float* buf, int slot, int ly, int lx) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty * 4 + i;
-            const int c = j0 + tx * 4 + j;
-            if (m >= a.rows || c >= a.hidden) continue;
-            const int64_t at = m * a.hidden + c;
-            ((T*)a.h)[at] = from_f32<T>(activate<false>(a.act, g[i][j]).x * u[i][j]);
-            if (a.gu != nullptr) a.gu[at] = g[i][j], a.gu[a.rows * a.hidden + at] = u[i][j];
-        }
+        for (int j = 0; j < 4; ++j) buf[(slot * kFfTile + ly * 8 + i) * kFfSumPitch + lx * 4 + j] = acc[i][j];
+}
+// Sum of eight warps' values of output (row, col)
+__device__ __forceinline__ float ff_sum(const float* buf, int row, int col) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += buf[(w * kFfTile + row) * kFfSumPitch + col];
+    return s;
 }
 
-// Value (m, c) of dg (c < hidden) or du (c >= hidden) from what the forward kept.
 template <typename T>
-__device__ __forceinline__ float ff_dgu(const FfArgs& a, int64_t m, int c) {
-    const bool up = c >= a.hidden;
-    const int j = up ? c - a.hidden : c;
-    const int64_t at = m * a.hidden + j;
-    const float dh = to_f32(((const T*)a.dh)[m * a.dh_stride + j]);
-    const float2 f = activate<true>(a.act, a.gu[at]);
-    return up ? dh * f.x : dh * a.gu[a.rows * a.hidden + at] * f.y;
+__global__ void __launch_bounds__(kFfFwdWarps * 32) ff_tile_fwd_kernel(FfArgs a) {
+    __shared__ __align__(16) float sums[kFfSums];                         // the slabs lie in the same memory
+    static_assert(kFfSums >= kFfFwdWarps * 3 * kFfSlab * kFfPitch, "the slabs must fit");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ly = lane >> 3, lx = lane & 7;
+    float (*sm)[kFfSlab][kFfPitch] = (float (*)[kFfSlab][kFfPitch])(sums + warp * 3 * kFfSlab * kFfPitch);
+    const int64_t m0 = (int64_t)blockIdx.x * kFfTile;
+    const int j0 = blockIdx.y * kFfTile;
+    const int per = (a.dim + kFfFwdWarps - 1) / kFfFwdWarps, k_lo = warp * per, k_hi = min(a.dim, k_lo + per);
+    const int lk = lane & 7, li = lane >> 3;          // 8 terms x 4 rows a load
+    const T* px = (const T*)a.x + (m0 + li) * a.x_stride + lk;
+    const T* pg = (const T*)a.wg + (int64_t)(j0 + li) * a.wg_stride + lk;
+    const T* pu = (const T*)a.wu + (int64_t)(j0 + li) * a.wu_stride + lk;
+    float x[8], wg[8], wu[8];
+    auto fetch = [&](int k0) {
+        const bool in = k0 + lk < k_hi;
+        const int nx = in ? (int)min((int64_t)kFfTile, a.rows - m0) : 0, nj = in ? min(kFfTile, a.hidden - j0) : 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int i = li + 4 * r;
+            x[r] = i < nx ? to_f32(px[4 * r * a.x_stride + k0]) : 0.f;
+            wg[r] = i < nj ? to_f32(pg[4 * r * a.wg_stride + k0]) : 0.f;
+            wu[r] = i < nj ? to_f32(pu[4 * r * a.wu_stride + k0]) : 0.f;
+        }
+    };
+    float g[8][4] = {}, u[8][4] = {};
+    fetch(k_lo);
+    for (int k0 = k_lo; k0 < k_hi; k0 += kFfSlab) {
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int i = li + 4 * r;
+            sm[0][lk][i] = x[r], sm[1][lk][i] = wg[r], sm[2][lk][i] = wu[r];
+        }
+        __syncwarp();
+        if (k0 + kFfSlab < k_hi) fetch(k0 + kFfSlab);
+        ff_slab(sm[0], sm[1], ly, lx, g);
+        ff_slab(sm[0], sm[2], ly, lx, u);
+    }
+    // row `warp` + 8 i and column `lane` of the tile, i = 0 .. 3
+    float gs[4];
+    __syncthreads();
+    ff_leave(g, sums, warp, ly, lx);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) gs[i] = ff_sum(sums, warp + 8 * i, lane);
+    __syncthreads();
+    ff_leave(u, sums, warp, ly, lx);
+    __syncthreads();
+    const int c = j0 + lane;
+    if (c >= a.hidden) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + warp + 8 * i, at = m * a.hidden + c;
+        if (m >= a.rows) break;
+        const float us = ff_sum(sums, warp + 8 * i, lane);
+        ((T*)a.h)[at] = from_f32<T>(activate_shared(a.act, gs[i]).x * us);
+        if (a.gu != nullptr) a.gu[at] = gs[i], a.gu[a.rows * a.hidden + at] = us;
+    }
 }
 
 // One launch for all gradients: the first `nx` blocks hold tiles of dx, the others tiles of [dWg; dWu].
 template <typename T>
-__global__ void __launch_bounds__(256) ff_tile_bwd_kernel(FfArgs a, int nx, int tiles_d) {
-    __shared__ float sa[kFfK][kFfTile + 4], sb[kFfK][kFfTile + 4];
-    const bool is_dx = (int)blockIdx.x < nx;
-    const int tile = is_dx ? blockIdx.x : blockIdx.x - nx;
+__global__ void __launch_bounds__(kFfBwdWarps * 32) ff_tile_bwd_kernel(FfArgs a, int nx, int tiles_d) {
+    __shared__ __align__(16) float sums[kFfBwdWarps * 2 * kFfSlab * kFfPitch];       // slabs, then the sums of half of the warps
+    static_assert(sizeof(sums) >= kFfSums * sizeof(float), "the sums must fit");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ly = lane >> 3, lx = lane & 7;
+    float (*sm)[kFfSlab][kFfPitch] = (float (*)[kFfSlab][kFfPitch])(sums + warp * 2 * kFfSlab * kFfPitch);
+    const bool dx = (int)blockIdx.x < nx;
+    const int tile = dx ? blockIdx.x : blockIdx.x - nx;
     const int64_t i0 = (int64_t)(tile / tiles_d) * kFfTile;      // row of the output: sample, or hidden unit (g, then u)
     const int d0 = (tile % tiles_d) * kFfTile;
-    const int64_t n_i = is_dx ? a.rows : 2 * (int64_t)a.hidden, n_k = is_dx ? 2 * (int64_t)a.hidden : a.rows;
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < n_k; k0 += kFfK) {
+    const int64_t n_i = dx ? a.rows : 2 * (int64_t)a.hidden, n_k = dx ? 2 * (int64_t)a.hidden : a.rows;
+    const int64_t per = (n_k + kFfBwdWarps - 1) / kFfBwdWarps, k_lo = warp * per, k_hi = min(n_k, k_lo + per);
+    // dx reads dgu along its rows (8 terms x 4 rows a load), dW down its columns: neighbouring lanes take neighbouring addresses
+    const int la = dx ? lane >> 3 : 0, step = dx ? 4 : 1;
+    float gv[8], uv[8], dv[8], bv[8];
+    bool up = false;
+    auto fetch = [&](int64_t k0) {
+        const int64_t unit = dx ? k0 + (lane & 7) : i0 + lane, row = dx ? i0 + la : k0;      // of dgu
+        up = unit >= a.hidden;
+        const int64_t j = up ? unit - a.hidden : unit;
+        const int n = (int)min((int64_t)kFfTile, dx ? (unit < k_hi ? n_i - row : 0) : (unit < n_i ? k_hi - row : 0));
+        const float* g = a.gu + row * a.hidden + j;
+        const float* u = g + a.rows * a.hidden;
+        const T* h = (const T*)a.dh + row * a.dh_stride + j;
+        const int nb = d0 + lane < a.dim ? (int)min((int64_t)kFfSlab, k_hi - k0) : 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            {
-                // dx reads dgu along its rows, dW down its columns: neighbouring threads take neighbouring addresses in both
-                const int k = is_dx ? (threadIdx.x & 15) : (threadIdx.x >> 6) + 4 * r;
-                const int i = is_dx ? (threadIdx.x >> 4) + 16 * r : (threadIdx.x & 63);
-                float v = 0.f;
-                if (k0 + k < n_k && i0 + i < n_i)
-                    v = is_dx ? ff_dgu<T>(a, i0 + i, (int)(k0 + k)) : ff_dgu<T>(a, k0 + k, (int)(i0 + i));
-                sa[k][i] = v;
-            }
-            const int k = (threadIdx.x >> 6) + 4 * r, d = threadIdx.x & 63;
-            float v = 0.f;
-            if (k0 + k < n_k && d0 + d < a.dim) {
-                if (!is_dx) v = to_f32(((const T*)a.x)[(k0 + k) * a.x_stride + d0 + d]);
-                else if (k0 + k < a.hidden) v = to_f32(((const T*)a.wg)[(k0 + k) * a.wg_stride + d0 + d]);
-                else v = to_f32(((const T*)a.wu)[(k0 + k - a.hidden) * a.wu_stride + d0 + d]);
-            }
-            sb[k][d] = v;
+        for (int r = 0; r < 8; ++r) {
+            const int q = step * r;
+            const bool in = q < n;
+            gv[r] = in ? g[(int64_t)q * a.hidden] : 0.f;
+            uv[r] = in && !up ? u[(int64_t)q * a.hidden] : 1.f;
+            dv[r] = in ? to_f32(h[q * a.dh_stride]) : 0.f;
+            const int64_t k = k0 + r;
+            const T* b = !dx ? (const T*)a.x + k * a.x_stride : k < a.hidden ? (const T*)a.wg + k * a.wg_stride : (const T*)a.wu + (k - a.hidden) * a.wu_stride;
+            bv[r] = r < nb ? to_f32(b[d0 + lane]) : 0.f;
         }
-        __syncthreads();
+    };
+    float acc[8][4] = {};
+    fetch(k_lo);
+    for (int64_t k0 = k_lo; k0 < k_hi; k0 += kFfSlab) {
+        __syncwarp();
 #pragma unroll
-        for (int kk = 0; kk < kFfK; ++kk) {
-            const float4 x = *(const float4*)&sa[kk][ty * 4], w = *(const float4*)&sb[kk][tx * 4];
-            const float xv[4] = {x.x, x.y, x.z, x.w}, wv[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
+        for (int r = 0; r < 8; ++r) {
+            const float2 f = activate_shared(a.act, gv[r]);
+            float* s = dx ? &sm[0][lane & 7][la + 4 * r] : &sm[0][r][lane];
+            *s = dv[r] * (up ? f.x : uv[r] * f.y);
+            sm[1][r][lane] = bv[r];
         }
-        __syncthreads();
+        __syncwarp();
+        if (k0 + kFfSlab < k_hi) fetch(k0 + kFfSlab);
+        ff_slab(sm[0], sm[1], ly, lx, acc);
     }
+    // the upper half of the warps hands its sums to the lower half, which then adds up as in the forward
+    __syncthreads();
+    if (warp >= 8) ff_leave(acc, sums, warp - 8, ly, lx);
+    __syncthreads();
+    if (warp < 8) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = i0 + ty * 4 + i;
-            const int d = d0 + tx * 4 + j;
-            if (r >= n_i || d >= a.dim) continue;
-            T* out = is_dx ? (T*)a.dx + r * a.dim : r < a.hidden ? (T*)a.dwg : (T*)a.dwu;
-            if (out == nullptr) continue;
-            if (!is_dx) out += (r < a.hidden ? r : r - a.hidden) * a.dim;
-            out[d] = from_f32<T>(acc[i][j]);
-        }
+            for (int j = 0; j < 4; ++j) acc[i][j] += sums[(warp * kFfTile + ly * 8 + i) * kFfSumPitch + lx * 4 + j];
+    }
+    __syncthreads();
+    if (warp < 8) ff_leave(acc, sums, warp, ly, lx);
+    __syncthreads();
+    const int d = d0 + lane;
+    if (d >= a.dim) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t r = i0 + warp + 16 * i;
+        if (r >= n_i) break;
+        T* out = dx ? (T*)a.dx + r * a.dim : r < a.hidden ? (T*)a.dwg : (T*)a.dwu;
+        if (out == nullptr) continue;
+        if (!dx && r >= a.hidden) out += (r - a.hidden) * a.dim;
+        else if (!dx) out += r * a.dim;
+        out[d] = from_f32<T>(ff_sum(sums, warp + 16 * i, lane));
+    }
 }
 
 // ---- operands of the tensor-core products ------------------------------------------------------------------------------
@@ -511,15 +584,23 @@ static int ff_fwd(const FfArgs& a, const FfPlan& q, char* ws, cudaStream_t st) {
     if (q.tensor) return ff_tensor<T>(a, q, 0, ws, st);
     launch_begin(K_FF_FWD, st);
     if (a.rows <= kFfFewRows) {
-        const unsigned grid = (unsigned)((a.hidden + 7) / 8);
+        const unsigned grid = (unsigned)((a.hidden + 3) / 4);
+        constexpr int N = Chunk<T>::N;
+        const bool edge = a.dim % N != 0 || a.x_stride % N != 0 || a.wg_stride % N != 0 || a.wu_stride % N != 0 ||
+                          ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.wg) | reinterpret_cast<uintptr_t>(a.wu)) & 15) != 0;
+#define CGB_FEW(M_)                                                             \
+    if (edge) ff_few_rows_kernel<T, M_, true><<<grid, 128, 0, st>>>(a);         \
+    else ff_few_rows_kernel<T, M_, false><<<grid, 128, 0, st>>>(a);             \
+    break
         switch (a.rows) {
-            case 1: ff_few_rows_kernel<T, 1><<<grid, 256, 0, st>>>(a); break;
-            case 2: ff_few_rows_kernel<T, 2><<<grid, 256, 0, st>>>(a); break;
-            case 3: ff_few_rows_kernel<T, 3><<<grid, 256, 0, st>>>(a); break;
-            default: ff_few_rows_kernel<T, 4><<<grid, 256, 0, st>>>(a); break;
+            case 1: CGB_FEW(1);
+            case 2: CGB_FEW(2);
+            case 3: CGB_FEW(3);
+            default: CGB_FEW(4);
         }
+#undef CGB_FEW
     } else {
-        ff_tile_fwd_kernel<T><<<dim3((unsigned)((a.rows + kFfTile - 1) / kFfTile), (a.hidden + kFfTile - 1) / kFfTile), 256, 0, st>>>(a);
+        ff_tile_fwd_kernel<T><<<dim3((unsigned)((a.rows + kFfTile - 1) / kFfTile), (a.hidden + kFfTile - 1) / kFfTile), kFfFwdWarps * 32, 0, st>>>(a);
     }
     launch_end(K_FF_FWD, st);
     CGB_CUDA(cudaGetLastError());
@@ -535,7 +616,7 @@ static int ff_bwd(const FfArgs& a, const FfPlan& q, int grads, char* ws, cudaStr
     if (nx + nw == 0) return CGB200_OK;
     CGB_REQUIRE(nx + nw <= 0x7fffffff, "gated feed-forward: too many tiles for one launch");
     launch_begin(K_FF_BWD, st);
-    ff_tile_bwd_kernel<T><<<(unsigned)(nx + nw), 256, 0, st>>>(a, (int)nx, tiles_d);
+    ff_tile_bwd_kernel<T><<<(unsigned)(nx + nw), kFfBwdWarps * 32, 0, st>>>(a, (int)nx, tiles_d);
     launch_end(K_FF_BWD, st);
     CGB_CUDA(cudaGetLastError());
     return CGB200_OK;
