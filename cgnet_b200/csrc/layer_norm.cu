@@ -6,6 +6,8 @@
 //
 // Everything is held in float32 between the loads and the one rounding of each result.  The variance is taken over centred
 // values that stay in registers (not as a difference of moments), so a large common offset of a row costs no digits.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "row_ops.cuh"
@@ -13,9 +15,13 @@
 
 namespace cgb200 {
 
+namespace cg = cooperative_groups;
+
 constexpr int kLnMaxChunks = 4;        // chunks of a row a thread of the forward kernel holds in registers
 constexpr int kLnBwdValues = 16;       // values of a row a thread of the backward kernel holds
 constexpr int kLnBwdMaxThreads = 512;
+constexpr int kLnCluster = 8;          // blocks of 16 warps that add up the parameters' gradients in one launch
+constexpr int64_t kLnClusterRows = 8 * 16 * kLnCluster;
 
 struct LnArgs {
     const void* x;
@@ -179,7 +185,8 @@ struct LnBwdArgs {
     const void* w;
     const float2* stats;
     void* dx;               // may be null: only the parameters' gradients are wanted
-    float* part;            // [gridDim.x][2][dim]; null: the parameters' gradients are not wanted
+    float* part;            // [gridDim.x][2][dim]; null: the parameters' gradients are not wanted, or are joined by the cluster
+    void *dw, *db;          // where the blocks are one cluster, which adds up its sums itself (each may be null)
     int64_t rows, dim;
 };
 
@@ -217,7 +224,7 @@ __device__ __forceinline__ void store_values(T* p, int64_t e0, int64_t n, const 
 // boundaries), NC accesses.  Each block leaves one partial sum per column; ln_param_reduce_kernel adds them, so the result does
 // not depend on timing.
 template <typename T, typename P, int VE, int NC>
-__global__ void __launch_bounds__(256) ln_bwd_kernel(LnBwdArgs a) {
+__global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_kernel(LnBwdArgs a) {
     extern __shared__ float sm[];
     const int t = (int)(threadIdx.x & 31), warp = threadIdx.x >> 5, nwarps = (int)(blockDim.x >> 5);
     const float inv_n = 1.f / (float)a.dim;
@@ -270,23 +277,34 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(LnBwdArgs a) {
             }
         }
     }
-    if (a.part == nullptr) return;
-    float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+    if (a.part == nullptr && a.dw == nullptr && a.db == nullptr) return;
     // the block's warps, in order
-    const int n2 = 2 * (int)a.dim;
+    const int n = (int)a.dim, n2 = 2 * n;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
             const int e = (t + c * 32) * VE + i;
-            if (e < a.dim) sm[warp * n2 + e] = dw[c][i], sm[warp * n2 + (int)a.dim + e] = db[c][i];
+            if (e < n) sm[warp * n2 + e] = dw[c][i], sm[warp * n2 + n + e] = db[c][i];
         }
     __syncthreads();
     for (int e = threadIdx.x; e < n2; e += blockDim.x) {
         float s = 0.f;
         for (int k = 0; k < nwarps; ++k) s += sm[k * n2 + e];
-        out[e] = s;
+        if (a.part != nullptr) a.part[(int64_t)blockIdx.x * n2 + e] = s;
+        else sm[e] = s;                  // only this thread has read column e of warp 0
     }
+    if (a.part != nullptr) return;
+    // and the cluster's blocks, in order: each block adds up its share of the columns
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int e = (int)(blockIdx.x * blockDim.x + threadIdx.x); e < n2; e += (int)(gridDim.x * blockDim.x)) {
+        float s = 0.f;
+        for (int k = 0; k < (int)gridDim.x; ++k) s += cluster.map_shared_rank(sm, k)[e];
+        P* out = (P*)(e < n ? a.dw : a.db);
+        if (out != nullptr) out[e < n ? e : e - n] = from_f32<P>(s);
+    }
+    cluster.sync();                      // no block leaves while its sums are read
 }
 
 // The same for rows of a block, which come through shared memory: a ring of `stages` rows of x and dy, filled by the bulk copies of
@@ -316,7 +334,6 @@ __device__ __forceinline__ RingRow ring_row(const T* r, int64_t row, int64_t row
 }
 template <typename T, bool EDGE>
 __device__ __forceinline__ uint4 ring_at(const uint4* slot, const RingRow& q, const T* r, int k, int n) {
-    constexpr int N = Chunk<T>::N;
     if (!EDGE) return slot[k];
     const uint4 lo = k >= q.g0 && k < q.g1 ? slot[k] : load_group(r, q.ph, k, n);
     if (q.ph == 0) return lo;
@@ -584,7 +601,7 @@ static int ln_fwd(const LnArgs& a, void* y, float2* stats, cudaStream_t st) {
 
 // Blocks of the backward kernel (= partial sums) for rows a thread can hold, and threads per block.
 struct LnBwdShape {
-    bool fits, warp;
+    bool fits, warp, cluster;
     int nc, threads, grid;
 };
 // N: values of a 16-byte group; vec: rows start and end on those
@@ -598,9 +615,12 @@ static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int N, bool vec) {
         const int64_t cols = (dim + 255) / 256;
         s.grid = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(rows, 256), (kNumSM * 8 + cols - 1) / cols));
     } else if (s.warp) {
-        s.threads = 256;
         s.nc = pow2_at_least(((vec ? chunks : dim) + 31) / 32);
-        s.grid = (int)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, kNumSM * 4));
+        // up to eight rows a warp of one cluster: a second launch for the sums would take longer than they do
+        s.cluster = rows > 0 && rows <= kLnClusterRows;
+        s.threads = s.cluster ? 512 : 256;
+        s.grid = s.cluster ? (int)std::min<int64_t>(kLnCluster, pow2_at_least((rows + 15) / 16))
+                           : (int)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, kNumSM * 4));
     } else {
         s.threads = (int)((chunks + 32 * (kLnBwdValues / N) - 1) / (32 * (kLnBwdValues / N))) * 32;
         const int per_sm = std::max(1, kLnBwdThreadsPerSM / s.threads);
@@ -610,13 +630,33 @@ static LnBwdShape ln_bwd_shape(int64_t rows, int64_t dim, int N, bool vec) {
     }
     return s;
 }
-template <typename T, typename P, int VE>
-static void ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
+template <typename T, typename P, int VE, int NC>
+static int ln_bwd_launch_nc(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
     const size_t smem = (size_t)(s.threads / 32) * 2 * a.dim * sizeof(float);
-#define CGB_LN_BWD(NC_)                                                                        \
-    if constexpr (NC_ * VE <= kLnBwdValues) {                                                  \
-        ln_bwd_kernel<T, P, VE, NC_><<<s.grid, s.threads, smem, st>>>(a);                      \
+    auto kern = ln_bwd_kernel<T, P, VE, NC>;
+    if (smem > 48 * 1024) CGB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (!s.cluster) {
+        kern<<<s.grid, s.threads, smem, st>>>(a);
+        return CGB200_OK;
     }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)s.grid);
+    cfg.blockDim = dim3((unsigned)s.threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)s.grid;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CGB_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+    return CGB200_OK;
+}
+template <typename T, typename P, int VE>
+static int ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st) {
+#define CGB_LN_BWD(NC_) \
+    if constexpr (NC_ * VE <= kLnBwdValues) return ln_bwd_launch_nc<T, P, VE, NC_>(s, a, st);
     switch (s.nc) {
         case 1: CGB_LN_BWD(1) break;
         case 2: CGB_LN_BWD(2) break;
@@ -625,6 +665,8 @@ static void ln_bwd_launch(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t 
         default: CGB_LN_BWD(16) break;
     }
 #undef CGB_LN_BWD
+    set_error("internal: layer norm asked for an unsupported row length");
+    return CGB200_ERR_UNSUPPORTED;
 }
 
 template <typename T, typename P, bool EDGE>
@@ -641,7 +683,7 @@ static int ln_bwd_ring(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st)
 }
 
 template <typename T, typename P>
-static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
+static int ln_bwd(LnBwdArgs a, void* dw, void* db, cudaStream_t st) {
     constexpr int N = Chunk<T>::N;
     auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     const bool vec = a.dim % N == 0 && a.x_stride % N == 0 && a.dy_stride % N == 0 && at16(a.x) && at16(a.dy) && at16(a.dx);
@@ -649,9 +691,10 @@ static int ln_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
     if (a.rows > 0) {
         if (s.fits) {
             int rc = CGB200_OK;
+            if (s.cluster) a.dw = dw, a.db = db, a.part = nullptr;
             launch_begin(K_LN_BWD, st);
-            if (vec && s.warp) ln_bwd_launch<T, P, N>(s, a, st);
-            else if (s.warp) ln_bwd_launch<T, P, 1>(s, a, st);
+            if (vec && s.warp) rc = ln_bwd_launch<T, P, N>(s, a, st);
+            else if (s.warp) rc = ln_bwd_launch<T, P, 1>(s, a, st);
             else if (vec) rc = ln_bwd_ring<T, P, false>(s, a, st);
             else rc = ln_bwd_ring<T, P, true>(s, a, st);
             launch_end(K_LN_BWD, st);
@@ -717,7 +760,8 @@ int cgb200_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, c
 int64_t cgb200_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int dtype) {
     if (ln_check(rows, dim, dtype, dtype) != CGB200_OK) return -1;
     const int n = dtype == CGB200_F32 ? 4 : 8;
-    const int parts = ln_bwd_shape(rows, dim, n, false).grid;
+    const LnBwdShape s = ln_bwd_shape(rows, dim, n, false);
+    const int parts = s.cluster ? 0 : s.grid;
     return (int64_t)parts * 2 * dim * (int64_t)sizeof(float);
 }
 
@@ -731,13 +775,13 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
     CGB_REQUIRE(x_stride >= 0 && x_stride <= (1ll << 40) && dy_stride >= 0 && dy_stride <= (1ll << 40), "layer norm: row stride out of range");
     if (params) {
         const int64_t need = cgb200_layer_norm_bwd_workspace_bytes(rows, dim, dtype);
-        if (workspace == nullptr || workspace_bytes < need) {
+        if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
             set_error("workspace too small: need " + std::to_string(need) + " bytes");
             return CGB200_ERR_WORKSPACE;
         }
         CGB_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");
     }
-    const LnBwdArgs a{x, x_stride, dy, dy_stride, weight, (const float2*)stats, dx, params ? (float*)workspace : nullptr, rows, dim};
+    const LnBwdArgs a{x, x_stride, dy, dy_stride, weight, (const float2*)stats, dx, params ? (float*)workspace : nullptr, nullptr, nullptr, rows, dim};
     cudaStream_t st = (cudaStream_t)stream;
 #define CGB_CALL(T_, P_) ln_bwd<T_, P_>(a, dweight, dbias, st)
     CGB_LN_TYPES(CGB_CALL);

@@ -13,11 +13,11 @@ bits from run to run.  (As with any torch operator, capture a backward pass only
 alive: torch ties a leaf's gradient accumulation to the stream it was first used on.)
 """
 import collections
+import functools
 import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .cg_layers import _current_stream
@@ -38,17 +38,18 @@ def _check_values(t, name, device=None, dtype=None):
     """A float32, bfloat16 or float16 CUDA tensor, on ``device`` and of ``dtype`` where those are given."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.dtype not in _DTYPES:
-        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if dtype is not None and t.dtype != dtype:
-        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+    own = t.dtype
+    if own not in _DTYPES:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {own}")
+    if dtype is not None and own is not dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {own}")
     if device is not None and t.device != device:
         raise RuntimeError(f"{name} lives on {t.device}, expected {device}")
     return t
 
 
 def _check_shape(t, name, shape):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t
 
@@ -83,8 +84,8 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(name, device, *args):
-    index = device.index
+def _call(name, index, *args):
+    """Run an entry point on the current stream of CUDA device ``index``."""
     fn = getattr(_lib.load(), name)
     if torch.cuda.current_device() == index:
         rc = fn(*args, _current_stream(index))
@@ -95,6 +96,13 @@ def _call(name, device, *args):
         _lib.check(rc, name)
 
 
+def _once():
+    """First line of every backward: the gradients are not differentiable themselves, and say so (autograd runs a backward with
+    gradients enabled only where its result is to be differentiated again)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the operators of cgnet_b200.head are differentiable once only")
+
+
 def _workspace(nbytes, device):
     """Scratch of one call, from torch's allocator (which keeps it apart from other streams' and graphs' calls)."""
     if nbytes < 0:
@@ -102,8 +110,9 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _differentiable(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _empty(rows, columns, like):
+    """(rows, columns) of ``like``'s type and device, contiguous."""
+    return torch.empty((rows, columns), dtype=like.dtype, device=like.device)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -111,12 +120,19 @@ def _differentiable(*tensors):
 # ---------------------------------------------------------------------------------------------------------------------
 def _layer_norm_fwd(x2, weight, bias, eps, keep):
     rows, dim = x2.shape
-    y = torch.empty(rows, dim, dtype=x2.dtype, device=x2.device)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=x2.device) if keep else None
+    index = x2.get_device()
+    y = _empty(rows, dim, x2)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x2.device) if keep else None
     param = weight if weight is not None else bias
-    _call("cgb200_layer_norm_fwd", x2.device, x2.data_ptr(), x2.stride(0), _ptr(weight), _ptr(bias), eps, y.data_ptr(), _ptr(stats), rows,
-          dim, _DTYPES[x2.dtype], _DTYPES[x2.dtype if param is None else param.dtype])
+    dtype = _DTYPES[x2.dtype]
+    _call("cgb200_layer_norm_fwd", index, x2.data_ptr(), x2.stride(0), _ptr(weight), _ptr(bias), eps, y.data_ptr(), _ptr(stats), rows, dim, dtype,
+          dtype if param is None else _DTYPES[param.dtype])
     return y, stats
+
+
+@functools.lru_cache(maxsize=1024)
+def _layer_norm_bwd_bytes(rows, dim, dtype):
+    return _lib.load().cgb200_layer_norm_bwd_workspace_bytes(rows, dim, dtype)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -128,27 +144,24 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _once()
         x2, weight, stats = ctx.saved_tensors
         rows, dim = x2.shape
         dy = _rows(dy)
-        need = ctx.needs_input_grad
-        dev = x2.device
-        dx = torch.empty(rows, dim, dtype=x2.dtype, device=dev) if need[0] else None
-        dw = torch.empty(dim, dtype=ctx.param_dtype, device=dev) if need[1] else None
-        db = torch.empty(dim, dtype=ctx.param_dtype, device=dev) if need[2] else None
-        dtype = _DTYPES[x2.dtype]
-        n = _lib.load().cgb200_layer_norm_bwd_workspace_bytes(rows, dim, dtype) if need[1] or need[2] else 0
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dev, dtype, param_dtype = x2.device, _DTYPES[x2.dtype], ctx.param_dtype
+        dx = _empty(rows, dim, x2) if need_x else None
+        dw = torch.empty(dim, dtype=param_dtype, device=dev) if need_w else None
+        db = torch.empty(dim, dtype=param_dtype, device=dev) if need_b else None
+        n = _layer_norm_bwd_bytes(rows, dim, dtype) if need_w or need_b else 0
         ws = _workspace(n, dev)
-        _call("cgb200_layer_norm_bwd", dev, x2.data_ptr(), x2.stride(0), dy.data_ptr(), dy.stride(0), _ptr(weight), stats.data_ptr(), _ptr(dx),
-              _ptr(dw), _ptr(db), rows, dim, dtype, _DTYPES[ctx.param_dtype], _ptr(ws), n)
+        _call("cgb200_layer_norm_bwd", x2.get_device(), x2.data_ptr(), x2.stride(0), dy.data_ptr(), dy.stride(0), _ptr(weight), stats.data_ptr(),
+              _ptr(dx), _ptr(dw), _ptr(db), rows, dim, dtype, _DTYPES[param_dtype], _ptr(ws), n)
         return dx, dw, db, None
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis.  ``weight`` and ``bias`` (``(dim,)``, of x's type or
-    float32, each optional) get gradients of their own type, summed over the rows in a fixed order."""
+def _check_layer_norm(x, weight, bias):
     _check_values(x, "x")
     _check_rows(x, "x")
     dim = x.shape[-1]
@@ -159,16 +172,22 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
                 raise RuntimeError(f"{name} must be {x.dtype} or float32, got {p.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    if not (eps >= 0.0 and math.isfinite(eps)):
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis.  ``weight`` and ``bias`` (``(dim,)``, of x's type or
+    float32, each optional) get gradients of their own type, summed over the rows in a fixed order."""
+    if not 0.0 <= eps < math.inf:
         raise RuntimeError(f"eps must be finite and not negative, got {eps}")
+    _check_layer_norm(x, weight, bias)
     _check_cuda(x, "x")
     x2 = _rows(x)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if _differentiable(x, weight, bias):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         y = _LayerNorm.apply(x2, weight, bias, float(eps))
     else:
-        y, _ = _layer_norm_fwd(x2, weight, bias, float(eps), False)
+        y = _layer_norm_fwd(x2, weight, bias, float(eps), False)[0]
     return y if x.dim() == 2 else y.view(x.shape)
 
 
@@ -184,7 +203,7 @@ def _gated_ff_fwd(x2, wg, wu, act, keep):
     operands = (x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
     n = _lib.load().cgb200_gated_ff_workspace_bytes(*operands, rows, dim, hidden, dtype, 0)
     ws = _workspace(n, dev)
-    _call("cgb200_gated_ff_fwd", dev, *operands, act, h.data_ptr(),
+    _call("cgb200_gated_ff_fwd", x2.get_device(), *operands, act, h.data_ptr(),
           _ptr(gate_up), rows, dim, hidden, dtype, _ptr(ws), n)
     return h, gate_up
 
@@ -198,8 +217,8 @@ class _GatedFeedForward(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh):
+        _once()
         x2, wg, wu, gate_up = ctx.saved_tensors
         rows, dim = x2.shape
         hidden = wg.shape[0]
@@ -212,7 +231,7 @@ class _GatedFeedForward(torch.autograd.Function):
         operands = (x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
         n = _lib.load().cgb200_gated_ff_workspace_bytes(*operands, rows, dim, hidden, dtype, bool(need[0]) + 2 * bool(need[1]) + 4 * bool(need[2]))
         ws = _workspace(n, dev)
-        _call("cgb200_gated_ff_bwd", dev, *operands, ctx.act, gate_up.data_ptr(), dh.data_ptr(), dh.stride(0), _ptr(dx), _ptr(dwg), _ptr(dwu), rows, dim, hidden, dtype, _ptr(ws), n)
+        _call("cgb200_gated_ff_bwd", x2.get_device(), *operands, ctx.act, gate_up.data_ptr(), dh.data_ptr(), dh.stride(0), _ptr(dx), _ptr(dwg), _ptr(dwu), rows, dim, hidden, dtype, _ptr(ws), n)
         return dx, dwg, dwu, None
 
 
@@ -233,7 +252,7 @@ def gated_feed_forward(x, w_gate, w_up, activation="silu"):
     _check_shape(w_up, "w_up", w_gate.shape)
     _check_cuda(x, "x")
     x2, wg, wu, act = _rows(x), _rows(w_gate), _rows(w_up), _ACTIVATIONS[activation]
-    if _differentiable(x, w_gate, w_up):
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         h = _GatedFeedForward.apply(x2, wg, wu, act)
     else:
         h, _ = _gated_ff_fwd(x2, wg, wu, act, False)
@@ -251,7 +270,7 @@ def _log_probs_fwd(z2, targets, top, keep):
     top_lp = torch.empty(rows, top, dtype=torch.float32, device=dev)
     top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
     stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if keep else None
-    _call("cgb200_log_probs_fwd", dev, z2.data_ptr(), z2.stride(0), _ptr(targets), top, log_prob.data_ptr(), entropy.data_ptr(),
+    _call("cgb200_log_probs_fwd", z2.get_device(), z2.data_ptr(), z2.stride(0), _ptr(targets), top, log_prob.data_ptr(), entropy.data_ptr(),
           top_lp.data_ptr(), top_ids.data_ptr(), _ptr(stats), rows, classes, _DTYPES[z2.dtype])
     return log_prob, entropy, top_lp, top_ids, stats
 
@@ -266,8 +285,8 @@ class _LogProbs(torch.autograd.Function):
         return log_prob, entropy, top_lp, top_ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent, _top_lp, _top_ids):
+        _once()
         z2, targets, entropy, stats = ctx.saved_tensors
         if targets is None:
             g_lp = None
@@ -277,7 +296,7 @@ class _LogProbs(torch.autograd.Function):
         g_lp = None if g_lp is None else g_lp.contiguous()
         g_ent = None if g_ent is None else g_ent.contiguous()
         dz = torch.empty(rows, classes, dtype=z2.dtype, device=z2.device)
-        _call("cgb200_log_probs_bwd", z2.device, z2.data_ptr(), z2.stride(0), _ptr(targets), entropy.data_ptr(), stats.data_ptr(), _ptr(g_lp),
+        _call("cgb200_log_probs_bwd", z2.get_device(), z2.data_ptr(), z2.stride(0), _ptr(targets), entropy.data_ptr(), stats.data_ptr(), _ptr(g_lp),
               _ptr(g_ent), dz.data_ptr(), rows, classes, _DTYPES[z2.dtype])
         return dz, None, None
 
@@ -298,7 +317,7 @@ def log_probs(logits, targets=None, top=0):
         targets = _check_classes(targets, "targets", lead, logits.device).reshape(-1)
     _check_cuda(logits, "logits")
     z2 = _rows(logits)
-    if _differentiable(logits):
+    if torch.is_grad_enabled() and logits.requires_grad:
         lp, ent, top_lp, top_ids = _LogProbs.apply(z2, targets, top)
     else:
         lp, ent, top_lp, top_ids, _ = _log_probs_fwd(z2, targets, top, False)
@@ -315,7 +334,7 @@ def _distill_fwd(z2, ids, scores, temperature, keep):
     dev = z2.device
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if keep else None
-    _call("cgb200_distill_fwd", dev, z2.data_ptr(), z2.stride(0), ids.data_ptr(), scores.data_ptr(), ids.shape[1], _DTYPES[scores.dtype],
+    _call("cgb200_distill_fwd", z2.get_device(), z2.data_ptr(), z2.stride(0), ids.data_ptr(), scores.data_ptr(), ids.shape[1], _DTYPES[scores.dtype],
           temperature, loss.data_ptr(), _ptr(stats), rows, classes, _DTYPES[z2.dtype])
     return loss, stats
 
@@ -329,13 +348,13 @@ class _Distill(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once()
         z2, ids, scores, stats = ctx.saved_tensors
         rows, classes = z2.shape
         g = g.contiguous()
         dz = torch.empty(rows, classes, dtype=z2.dtype, device=z2.device)
-        _call("cgb200_distill_bwd", z2.device, z2.data_ptr(), z2.stride(0), ids.data_ptr(), scores.data_ptr(), ids.shape[1],
+        _call("cgb200_distill_bwd", z2.get_device(), z2.data_ptr(), z2.stride(0), ids.data_ptr(), scores.data_ptr(), ids.shape[1],
               _DTYPES[scores.dtype], ctx.temperature, stats.data_ptr(), g.data_ptr(), dz.data_ptr(), rows, classes, _DTYPES[z2.dtype])
         return dz, None, None, None
 
@@ -362,7 +381,7 @@ def distillation_loss(logits, teacher_ids, teacher_scores, temperature=1.0):
         raise RuntimeError(f"temperature must be between 0.001 and 1000, got {temperature}")
     _check_cuda(logits, "logits")
     z2, scores = _rows(logits), teacher_scores.detach().reshape(-1, k).contiguous()
-    if _differentiable(logits):
+    if torch.is_grad_enabled() and logits.requires_grad:
         loss = _Distill.apply(z2, ids, scores, float(temperature))
     else:
         loss, _ = _distill_fwd(z2, ids, scores, float(temperature), False)

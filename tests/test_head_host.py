@@ -66,7 +66,7 @@ def test_library_refusals_need_no_gpu():
     assert lib.cgb200_layer_norm_fwd(None, 4, None, None, 1e-5, p, None, 2, 4, 0, 0, None) == bad
     assert lib.cgb200_layer_norm_fwd(None, 4, None, None, 1e-5, None, None, 0, 4, 0, 0, None) == 0
     assert lib.cgb200_layer_norm_bwd_workspace_bytes(-1, 4, 0) == -1
-    assert lib.cgb200_layer_norm_bwd(p, 4, p, 4, None, p, p, p, p, 100, 64, 0, 0, None, 0, None) == 4
+    assert lib.cgb200_layer_norm_bwd(p, 64, p, 64, None, p, p, p, p, 100000, 64, 0, 0, None, 0, None) == 4
     assert b"need" in lib.cgb200_last_error()
     assert lib.cgb200_gated_ff_fwd(p, 4, p, 4, p, 4, 3, p, None, 2, 4, 4, 0, None, 0, None) == bad
     assert lib.cgb200_gated_ff_fwd(p, 4, p, 4, None, 4, 0, p, None, 2, 4, 4, 0, None, 0, None) == bad
