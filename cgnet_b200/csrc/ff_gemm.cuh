@@ -89,18 +89,37 @@ __device__ __forceinline__ uint64_t box_desc(uint32_t saddr, int mn) {
 }
 
 // act(g) and its derivative
-template <bool GRAD>
-__device__ __forceinline__ float2 activate(int act, float g) {
-    if (act == CGB200_ACT_RELU) return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);
-    if (act == CGB200_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-g));
-        // where s is 0, g may be -inf
-        return s == 0.f ? make_float2(0.f, 0.f) : make_float2(g * s, GRAD ? s * (1.f + g * (1.f - s)) : 0.f);
+template <int ACT, bool GRAD>
+__device__ __forceinline__ float2 activate_as(float g) {
+    if (ACT == CGB200_ACT_RELU) return g > 0.f ? make_float2(g, 1.f) : make_float2(g != g ? g : 0.f, 0.f);
+    if (ACT == CGB200_ACT_SILU) {
+        // below -88 the exponential leaves float32's range, and g may be -inf; a NaN fails the comparison
+        const float s = g < -88.f ? 0.f : __fdividef(1.f, 1.f + __expf(-g));
+        return g < -88.f ? make_float2(0.f, 0.f) : make_float2(g * s, GRAD ? s * (1.f + g * (1.f - s)) : 0.f);
     }
     const float c = 0.5f * erfcf(-0.70710678118654752f * g);
     return make_float2(c == 0.f ? 0.f : g * c, GRAD ? c + (fabsf(g) > 20.f ? 0.f : g * __expf(-0.5f * g * g) * 0.39894228040143268f) : 0.f);
 }
-
+template <bool GRAD>
+__device__ __forceinline__ float2 activate(int act, float g) {
+    if (act == CGB200_ACT_RELU) return activate_as<CGB200_ACT_RELU, GRAD>(g);
+    if (act == CGB200_ACT_SILU) return activate_as<CGB200_ACT_SILU, GRAD>(g);
+    return activate_as<CGB200_ACT_GELU, GRAD>(g);
+}
+// g = act(g) * u for n values; the choice is made once, outside the unrolled loop
+template <int N>
+__device__ __forceinline__ void gate(int act, float (&g)[N], const float (&u)[N]) {
+    if (act == CGB200_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = activate_as<CGB200_ACT_RELU, false>(g[i]).x * u[i];
+    } else if (act == CGB200_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = activate_as<CGB200_ACT_SILU, false>(g[i]).x * u[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = activate_as<CGB200_ACT_GELU, false>(g[i]).x * u[i];
+    }
+}
 // The same, one copy of it, for kernels that want short code
 __device__ __noinline__ float2 activate_shared(int act, float g) { return activate<true>(act, g); }
 
@@ -301,8 +320,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                         write_block(g, st, (float*)p.out[1], row0, p.n_i, p.n_j, col0, p.n_j);
                         write_block(up, st, (float*)p.out[1] + p.n_i * p.n_j, row0, p.n_i, p.n_j, col0, p.n_j);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) g[i] = activate<false>(a.act, g[i]).x * up[i];
+                    gate(a.act, g, up);
                     write_block(g, st, (T*)p.out[0], row0, p.n_i, p.n_j, col0, p.n_j);
                 } else if (p.splits > 1) {
                     float* part = p.part + ((int64_t)t.split * p.sets + t.set) * p.n_i * p.n_j;
@@ -316,7 +334,8 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                 ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, a.polls);
                 tc_fence_after();
                 const uint32_t d = lanes + acc * kAccCols + side * (JW / 2);
-#pragma unroll
+                // not unrolled: the epilogue's code has to stay in the instruction cache beside the two other roles'
+#pragma unroll 1
                 for (int c = 0; c < kBlocks; ++c) {
                     float g[32], up[32];
                     if (ok) {
