@@ -56,6 +56,11 @@ __device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, int c
                  "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -194,31 +199,39 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_ptr;
+    const uint32_t tmem = tmem_ptr, polls = a.polls;
 
+    // The two issuing roles run on one elected thread: under elect.sync the compiler knows that, and keeps what the copies and
+    // products take in uniform registers (under `lane == 0` a copy took 80 cycles to issue and bounded the kernel).
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, issued = 0;
             uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < a.units && ok; u += gridDim.x) {
                 const FfUnit t = ff_unit(a, u, JW);
-                const FfProblem& p = *t.p;
-                for (int it = t.k0; it < t.k1; ++it) {
-                    if (!mbar_wait(&empty[s], ph, failed, a.polls)) {
+                // in registers: what the loop looked up in the arguments each time cost it more than the copies' own time
+                const int kblk = t.p->kblk, a_mn = t.p->a_mn, b_mn = t.p->b_mn, i0 = (int)t.i0, j0 = t.j0, k1 = t.k1;
+                const bool two = t.p->sources > 1;
+                const CUtensorMap* a0 = &a.map[t.p->a_map[t.p->sets > 1 ? t.set : 0]];
+                const CUtensorMap* a1 = &a.map[t.p->a_map[1]];
+                const CUtensorMap *b0 = &a.map[t.p->b_map[0]], *b1 = &a.map[t.p->b_map[1]];
+                for (int it = t.k0; it < k1; ++it) {
+                    if (!mbar_wait(&empty[s], ph, failed, polls)) {
                         ok = false;
                         break;
                     }
-                    const int src = p.sources > 1 && it >= p.kblk ? 1 : 0, k = (it - src * p.kblk) * kFfBK;
-                    const CUtensorMap* am = &a.map[p.a_map[p.sets > 1 ? t.set : src]];
+                    const bool src = two && it >= kblk;
+                    const int k = (src ? it - kblk : it) * kFfBK;
+                    const CUtensorMap* am = src ? a1 : a0;
                     char* d = base + s * kStage;
                     mbar_arrive_expect_tx(&full[s], kStage);
 #pragma unroll
                     for (int q = 0; q < PLANES; ++q) {
 #pragma unroll
                         for (int b = 0; b < kFfBM / 64; ++b, d += kFfBox) {
-                            const int i = (int)t.i0 + 64 * b;
-                            tma_box(d, am, p.a_mn ? i : k, p.a_mn ? k : i, q, &full[s]);
+                            const int i = i0 + 64 * b;
+                            tma_box(d, am, a_mn ? i : k, a_mn ? k : i, q, &full[s]);
                         }
                     }
 #pragma unroll
@@ -226,9 +239,8 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
 #pragma unroll
                         for (int b = 0; b < BN / 64; ++b, d += kFfBox) {
                             const int second = FWD && b >= BN / 128;      // the up projection's half of the columns
-                            const CUtensorMap* bm = &a.map[p.b_map[FWD ? second : src]];
-                            const int j = t.j0 + 64 * (b - second * (BN / 128));
-                            tma_box(d, bm, p.b_mn ? j : k, p.b_mn ? k : j, q, &full[s]);
+                            const int j = j0 + 64 * (b - second * (BN / 128));
+                            tma_box(d, (FWD ? second : src) ? b1 : b0, b_mn ? j : k, b_mn ? k : j, q, &full[s]);
                         }
                     }
                     ++issued;
@@ -237,37 +249,37 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             }
             if (!ok) {
                 // let the copies in flight land before the block gives up its shared memory: the last kStages issued ones
-                for (int n = max(0, issued - kStages); n < issued; ++n) mbar_drain(&full[n % kStages], (n / kStages) & 1, a.polls);
+                for (int n = max(0, issued - kStages); n < issued; ++n) mbar_drain(&full[n % kStages], (n / kStages) & 1, polls);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, acc = 0;
             uint32_t ph = 0, acc_ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < a.units && ok; u += gridDim.x) {
                 const FfUnit t = ff_unit(a, u, JW);
-                const FfProblem& p = *t.p;
-                const uint32_t idesc = (1u << 4) | a.idesc_type | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
+                const int a_mn = t.p->a_mn, b_mn = t.p->b_mn, k1 = t.k1;
+                const uint32_t idesc = (1u << 4) | a.idesc_type | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
                                        ((uint32_t)(kFfBM >> 4) << 24);
-                const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-                for (int it = t.k0; it < t.k1;) {
-                    if (!mbar_wait(&acc_empty[acc], acc_ph, failed, a.polls)) {
+                const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+                const uint64_t da0 = box_desc(smem_u32(base), a_mn), db0 = box_desc(smem_u32(base) + PLANES * kFfBM * kFfBK * 2, b_mn);
+                for (int it = t.k0; it < k1;) {
+                    if (!mbar_wait(&acc_empty[acc], acc_ph, failed, polls)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t d = tmem + acc * kAccCols;
-                    const int stop = min(t.k1 - it, kFlush) + it;
+                    const int stop = min(k1 - it, kFlush) + it;
                     bool first = true;
                     for (; it < stop; ++it) {
-                        if (!mbar_wait(&full[s], ph, failed, a.polls)) {
+                        if (!mbar_wait(&full[s], ph, failed, polls)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t sa = smem_u32(base + s * kStage), sb = sa + PLANES * kFfBM * kFfBK * 2;
-                        const uint64_t da = box_desc(sa, p.a_mn), db = box_desc(sb, p.b_mn);
+                        const uint64_t da = desc_advance(da0, s * kStage), db = desc_advance(db0, s * kStage);
                         if constexpr (PLANES == 1) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
@@ -296,7 +308,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             }
             if (!ok) {      // the products issued so far end before the block gives up its memories
                 tc_commit(&stopped);
-                mbar_drain(&stopped, 0, a.polls);
+                mbar_drain(&stopped, 0, polls);
             }
         }
     } else if (warp >= 4) {
@@ -331,7 +343,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             };
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
             if constexpr (PLANES == 1) {
-                ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, a.polls);
+                ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, polls);
                 tc_fence_after();
                 const uint32_t d = lanes + acc * kAccCols + side * (JW / 2);
                 // not unrolled: the epilogue's code has to stay in the instruction cache beside the two other roles'
@@ -361,7 +373,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
                 for (int it = t.k0; it < t.k1; it += kFlush) {
-                    ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, a.polls);
+                    ok = ok && mbar_wait_warp(&acc_full[acc], acc_ph, failed, polls);
                     tc_fence_after();
                     if (ok) {
                         const uint32_t d = lanes + acc * kAccCols + side * (JW / 2);
