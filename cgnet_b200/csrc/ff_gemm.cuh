@@ -25,7 +25,7 @@ constexpr int kFfEpiWarps = 8;
 constexpr int kFfBox = 64 * 64 * 2;            // bytes of one copy
 constexpr int kFfStageBytes = 192 * 1024;      // all stages of a block
 constexpr int kFfFlush = 4;                    // stages between flushes of the three-plane form (16 truncating additions)
-constexpr int kFfStaging = 32 * 33;            // floats an epilogue warp turns rows into columns with
+constexpr int kFfStaging = 32 * 32;            // floats of an epilogue warp's staging area
 constexpr size_t kFfSmem = 1024 + kFfStageBytes + kFfEpiWarps * kFfStaging * sizeof(float);
 static_assert(kFfSmem <= kMaxDynSmem, "stages and staging must fit a block's shared memory");
 
@@ -38,11 +38,13 @@ struct FfProblem {
     int unit0;                  // first work unit of this problem
     int64_t n_i;                // rows of a set
     int n_j;
-    void* out[2];               // per set; the forward: h, and g followed by u
+    int h_aligned;              // the forward: rows of h start on 16-byte boundaries
+    void* out[2];               // per set; the forward: h
+    int out_map[2];             // tensor map of the output by bulk copies, -1: written by threads; the forward: [0] g and u, -1: not kept
     float* part;                // [splits][sets * n_i][n_j] where splits > 1
 };
 struct FfGemmArgs {
-    CUtensorMap map[5];
+    CUtensorMap map[8];         // x, Wg, Wu, dg, du, then outputs
     FfProblem p[2];
     int problems, units;
     uint32_t idesc_type;        // operand format bits of the instruction descriptor
@@ -85,6 +87,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+// 16 columns at either address
+__device__ __forceinline__ void tmem_ld16x2(uint32_t at0, uint32_t at1, float (&v)[32]) {
+    uint32_t a[16], b[16];
+    tmem_ld16(at0, a);
+    tmem_ld16(at1, b);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(a[i]), v[16 + i] = __uint_as_float(b[i]);
+}
 // Descriptor of an operand tile made of 64 x 64 boxes in the 128-byte swizzle.  k contiguous: a box is 64 rows of 128 bytes, 8-row
 // groups 1024 bytes apart.  i / j contiguous: a box is 64 k-rows of 64 values; groups of 8 k are 1024 bytes apart (stride offset),
 // the next 64 values one box (leading offset).  [61,64) = 2 is the 128-byte swizzle.
@@ -110,20 +120,6 @@ __device__ __forceinline__ float2 activate(int act, float g) {
     if (act == CGB200_ACT_RELU) return activate_as<CGB200_ACT_RELU, GRAD>(g);
     if (act == CGB200_ACT_SILU) return activate_as<CGB200_ACT_SILU, GRAD>(g);
     return activate_as<CGB200_ACT_GELU, GRAD>(g);
-}
-// g = act(g) * u for n values; the choice is made once, outside the unrolled loop
-template <int N>
-__device__ __forceinline__ void gate(int act, float (&g)[N], const float (&u)[N]) {
-    if (act == CGB200_ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = activate_as<CGB200_ACT_RELU, false>(g[i]).x * u[i];
-    } else if (act == CGB200_ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = activate_as<CGB200_ACT_SILU, false>(g[i]).x * u[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = activate_as<CGB200_ACT_GELU, false>(g[i]).x * u[i];
-    }
 }
 // The same, one copy of it, for kernels that want short code
 __device__ __noinline__ float2 activate_shared(int act, float g) { return activate<true>(act, g); }
@@ -154,23 +150,63 @@ __device__ __forceinline__ FfUnit ff_unit(const FfGemmArgs& a, int u, int jw) {
     return t;
 }
 
-// 32 x 32 values, row = lane, to columns col0.. of rows row0.. of a row-major matrix: through shared memory, so that a warp
-// writes neighbouring columns.
-template <typename O>
-__device__ __forceinline__ void write_block(const float (&v)[32], float* st, O* out, int64_t row0, int64_t n_rows, int64_t ld, int col0, int n_cols) {
+// Outputs leave through a warp's 4 KB of shared memory by bulk copies of 32 rows x 64 bytes (64-byte swizzle: the 16-byte pieces of a
+// row are permuted by its number, so that neither side has bank conflicts): a quarter of the load/store instructions of turning
+// the rows by hand, which competed with the products for shared memory.
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(c0),
+                 "r"(c1), "r"(c2)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until at most N of this thread's stores still read their shared memory
+template <int N>
+__device__ __forceinline__ void tma_store_wait() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+// 64 bytes of this lane's row into a 2 KB block
+__device__ __forceinline__ void put_row(char* block, const uint4 (&u)[4]) {
     const int lane = threadIdx.x & 31;
-    __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 32; ++c) st[lane * 33 + c] = v[c];
-    __syncwarp();
-    if (col0 + lane < n_cols) {
-        const int n = (int)min((int64_t)32, n_rows - row0);
-        O* o = out + row0 * ld + col0 + lane;
-#pragma unroll 8
-        for (int r = 0; r < n; ++r) o[r * ld] = from_f32<O>(st[r * 33 + lane]);
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(block + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = u[j];
+}
+__device__ __forceinline__ void pack_row(const float* v, uint4 (&u)[4], const float*) {      // 16 values
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        u[j] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+}
+template <typename T>
+__device__ __forceinline__ void pack_row(const float* v, uint4 (&u)[4], const T*) {          // 32 values
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = v[8 * j + i];
+        u[j] = pack16(t, (const T*)nullptr);
     }
 }
-
+// 32 x W values, row = lane, to columns col0.. of rows row0.. of a row-major matrix of any alignment: turned in shared memory, so that
+// a warp writes neighbouring columns.
+template <int W, typename O>
+__device__ __forceinline__ void write_block(const float* v, float* st, O* out, int64_t row0, int64_t n_rows, int64_t ld, int col0, int n_cols) {
+    const int lane = threadIdx.x & 31, cc = lane % W;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < W; ++c) st[lane * W + (c ^ (lane % W))] = v[c];
+    __syncwarp();
+    if (col0 + cc < n_cols) {
+        const int n = (int)min((int64_t)32, n_rows - row0);
+        O* o = out + row0 * ld + col0 + cc;
+#pragma unroll 8
+        for (int r = lane / W; r < n; r += 32 / W) o[r * ld] = from_f32<O>(st[r * W + (cc ^ (r % W))]);
+    }
+}
+// h = act(g) u of 16 columns of this lane's row, in place of g
+template <int ACT>
+__device__ __forceinline__ void gate(float (&g)[16], const float (&u)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) g[i] = activate_as<ACT, false>(g[i]).x * u[i];
+}
 
 template <int PLANES, int BN, typename T, bool FWD>
 __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_constant__ FfGemmArgs a) {
@@ -314,7 +350,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
     } else if (warp >= 4) {
         const int ew = warp - 4, quad = ew & 3, side = ew >> 2;      // 32 rows of the tile, half of its columns
         float* st = (float*)(base + kFfStageBytes) + ew * kFfStaging;
-        int acc = 0;
+        int acc = 0, flip = 0;         // flip: the half of the staging area that the next 16-bit block goes through
         uint32_t acc_ph = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
@@ -322,23 +358,79 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             const FfProblem& p = *t.p;
             const int64_t row0 = t.i0 + quad * 32;
             const bool rows_here = row0 < p.n_i;
-            constexpr int kBlocks = JW / 64;                         // 32-column blocks of this warp's half
-            // what the block of output columns `c` of this warp is made of: accumulator columns `at` (and at + BN / 2 for the up half)
-            auto emit = [&](int c, float (&g)[32], float (&up)[32]) {
-                const int col0 = t.j0 + side * (JW / 2) + c * 32;
+            // a block of columns of this warp's half: 32 of a plain product, 16 of g and as many of u
+            constexpr int kCols = FWD ? 16 : 32, kBlocks = JW / 2 / kCols;
+            auto emit = [&](int c, const float* v, const float* w) {
+                const int col0 = t.j0 + side * (JW / 2) + c * kCols;
                 if (!rows_here || col0 >= p.n_j) return;
+                char* bytes = (char*)st;
                 if constexpr (FWD) {
-                    if (p.out[1] != nullptr) {
-                        write_block(g, st, (float*)p.out[1], row0, p.n_i, p.n_j, col0, p.n_j);
-                        write_block(up, st, (float*)p.out[1] + p.n_i * p.n_j, row0, p.n_i, p.n_j, col0, p.n_j);
+                    float g[16], u[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) g[i] = v[i], u[i] = w[i];
+                    const bool keep = p.out_map[0] >= 0;
+                    if (keep) {
+                        if (lane == 0) tma_store_wait<0>();
+                        __syncwarp();
+                        uint4 q[4];
+                        pack_row(g, q, (const float*)nullptr);
+                        put_row(bytes, q);
+                        pack_row(u, q, (const float*)nullptr);
+                        put_row(bytes + 2048, q);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) tma_store(&a.map[p.out_map[0]], bytes, col0, (int)row0, 0);
                     }
-                    gate(a.act, g, up);
-                    write_block(g, st, (T*)p.out[0], row0, p.n_i, p.n_j, col0, p.n_j);
+                    if (a.act == CGB200_ACT_RELU) gate<CGB200_ACT_RELU>(g, u);
+                    else if (a.act == CGB200_ACT_SILU) gate<CGB200_ACT_SILU>(g, u);
+                    else gate<CGB200_ACT_GELU>(g, u);
+                    T* h = (T*)p.out[0] + (row0 + lane) * p.n_j + col0;
+                    if (p.h_aligned && col0 + 16 <= p.n_j) {
+                        if (row0 + lane < p.n_i) {
+#pragma unroll
+                            for (int j = 0; j < 16 / Chunk<T>::N; ++j) {
+                                float x[Chunk<T>::N];
+#pragma unroll
+                                for (int i = 0; i < Chunk<T>::N; ++i) x[i] = g[j * Chunk<T>::N + i];
+                                *(reinterpret_cast<uint4*>(h) + j) = pack16(x, (const T*)nullptr);
+                            }
+                        }
+                    } else {
+                        if (keep && lane == 0) tma_store_wait<0>();
+                        write_block<16>(g, st, (T*)p.out[0], row0, p.n_i, p.n_j, col0, p.n_j);
+                        fence_proxy_async();
+                    }
                 } else if (p.splits > 1) {
                     float* part = p.part + ((int64_t)t.split * p.sets + t.set) * p.n_i * p.n_j;
-                    write_block(g, st, part, row0, p.n_i, p.n_j, col0, p.n_j);
+                    write_block<32>(v, st, part, row0, p.n_i, p.n_j, col0, p.n_j);
+                } else if (p.out_map[t.set] >= 0) {
+                    const CUtensorMap* map = &a.map[p.out_map[t.set]];
+                    uint4 q[4];
+                    if constexpr (sizeof(T) == 2) {
+                        if (lane == 0) tma_store_wait<1>();
+                        __syncwarp();
+                        pack_row(v, q, (const T*)nullptr);
+                        put_row(bytes + flip, q);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) tma_store(map, bytes + flip, col0, (int)row0, 0);
+                        flip ^= 2048;
+                    } else {
+                        if (lane == 0) tma_store_wait<0>();
+                        __syncwarp();
+                        pack_row(v, q, (const float*)nullptr);
+                        put_row(bytes, q);
+                        pack_row(v + 16, q, (const float*)nullptr);
+                        put_row(bytes + 2048, q);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store(map, bytes, col0, (int)row0, 0);
+                            if (col0 + 16 < p.n_j) tma_store(map, bytes + 2048, col0 + 16, (int)row0, 0);
+                        }
+                    }
                 } else if (p.out[t.set] != nullptr) {
-                    write_block(g, st, (T*)p.out[t.set], row0, p.n_i, p.n_j, col0, p.n_j);
+                    write_block<32>(v, st, (T*)p.out[t.set], row0, p.n_i, p.n_j, col0, p.n_j);
                 }
             };
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -349,27 +441,27 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                 // not unrolled: the epilogue's code has to stay in the instruction cache beside the two other roles'
 #pragma unroll 1
                 for (int c = 0; c < kBlocks; ++c) {
-                    float g[32], up[32];
+                    float v[32];           // a forward's: g, then u
                     if (ok) {
-                        tmem_ld32(d + c * 32, g);
-                        if (FWD) tmem_ld32(d + BN / 2 + c * 32, up);
+                        if (FWD) tmem_ld16x2(d + c * 16, d + BN / 2 + c * 16, v);
+                        else tmem_ld32(d + c * 32, v);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) g[i] = up[i] = __uint_as_float(kNaNBits);
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(kNaNBits);
                     }
                     if (c == kBlocks - 1 && ok) {      // all of this accumulator is in registers or written
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&acc_empty[acc]);
                     }
-                    emit(c, g, up);
+                    emit(c, v, v + 16);
                 }
                 if (++acc == 2) acc = 0, acc_ph ^= 1;
             } else {
-                constexpr int kSums = FWD ? 2 * kBlocks : kBlocks;
-                float sum[kSums][32];
+                constexpr int kSums = JW / (FWD ? 32 : 64);       // 32 columns each; a forward's: g's, then u's
+                float sum[FWD ? 2 * kSums : kSums][32];
 #pragma unroll
-                for (int c = 0; c < kSums; ++c)
+                for (int c = 0; c < (FWD ? 2 * kSums : kSums); ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
                 for (int it = t.k0; it < t.k1; it += kFlush) {
@@ -378,8 +470,8 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                     if (ok) {
                         const uint32_t d = lanes + acc * kAccCols + side * (JW / 2);
 #pragma unroll
-                        for (int c = 0; c < kSums; ++c) {
-                            const uint32_t at = d + (FWD && c >= kBlocks ? BN / 2 + (c - kBlocks) * 32 : c * 32);
+                        for (int c = 0; c < (FWD ? 2 * kSums : kSums); ++c) {
+                            const uint32_t at = d + (FWD && c >= kSums ? BN / 2 + (c - kSums) * 32 : c * 32);
                             float lead[32], rest[32];
                             tmem_ld32(at, lead);
                             tmem_ld32(at + BN, rest);
@@ -394,14 +486,18 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                 }
                 if (!ok) {
 #pragma unroll
-                    for (int c = 0; c < kSums; ++c)
+                    for (int c = 0; c < (FWD ? 2 * kSums : kSums); ++c)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) sum[c][i] = __uint_as_float(kNaNBits);
                 }
 #pragma unroll
-                for (int c = 0; c < kBlocks; ++c) emit(c, sum[c], sum[FWD ? c + kBlocks : c]);
+                for (int c = 0; c < kBlocks; ++c) {
+                    if (FWD) emit(c, &sum[c / 2][c % 2 * 16], &sum[kSums + c / 2][c % 2 * 16]);
+                    else emit(c, sum[c], sum[c]);
+                }
             }
         }
+        if (lane == 0) tma_store_wait<0>();      // the stores have read their memory before the block gives it up
     }
     tc_fence_before();
     __syncthreads();

@@ -21,7 +21,8 @@ struct FfArgs {
     int64_t rows;
     int dim, hidden, act;
     void* h;                                   // forward
-    float* gu;                                 // [2][rows][hidden]: g, u; null where no backward follows
+    float* gu;                                 // [2][rows][gu_pitch]: g, u; null where no backward follows
+    int64_t gu_pitch;                          // hidden rounded up to whole 16 bytes
     const void* dh;                            // backward
     int64_t dh_stride;
     void *dx, *dwg, *dwu;                      // each may be null
@@ -81,8 +82,8 @@ __global__ void __launch_bounds__(128) ff_few_rows_kernel(FfArgs a) {
         if (lane == 0) {
             ((T*)a.h)[m * (int64_t)a.hidden + j] = from_f32<T>(activate<false>(a.act, g[m]).x * u[m]);
             if (a.gu != nullptr) {
-                a.gu[m * (int64_t)a.hidden + j] = g[m];
-                a.gu[(a.rows + m) * (int64_t)a.hidden + j] = u[m];
+                a.gu[m * a.gu_pitch + j] = g[m];
+                a.gu[(a.rows + m) * a.gu_pitch + j] = u[m];
             }
         }
     }
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kFfFwdWarps * 32) ff_tile_fwd_kernel(FfArgs a)
         if (m >= a.rows) break;
         const float us = ff_sum(sums, warp + 8 * i, lane);
         ((T*)a.h)[at] = from_f32<T>(activate_shared(a.act, gs[i]).x * us);
-        if (a.gu != nullptr) a.gu[at] = gs[i], a.gu[a.rows * a.hidden + at] = us;
+        if (a.gu != nullptr) a.gu[m * a.gu_pitch + c] = gs[i], a.gu[(a.rows + m) * a.gu_pitch + c] = us;
     }
 }
 
@@ -206,16 +207,16 @@ __global__ void __launch_bounds__(kFfBwdWarps * 32) ff_tile_bwd_kernel(FfArgs a,
         up = unit >= a.hidden;
         const int64_t j = up ? unit - a.hidden : unit;
         const int n = (int)min((int64_t)kFfTile, dx ? (unit < k_hi ? n_i - row : 0) : (unit < n_i ? k_hi - row : 0));
-        const float* g = a.gu + row * a.hidden + j;
-        const float* u = g + a.rows * a.hidden;
+        const float* g = a.gu + row * a.gu_pitch + j;
+        const float* u = g + a.rows * a.gu_pitch;
         const T* h = (const T*)a.dh + row * a.dh_stride + j;
         const int nb = d0 + lane < a.dim ? (int)min((int64_t)kFfSlab, k_hi - k0) : 0;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const int q = step * r;
             const bool in = q < n;
-            gv[r] = in ? g[(int64_t)q * a.hidden] : 0.f;
-            uv[r] = in && !up ? u[(int64_t)q * a.hidden] : 1.f;
+            gv[r] = in ? g[q * a.gu_pitch] : 0.f;
+            uv[r] = in && !up ? u[q * a.gu_pitch] : 1.f;
             dv[r] = in ? to_f32(h[q * a.dh_stride]) : 0.f;
             const int64_t k = k0 + r;
             const T* b = !dx ? (const T*)a.x + k * a.x_stride : k < a.hidden ? (const T*)a.wg + k * a.wg_stride : (const T*)a.wu + (k - a.hidden) * a.wu_stride;
@@ -324,13 +325,13 @@ template <typename T>
 __global__ void __launch_bounds__(256) ff_dgu_kernel(FfArgs a, void* dg, void* du, int64_t pitch) {
     const int64_t chunks = pitch / 8, n = a.rows * chunks;
     const float* g = a.gu;
-    const float* u = a.gu + a.rows * a.hidden;
+    const float* u = a.gu + a.rows * a.gu_pitch;
     for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < n; c += (int64_t)gridDim.x * 256) {
         const int64_t r = c / chunks;
         const int e0 = (int)(c - r * chunks) * 8;
         float gv[8], uv[8], dv[8];
-        load_params<float, 8>(g + r * a.hidden, e0, a.hidden, gv);
-        load_params<float, 8>(u + r * a.hidden, e0, a.hidden, uv);
+        load_params<float, 8>(g + r * a.gu_pitch, e0, a.hidden, gv);
+        load_params<float, 8>(u + r * a.gu_pitch, e0, a.hidden, uv);
         load_params<T, 8>((const T*)a.dh + r * a.dh_stride, e0, a.hidden, dv);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -474,14 +475,26 @@ static EncodeTiled encode_tiled() {
     }
     return (EncodeTiled)f;
 }
+static bool encode(CUtensorMap* m, EncodeTiled enc, CUtensorMapDataType type, int size, const void* p, int64_t pitch, int64_t rows, int cols,
+                   int planes, cuuint32_t box_cols, cuuint32_t box_rows, cuuint32_t box_planes, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)(pitch * size), (cuuint64_t)((planes > 1 ? rows * pitch : pitch) * size)};
+    const cuuint32_t box[3] = {box_cols, box_rows, box_planes}, step[3] = {1, 1, 1};
+    return enc(m, type, 3, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 // [planes][rows][pitch] of 16-bit values, read in boxes of 64 rows x 64 columns; what lies outside reads as zero
 static bool ff_map(CUtensorMap* m, EncodeTiled enc, const void* p, int64_t pitch, int64_t rows, int cols, int planes, bool half) {
-    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)(pitch * 2), (cuuint64_t)((planes > 1 ? rows * pitch : pitch) * 2)};
-    const cuuint32_t box[3] = {64, 64, 1}, step[3] = {1, 1, 1};
-    return enc(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
-           CUDA_SUCCESS;
+    return encode(m, enc, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p, pitch, rows, cols, planes, 64, 64, 1,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// An output, written in boxes of 32 rows x 64 bytes; g and u together
+template <typename T>
+static bool ff_out_map(CUtensorMap* m, EncodeTiled enc, const void* p, int64_t pitch, int64_t rows, int cols, int planes) {
+    const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : sizeof(T) == 2               ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    return encode(m, enc, type, (int)sizeof(T), p, pitch, rows, cols, planes, 64 / sizeof(T), 32, planes, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <int PLANES, int BN, typename T, bool FWD>
@@ -553,7 +566,30 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
         g.p[i].part = (float*)(ws + q.off_part[i]);
         g.units += g.p[i].sets * g.p[i].tiles_i * g.p[i].tiles_j * g.p[i].splits;
     }
-    if (fwd) g.p[0].out[0] = a.h, g.p[0].out[1] = a.gu;
+    auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    for (int i = 0; i < q.n_problems; ++i) {
+        FfProblem& p = g.p[i];
+        p.out_map[0] = p.out_map[1] = -1;
+        if (fwd) {
+            p.out[0] = a.h;
+            p.h_aligned = at16(a.h) && a.hidden % Chunk<T>::N == 0;
+            if (a.gu != nullptr) {
+                p.out_map[0] = 5;
+                ok = ok && ff_out_map<float>(&g.map[5], enc, a.gu, a.gu_pitch, a.rows, a.hidden, 2);
+            }
+            continue;
+        }
+        for (int k = 0; k < p.sets; ++k)
+            if (p.splits == 1 && p.out[k] != nullptr && at16(p.out[k]) && a.dim % Chunk<T>::N == 0) {
+                const int m = p.a_mn ? 6 + k : 5;
+                p.out_map[k] = m;
+                ok = ok && ff_out_map<T>(&g.map[m], enc, p.out[k], a.dim, p.n_i, a.dim, 1);
+            }
+    }
+    if (!ok) {
+        set_error("gated feed-forward: an output's layout was refused by the driver");
+        return CGB200_ERR_CUDA;
+    }
     g.idesc_type = half ? 0u : (1u << 7) | (1u << 10);
     g.act = a.act, g.polls = kDefaultWaitPolls;
     int rc;
@@ -663,9 +699,11 @@ int cgb200_gated_ff_fwd(const void* x, int64_t x_stride, const void* w_gate, int
     FfArgs a{};
     a.x = x, a.wg = w_gate, a.wu = w_up, a.x_stride = x_stride, a.wg_stride = w_gate_stride, a.wu_stride = w_up_stride;
     a.rows = rows, a.dim = (int)dim, a.hidden = (int)hidden, a.act = activation, a.h = h, a.gu = gate_up;
+    a.gu_pitch = up(hidden, 4);
     if (int rc = ff_check(a, rows, dim, hidden, activation, dtype)) return rc;
     if (rows == 0) return CGB200_OK;
     CGB_REQUIRE(h != nullptr, "gated feed-forward: null buffer");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(gate_up) & 15) == 0, "gated feed-forward: gate_up must be 16-byte aligned");
     const FfPlan q = ff_plan(a, dtype, 0);
     if (int rc = ff_workspace(q, workspace, workspace_bytes)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
@@ -679,6 +717,7 @@ int cgb200_gated_ff_bwd(const void* x, int64_t x_stride, const void* w_gate, int
     FfArgs a{};
     a.x = x, a.wg = w_gate, a.wu = w_up, a.x_stride = x_stride, a.wg_stride = w_gate_stride, a.wu_stride = w_up_stride;
     a.rows = rows, a.dim = (int)dim, a.hidden = (int)hidden, a.act = activation, a.gu = const_cast<float*>(gate_up);
+    a.gu_pitch = up(hidden, 4);
     a.dh = dh, a.dh_stride = dh_stride, a.dx = dx, a.dwg = dw_gate, a.dwu = dw_up;
     if (int rc = ff_check(a, rows, dim, hidden, activation, dtype)) return rc;
     CGB_REQUIRE(rows == 0 || (gate_up != nullptr && dh != nullptr), "gated feed-forward: null buffer");

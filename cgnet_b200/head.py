@@ -199,7 +199,7 @@ def _gated_ff_fwd(x2, wg, wu, act, keep):
     hidden = wg.shape[0]
     dev, dtype = x2.device, _DTYPES[x2.dtype]
     h = torch.empty(rows, hidden, dtype=x2.dtype, device=dev)
-    gate_up = torch.empty(2, rows, hidden, dtype=torch.float32, device=dev) if keep else None
+    gate_up = torch.empty((2, rows, (hidden + 3) & ~3), dtype=torch.float32, device=dev) if keep else None
     operands = (x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
     n = _lib.load().cgb200_gated_ff_workspace_bytes(*operands, rows, dim, hidden, dtype, 0)
     ws = _workspace(n, dev)

@@ -305,7 +305,8 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
 /*
  * Gated feed-forward block:  h = act(x Wg^T) * (x Wu^T),  Wg and Wu [hidden][dim].
  *   h         [rows][hidden], contiguous
- *   gate_up   float[2][rows][hidden]: the two projections, for the backward; NULL where none follows
+ *   gate_up   float[2][rows][hidden rounded up to a multiple of 4]: the two projections, for the backward, 16-byte aligned; NULL
+ *             where none follows
  * Backward: dx [rows][dim], dw_gate and dw_up [hidden][dim], each NULL where it is not wanted; with 0 rows it writes zeros to
  * the weights' gradients.  workspace: cgb200_gated_ff_workspace_bytes bytes (`gradients` = 0 for the forward, else the sum of 1 for
  * dx, 2 for dw_gate and 4 for dw_up, as the call asks for them; the operands' addresses and strides decide whether they have to
