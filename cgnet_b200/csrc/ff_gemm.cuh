@@ -236,6 +236,9 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_ptr, polls = a.polls;
+    // Units are listed longest first; blocks take them in turn, there and back, so that who had a long one gets a short one next.
+    // (In an odd round the places may lie beyond the last unit for this block while other blocks still have one: it is done then.)
+    auto unit_of = [&](int n) { return n * (int)gridDim.x + (n & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); };
 
     // The two issuing roles run on one elected thread: under elect.sync the compiler knows that, and keeps what the copies and
     // products take in uniform registers (under `lane == 0` a copy took 80 cycles to issue and bounded the kernel).
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             int s = 0, issued = 0;
             uint32_t ph = 1;
             bool ok = true;
-            for (int u = blockIdx.x; u < a.units && ok; u += gridDim.x) {
+            for (int n = 0, u; (u = unit_of(n)) < a.units && ok; ++n) {
                 const FfUnit t = ff_unit(a, u, JW);
                 // in registers: what the loop looked up in the arguments each time cost it more than the copies' own time
                 const int kblk = t.p->kblk, a_mn = t.p->a_mn, b_mn = t.p->b_mn, i0 = (int)t.i0, j0 = t.j0, k1 = t.k1;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             int s = 0, acc = 0;
             uint32_t ph = 0, acc_ph = 1;
             bool ok = true;
-            for (int u = blockIdx.x; u < a.units && ok; u += gridDim.x) {
+            for (int n = 0, u; (u = unit_of(n)) < a.units && ok; ++n) {
                 const FfUnit t = ff_unit(a, u, JW);
                 const int a_mn = t.p->a_mn, b_mn = t.p->b_mn, k1 = t.k1;
                 const uint32_t idesc = (1u << 4) | a.idesc_type | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
         int acc = 0, flip = 0;         // flip: the half of the staging area that the next 16-bit block goes through
         uint32_t acc_ph = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
+        for (int n = 0, u; (u = unit_of(n)) < a.units; ++n) {
             const FfUnit t = ff_unit(a, u, JW);
             const FfProblem& p = *t.p;
             const int64_t row0 = t.i0 + quad * 32;

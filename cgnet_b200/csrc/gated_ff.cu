@@ -358,15 +358,39 @@ __global__ void __launch_bounds__(256) ff_reduce_kernel(FfReduceArgs a) {
     const float* src = a.part[p] + set * a.n[p];
     const int64_t step = a.sets[p] * a.n[p];
     T* out = (T*)a.out[p][set];
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n[p]; i += (int64_t)gridDim.x * 256) {
+    const int splits = a.splits[p];
+    const int64_t n = a.n[p];
+    if (n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {      // the parts start on 16-byte boundaries then
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+            float4 s = *(const float4*)(src + i);
+#pragma unroll 4
+            for (int k = 1; k < splits; ++k) {
+                const float4 v = *(const float4*)(src + k * step + i);
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            T r[4] = {from_f32<T>(s.x), from_f32<T>(s.y), from_f32<T>(s.z), from_f32<T>(s.w)};
+            if constexpr (sizeof(T) == 2) {
+                uint2 u;
+                memcpy(&u, r, 8);
+                *(uint2*)(out + i) = u;
+            } else {
+                *(float4*)(out + i) = make_float4(r[0], r[1], r[2], r[3]);
+            }
+        }
+        return;
+    }
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float s = src[i];
-        for (int k = 1; k < a.splits[p]; ++k) s += src[k * step + i];
+#pragma unroll 4
+        for (int k = 1; k < splits; ++k) s += src[k * step + i];
         out[i] = from_f32<T>(s);
     }
 }
 
 // ---- which path, and what it needs -------------------------------------------------------------------------------------
 constexpr int64_t kFfTensorWork = 4 << 20;      // rows x dim x hidden from which the tensor cores are used
+
+constexpr int kFfOutputStages = 8;
 
 struct FfPlan {
     bool tensor;
@@ -439,12 +463,18 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
         p.n_i = a.hidden, p.n_j = a.dim;
         p.out[0] = (grads & 2) ? a.dwg : a.dwu, p.out[1] = a.dwu;
     }
-    const int64_t units = units_at(q.bn);
+    // Units of very different length, or fewer than SMs: a long contraction goes in parts that are added in order afterwards.  A unit's
+    // length is its stages and, for its output, about eight more; one much beyond an SM's share of all would be waited for.
+    int64_t total = 0;
+    for (int i = 0; i < q.n_problems; ++i) {
+        const FfProblem& p = q.problem[i];
+        total += (int64_t)p.sets * p.tiles_i * p.tiles_j * (p.sources * p.kblk + kFfOutputStages);
+    }
+    const double share = (double)total / kNumSM;
     for (int i = 0; i < q.n_problems; ++i) {
         FfProblem& p = q.problem[i];
-        const int stages = p.sources * p.kblk;
-        // fewer tiles than SMs: the contraction in parts of at least four stages, added in order afterwards
-        int splits = fwd || units >= kNumSM ? 1 : (int)std::min<int64_t>(8, kNumSM / units);
+        const int stages = p.sources * p.kblk, length = stages + kFfOutputStages;
+        int splits = fwd || length <= 1.5 * share ? 1 : (int)std::min(8.0, length / std::max(0.5 * share, 2.0 * kFfOutputStages) + 0.999);
         splits = std::max(1, std::min(splits, stages / 4));
         p.kper = (stages + splits - 1) / splits;
         p.splits = (stages + p.kper - 1) / p.kper;
@@ -608,7 +638,7 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
     }
     if (any && !fwd) {
         launch_begin(kid, st);
-        ff_reduce_kernel<T><<<dim3((unsigned)std::min<int64_t>((n + 255) / 256, kNumSM * 8), 4), 256, 0, st>>>(r);
+        ff_reduce_kernel<T><<<dim3((unsigned)std::min<int64_t>((n + 1023) / 1024, kNumSM * 8), 2 * g.problems), 256, 0, st>>>(r);
         launch_end(kid, st);
         CGB_CUDA(cudaGetLastError());
     }
