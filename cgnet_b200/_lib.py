@@ -73,8 +73,6 @@ FN_PRESENT, FN_UPDATE, FN_KEEP_MID = 0x1, 0x2, 0x4
 PLAN_DEPTHWISE = 0x1
 AUTO = -1
 F32, BF16, F16 = range(3)
-ACT_SILU, ACT_GELU, ACT_RELU = range(3)
-MAX_TOP, MAX_TEACHER = 128, 1024
 (OPT_TC_FWD, OPT_TC_GRAD_W, OPT_TC_GRAD_F, OPT_TC_STAGES, OPT_FWD_SLAB, OPT_GRAD_F_SPLIT, OPT_STATS_SPLIT, OPT_BWD_SERIAL,
  OPT_WAIT_POLLS, OPT_TEST_IDLE_MMA, OPT_TC_STAGED, OPT_TC_ABUF, OPT_TC_FWD_SPLIT, OPT_GRAD_MID_GEMM,
  OPT_FWD_KEEP_MID, OPT_SHORT_GROUP) = range(16)

@@ -338,7 +338,7 @@ def check_log_probs(z, target, top, g_lp=None, g_ent=None):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows, classes, top", [(1, 1, 1), (3, 2, 2), (4, 10, 10), (64, 55, 5), (9, 130, 128), (17, 1000, 20), (3, 1024, 128), (5, 1025, 20), (2, 2047, 3),
-                                                (300, 5000, 7), (2, 9001, 128), (1, 40003, 1), (1, 131072, 20), (3, 131075, 128), (160, 16385, 0)])
+                                                (300, 5000, 7), (2, 9001, 128), (1, 40003, 1), (1, 131072, 20), (3, 131075, 128), (160, 16385, 0), (150, 70001, 128), (150, 40000, 50)])
 def test_log_probs(rows, classes, top, dtype):
     g = gen(rows + classes + top)
     z = (3 * randn(g, rows, classes)).to(dtype)
@@ -570,6 +570,16 @@ def test_network_with_a_head_trains_and_is_taught():
     fast = cg.SphericalCNN_fast(3, [2] * 4, 2, num_channels_input=2, head=(16, 5))
     c = torch.randn(6, 2, 16, 2, device=cuda())
     assert fast(c).shape == (6, 5) and fast.embed(c).shape == (6, fast.output_length) and fast.log_probs(c, top=2).top_ids.shape == (6, 2)
+
+
+def test_second_derivatives_are_refused():
+    import cgnet_b200 as cg
+    g = gen(41)
+    x, w = randn(g, 4, 8).requires_grad_(), randn(g, 6, 8).requires_grad_()
+    ids = torch.zeros(4, 2, dtype=torch.long, device=cuda())
+    for out in (cg.layer_norm(x), cg.gated_feed_forward(x, w, w), cg.log_probs(x).entropy, cg.distillation_loss(x, ids, randn(g, 4, 2))):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
 
 
 def chain(x, w, b, wg, wu, ws, target, ids, scores):
