@@ -28,6 +28,7 @@ constexpr int kScChunks = 512;                   // chunks with a score that may
 constexpr int kScNewKeys = 256;                  // candidates expected between two looks
 constexpr int kScMaxTop = 128;
 constexpr int kScWarpValues = 32;                // values per lane of the kernel for short rows
+constexpr int kScWarpList = 256;                 // classes a warp of it ranks against each other
 constexpr float kScMargin = 10.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
@@ -308,7 +309,55 @@ __global__ void __launch_bounds__(kScThreads) scores_warp_kernel(ScoreArgs a) {
         }
     }
     if (a.top == 0) return;
-    // the best of each lane, and the best of those, `top` times over
+    uint32_t order[CH][N];             // 0 beyond the row
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = (lane + 32 * c) * N - ph + i;
+            order[c][i] = e >= 0 && e < a.classes ? order_of(v[c][i]) : 0u;
+        }
+    auto leave = [&](int k, uint64_t key) {
+        a.top_ids[row * a.top + k] = index_of(key);
+        a.top_lp[row * a.top + k] = log_prob_of(st, log2_s, score_of((uint32_t)(key >> 32)), a.scale);
+    };
+    if (a.top > 2) {
+        // the top-th highest order, in its upper 16 bits; the classes from there on go to a list and are counted against each
+        // other.  (Picking the best of all lanes `top` times over took a microsecond for each.)
+        __shared__ uint64_t lists[kScThreads / 32][kScWarpList];
+        uint64_t* list = lists[threadIdx.x >> 5];
+        uint32_t t = 0;
+        for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+            int n = 0;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < N; ++i) n += order[c][i] >= (t | bit);
+            if (__reduce_add_sync(0xffffffffu, n) >= a.top) t |= bit;
+        }
+        int n = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool in = order[c][i] >= t && order[c][i] != 0;
+                const unsigned votes = __ballot_sync(0xffffffffu, in);
+                const int at = n + __popc(votes & ((1u << lane) - 1u));
+                if (in && at < kScWarpList) list[at] = ((uint64_t)order[c][i] << 32) | (0xffffffffu - (uint32_t)((lane + 32 * c) * N - ph + i));
+                n += __popc(votes);
+            }
+        if (n <= kScWarpList) {
+            __syncwarp();
+            for (int i = lane; i < n; i += 32) {
+                const uint64_t key = list[i];
+                int rank = 0;
+                for (int j = 0; j < n; ++j) rank += list[j] > key;
+                if (rank < a.top) leave(rank, key);
+            }
+            return;
+        }
+    }
+    // one or two classes, or many of one score: the best of each lane, and the best of those, `top` times over
     uint64_t last = ~0ull, best = 0;
     for (int k = 0; k < a.top; ++k) {
         if (k == 0 || best == last) {       // this lane's best is not known, or was the one just taken
@@ -317,19 +366,14 @@ __global__ void __launch_bounds__(kScThreads) scores_warp_kernel(ScoreArgs a) {
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int e = (lane + 32 * c) * N - ph + i;
-                    if (e < 0 || e >= a.classes) continue;
-                    const uint64_t key = key_of(v[c][i], (uint32_t)e);
-                    if (key < last && key > best) best = key;
+                    const uint64_t key = ((uint64_t)order[c][i] << 32) | (0xffffffffu - (uint32_t)((lane + 32 * c) * N - ph + i));
+                    if (order[c][i] != 0 && key < last && key > best) best = key;
                 }
         }
         const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
         const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
         last = ((uint64_t)hi << 32) | lo;
-        if (lane == 0) {
-            a.top_ids[row * a.top + k] = index_of(last);
-            a.top_lp[row * a.top + k] = log_prob_of(st, log2_s, score_of(hi), a.scale);
-        }
+        if (lane == 0) leave(k, last);
     }
 }
 

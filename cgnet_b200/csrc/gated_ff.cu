@@ -388,7 +388,15 @@ __global__ void __launch_bounds__(256) ff_reduce_kernel(FfReduceArgs a) {
 }
 
 // ---- which path, and what it needs -------------------------------------------------------------------------------------
-constexpr int64_t kFfTensorWork = 4 << 20;      // rows x dim x hidden from which the tensor cores are used
+// The tensor cores are used from this length of the longest contraction on (forward: dim; backward: rows or 2 hidden), or from this
+// much work (rows x dim x hidden).  CUDA cores / tensor cores, us, launches of a graph: 16 bits, forward 16 x 64 -> 64 5.0 / 6.3,
+// 16 x 128 -> 256 6.8 / 6.4, 10 x 976 -> 104 36 / 9.6; backward 7.0 / 7.2, 19 / 8.7, 11 / 7.8.  float32 (three planes, a copy in
+// front), forward 100 x 256 -> 256 9.5 / 13, 32 x 1024 -> 128 27 / 25; backward 16 / 19, 1000 x 48 -> 48 28 / 21.
+struct FfLimits {
+    int forward, backward;
+    int64_t work;
+};
+static FfLimits ff_limits(int dtype) { return dtype == CGB200_F32 ? FfLimits{768, 640, 16 << 20} : FfLimits{128, 160, 8 << 20}; }
 
 constexpr int kFfOutputStages = 8;
 
@@ -412,7 +420,9 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     FfPlan q{};
     const bool fwd = grads == 0;
     const int64_t work = a.rows * a.dim * (int64_t)a.hidden;
-    q.tensor = a.rows > 0 && work >= kFfTensorWork && !(fwd && a.rows <= kFfFewRows);
+    const FfLimits limit = ff_limits(dtype);
+    const bool longer = fwd ? a.dim >= limit.forward : std::max<int64_t>(a.rows, 2 * (int64_t)a.hidden) >= limit.backward;
+    q.tensor = a.rows > 0 && (longer || work >= limit.work) && !(fwd && a.rows <= kFfFewRows);
     if (!q.tensor) return q;
     q.planes = dtype == CGB200_F32 ? 3 : 1;
     const bool need[3] = {true, fwd || (grads & 1), fwd || (grads & 1)};
@@ -543,6 +553,10 @@ template <typename T>
 static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cudaStream_t st) {
     constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
     const bool fwd = grads == 0;
+    // a thread that has made no CUDA call yet (autograd's, in its first backward) has no context, and the driver refuses to encode
+    int device;
+    CGB_CUDA(cudaGetDevice(&device));
+    CGB_CUDA(cudaSetDevice(device));
     EncodeTiled enc = encode_tiled();
     if (enc == nullptr) {
         set_error("the driver has no cuTensorMapEncodeTiled");

@@ -627,6 +627,36 @@ def test_captured_steps_replay_and_do_not_disturb_each_other():
             assert all(torch.equal(p, q) for p, q in zip(grads, want))
 
 
+def test_threads_that_made_no_cuda_call_before():
+    """The first CUDA call of a thread is the operator's (memory comes from torch's cache)."""
+    import threading
+
+    import cgnet_b200 as cg
+    g = gen(43)
+    x, wg, wu, dh = (t.bfloat16() for t in (randn(g, 256, 256), randn(g, 512, 256) / 16, randn(g, 512, 256) / 16, randn(g, 256, 512)))
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    want = torch.autograd.grad(cg.gated_feed_forward(*leaves), leaves, dh)
+    with torch.no_grad():
+        h = cg.gated_feed_forward(x, wg, wu)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            with torch.no_grad():
+                got.append(cg.gated_feed_forward(x, wg, wu))
+        except RuntimeError as e:
+            got.append(e)
+
+    for _ in range(2):
+        thread = threading.Thread(target=work)
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert all(isinstance(p, torch.Tensor) and torch.equal(p, h) for p in got), got
+    assert all(torch.isfinite(p).all() for p in want)
+
+
 def test_side_streams_and_two_calls_at_once():
     ts = [t.requires_grad_(i < 6) for i, t in enumerate(chain_inputs(3, rows=700, dim=256, hidden=512))]
     loss, _ = chain(*ts)
