@@ -999,6 +999,7 @@ int cgb200_log_probs_fwd(const void* logits, int64_t stride, const int64_t* targ
     if (rows == 0) return CGB200_OK;
     CGB_REQUIRE(entropy != nullptr && (targets == nullptr || log_prob != nullptr) && (top == 0 || (top_log_probs != nullptr && top_ids != nullptr)),
                 "log probabilities: null buffer");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "log probabilities: stats must be 8-byte aligned");
     ScoreArgs a{};
     a.z = logits, a.z_stride = stride, a.rows = rows, a.classes = (int)classes, a.scale = kLog2e, a.stats = (float2*)stats;
     a.targets = targets, a.log_prob = log_prob, a.entropy = entropy, a.top = top, a.top_lp = top_log_probs, a.top_ids = top_ids;
@@ -1010,6 +1011,7 @@ int cgb200_log_probs_bwd(const void* logits, int64_t stride, const int64_t* targ
     if (int rc = score_check(logits, stride, rows, classes, dtype)) return rc;
     if (rows == 0) return CGB200_OK;
     CGB_REQUIRE(stats != nullptr && dlogits != nullptr && (g_entropy == nullptr || entropy != nullptr), "log probabilities: null buffer");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "log probabilities: stats must be 8-byte aligned");
     ScoreGradArgs a{};
     a.f.z = logits, a.f.z_stride = stride, a.f.rows = rows, a.f.classes = (int)classes, a.f.scale = kLog2e, a.f.stats = (float2*)stats;
     a.f.targets = targets, a.f.entropy = const_cast<float*>(entropy);

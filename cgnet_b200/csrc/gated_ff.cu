@@ -705,6 +705,7 @@ static int ff_bwd(const FfArgs& a, const FfPlan& q, int grads, char* ws, cudaStr
 static int ff_check(const FfArgs& a, int64_t rows, int64_t dim, int64_t hidden, int act, int dtype) {
     CGB_REQUIRE(rows >= 0 && rows <= (1ll << 24) && dim > 0 && dim <= (1 << 20) && hidden > 0 && hidden <= (1 << 20),
                 "gated feed-forward: sizes out of range");
+    CGB_REQUIRE(rows * std::max(dim, hidden) <= (1ll << 38), "gated feed-forward: sizes out of range");      // the tile counts are int
     CGB_REQUIRE(dtype >= CGB200_F32 && dtype <= CGB200_F16, "gated feed-forward: unknown type");
     CGB_REQUIRE(act >= CGB200_ACT_SILU && act <= CGB200_ACT_RELU, "gated feed-forward: unknown activation");
     CGB_REQUIRE(a.wg != nullptr && a.wu != nullptr && (rows == 0 || a.x != nullptr), "gated feed-forward: null buffer");

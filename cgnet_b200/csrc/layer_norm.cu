@@ -750,6 +750,7 @@ int cgb200_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, c
     if (rows == 0) return CGB200_OK;
     CGB_REQUIRE(x != nullptr && y != nullptr, "layer norm: null buffer");
     CGB_REQUIRE(x_stride >= 0 && x_stride <= (1ll << 40), "layer norm: row stride out of range");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "layer norm: stats must be 8-byte aligned");
     const LnArgs a{x, x_stride, weight, bias, eps, rows, dim};
     cudaStream_t st = (cudaStream_t)stream;
 #define CGB_CALL(T_, P_) ln_fwd<T_, P_>(a, y, (float2*)stats, st)
@@ -773,6 +774,7 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
     if (!params && (dx == nullptr || rows == 0)) return CGB200_OK;
     CGB_REQUIRE(rows == 0 || (x != nullptr && dy != nullptr && stats != nullptr), "layer norm: null buffer");
     CGB_REQUIRE(x_stride >= 0 && x_stride <= (1ll << 40) && dy_stride >= 0 && dy_stride <= (1ll << 40), "layer norm: row stride out of range");
+    CGB_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "layer norm: stats must be 8-byte aligned");
     if (params) {
         const int64_t need = cgb200_layer_norm_bwd_workspace_bytes(rows, dim, dtype);
         if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {

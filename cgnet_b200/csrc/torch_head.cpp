@@ -80,7 +80,9 @@ Tensor classes_of(PyObject* o, const char* name, at::IntArrayRef want, const Ten
     return t.to(at::kLong).contiguous();
 }
 // (rows, columns) whose columns are neighbours in memory; rows may be any distance apart
-Tensor rows_of(const Tensor& t) {
+// (a lazily negated view, such as the imaginary part of a conjugate, is negated first)
+Tensor rows_of(const Tensor& given) {
+    const Tensor t = given.is_neg() ? given.resolve_neg() : given;
     const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
     return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
@@ -173,7 +175,7 @@ Tensor layer_norm(PyObject* const* a) {
         check_shape(t, names[i], {x.size(-1)});
         if (t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat)
             fail(std::string(names[i]) + " must be " + type_name(x) + " or float32, got " + type_name(t));
-        p[i] = t.contiguous();
+        p[i] = t.resolve_neg().contiguous();
     }
     if (p[0].has_value() && p[1].has_value() && p[0]->scalar_type() != p[1]->scalar_type())
         fail("weight and bias must have one type, got " + type_name(*p[0]) + " and " + type_name(*p[1]));
@@ -287,8 +289,8 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
         once();
         const auto saved = ctx->get_saved_variables();
         const Tensor &z = saved[0], &targets = saved[1], &ent = saved[2], &stats = saved[3];
-        const Tensor g_lp = targets.defined() && grads[0].defined() ? grads[0].contiguous() : Tensor();
-        const Tensor g_ent = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor g_lp = targets.defined() && grads[0].defined() ? grads[0].resolve_neg().contiguous() : Tensor();
+        const Tensor g_ent = grads[1].defined() ? grads[1].resolve_neg().contiguous() : Tensor();
         if (!ctx->needs_input_grad(0) || (!g_lp.defined() && !g_ent.defined())) return {Tensor(), Tensor(), Tensor()};
         const int64_t rows = z.size(0), classes = z.size(1);
         const Tensor dz = empty({rows, classes}, z);
@@ -352,7 +354,7 @@ struct Distill : torch::autograd::Function<Distill> {
         once();
         const auto saved = ctx->get_saved_variables();
         const Tensor &z = saved[0], &ids = saved[1], &scores = saved[2], &stats = saved[3];
-        const Tensor g = grads[0].contiguous();
+        const Tensor g = grads[0].resolve_neg().contiguous();
         const int64_t rows = z.size(0), classes = z.size(1);
         const Tensor dz = empty({rows, classes}, z);
         const Launch l(z);
@@ -381,7 +383,7 @@ Tensor distillation_loss(PyObject* const* a) {
         fail("temperature must be between 0.001 and 1000, got " + std::to_string(temperature));
     }
     check_cuda(z, "logits");
-    const Tensor z2 = rows_of(z), scores = given.detach().reshape({-1, k}).contiguous();
+    const Tensor z2 = rows_of(z), scores = given.detach().resolve_neg().reshape({-1, k}).contiguous();
     const Tensor loss = at::GradMode::is_enabled() && z.requires_grad() ? Distill::apply(z2, ids, scores, temperature)
                                                                         : distill_fwd(z2, ids, scores, temperature, false).first;
     return lead.size() == 1 ? loss : loss.view(lead);

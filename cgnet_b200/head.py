@@ -12,7 +12,8 @@ current stream; the checks of the arguments, the allocations and the autograd no
 ``csrc/torch_head.cpp``).  There is no CPU path and no fallback: a missing library or a bad argument raises RuntimeError before
 anything is launched.  Every operator is differentiable once, can be captured in a CUDA graph, and gives the same bits from run
 to run for the same tensors.  (As with any torch operator, capture a backward pass only while no eager graph of the same leaves
-is alive: torch ties a leaf's gradient accumulation to the stream it was first used on.)
+is alive: torch ties a leaf's gradient accumulation to the stream it was first used on.)  The order of a row's sums follows
+the 16-byte groups it lies in, so its last bits can depend on its address modulo 16.
 """
 import collections
 import importlib

@@ -280,7 +280,8 @@ int cgb200_raycast_sphere(const float* vertices, int64_t n_vertices, const int32
  * The operators between a network's invariant embedding and its answers (no counterpart in the reference's kernels, which
  * leaves them to torch).  Matrices are row-major with the given number of values between rows (`stride`), values of one of
  * three types; sums, norms and softmax statistics are held in float32 or more and every result is rounded once.  Pointers
- * need the alignment of their type only.  Results do not depend on timing (no float atomics).
+ * need the alignment of their type only, except where more is said.  Results do not depend on timing (no float atomics); the order of
+ * a row's sums follows the 16-byte groups it lies in, so its last bits can depend on its address modulo 16.
  */
 #define CGB200_F32              0
 #define CGB200_BF16             1
@@ -290,7 +291,7 @@ int cgb200_raycast_sphere(const float* vertices, int64_t n_vertices, const int32
  * Layer norm of each row:  y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps).
  *   weight, bias   [dim] of type param_dtype (that of x, or CGB200_F32); NULL = 1 and 0
  *   y              [rows][dim], contiguous
- *   stats          float[rows][2] (mean, rstd) for the backward; NULL where none follows
+ *   stats          float[rows][2] (mean, rstd) for the backward, 8-byte aligned; NULL where none follows
  * Backward: dx [rows][dim], dweight and dbias [dim] of type param_dtype, each NULL where it is not wanted.  With dweight or
  * dbias it needs a workspace of cgb200_layer_norm_bwd_workspace_bytes (16-byte aligned, contents undefined); with 0 rows it
  * writes zeros to them.
@@ -311,6 +312,7 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
  * the weights' gradients.  workspace: cgb200_gated_ff_workspace_bytes bytes (`gradients` = 0 for the forward, else the sum of 1 for
  * dx, 2 for dw_gate and 4 for dw_up, as the call asks for them; the operands' addresses and strides decide whether they have to
  * be copied), 256-byte aligned, contents undefined; one workspace serves one call at a time.
+ * A tensor-core block that gives up on a bounded wait fills what it still owes with NaN.
  * Small products run on the CUDA cores, others on the tensor cores (float32 in three bfloat16 parts, accurate to float32).  A row of
  * x that is not finite spoils that row of h and dx; in float32 it may come out as NaN where the formula gives an infinity.
  */
@@ -331,7 +333,7 @@ int cgb200_gated_ff_bwd(const void* x, int64_t x_stride, const void* w_gate, int
  *   targets         int64[rows]; a negative class marks a row without one (log probability 0, no gradient through it), one beyond
  *                   the last gives NaN.  NULL: none wanted (log_prob unused)
  *   top             0..128, at most `classes`; top_ids int64[rows][top] in order of score, equal scores by class, NaN first
- *   stats           float[rows][2] for the backward, NULL where none follows
+ *   stats           float[rows][2] for the backward, 8-byte aligned, NULL where none follows
  * A row of nothing but -inf has no distribution: log probabilities -inf, entropy 0, gradients 0.
  * Backward: dlogits [rows][classes] = gradient through log_prob and entropy (g_* float[rows]; NULL = 0).
  */

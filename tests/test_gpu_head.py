@@ -572,6 +572,24 @@ def test_network_with_a_head_trains_and_is_taught():
     assert fast(c).shape == (6, 5) and fast.embed(c).shape == (6, fast.output_length) and fast.log_probs(c, top=2).top_ids.shape == (6, 2)
 
 
+def test_lazily_negated_views():
+    """The imaginary part of a conjugate is a view with torch's negative bit: its memory holds the opposite sign."""
+    import cgnet_b200 as cg
+    g = gen(47)
+
+    def negated(*shape):
+        t = torch.complex(randn(g, *shape), randn(g, *shape)).conj().imag
+        assert t.is_neg()
+        return t, t.resolve_neg().contiguous()
+
+    (x, x_), (w, w_), (b, b_), (v, v_), (s, s_) = negated(6, 40), negated(40), negated(40), negated(24, 40), negated(6, 5)
+    ids = torch.randint(0, 40, (6, 5), generator=g, device=cuda())
+    assert torch.equal(cg.layer_norm(x, w, b), cg.layer_norm(x_, w_, b_))
+    assert torch.equal(cg.gated_feed_forward(x, v, v), cg.gated_feed_forward(x_, v_, v_))
+    assert all(torch.equal(p, q) for p, q in zip(cg.log_probs(x, ids[:, 0], top=3), cg.log_probs(x_, ids[:, 0], top=3)))
+    assert torch.equal(cg.distillation_loss(x, ids, s), cg.distillation_loss(x_, ids, s_))
+
+
 def test_second_derivatives_are_refused():
     import cgnet_b200 as cg
     g = gen(41)

@@ -65,20 +65,27 @@ def test_library_refusals_need_no_gpu():
     assert lib.cgb200_layer_norm_fwd(p, -4, None, None, 1e-5, p, None, 2, 4, 0, 0, None) == bad
     assert lib.cgb200_layer_norm_fwd(None, 4, None, None, 1e-5, p, None, 2, 4, 0, 0, None) == bad
     assert lib.cgb200_layer_norm_fwd(None, 4, None, None, 1e-5, None, None, 0, 4, 0, 0, None) == 0
+    assert lib.cgb200_layer_norm_fwd(p, 4, None, None, 1e-5, p, p + 4, 2, 4, 0, 0, None) == bad
     assert lib.cgb200_layer_norm_bwd_workspace_bytes(-1, 4, 0) == -1
     assert lib.cgb200_layer_norm_bwd(p, 64, p, 64, None, p, p, p, p, 100000, 64, 0, 0, None, 0, None) == 4
     assert b"need" in lib.cgb200_last_error()
     assert lib.cgb200_gated_ff_fwd(p, 4, p, 4, p, 4, 3, p, None, 2, 4, 4, 0, None, 0, None) == bad
     assert lib.cgb200_gated_ff_fwd(p, 4, p, 4, None, 4, 0, p, None, 2, 4, 4, 0, None, 0, None) == bad
     assert lib.cgb200_gated_ff_fwd(p, 4, p, 4, p, 4, 0, p, None, 2, 4, (1 << 20) + 1, 0, None, 0, None) == bad
+    assert lib.cgb200_gated_ff_fwd(p, 4, p, 4, p, 4, 0, p, p + 4, 2, 4, 4, 0, None, 0, None) == bad
+    assert lib.cgb200_gated_ff_fwd(p, 1 << 20, p, 1 << 20, p, 1 << 20, 0, p, None, 1 << 24, 1 << 20, 4, 0, None, 0, None) == bad
+    assert lib.cgb200_gated_ff_workspace_bytes(p, 4, p, 4, p, 4, 2, 0, 4, 0, 0) == -1
+    assert lib.cgb200_gated_ff_fwd(p, 64, p, 64, p, 64, 0, p, None, 4096, 1024, 1024, 0, None, 0, None) == 4
     assert lib.cgb200_gated_ff_bwd(p, 4, p, 4, p, 4, 0, None, p, 4, p, p, p, 2, 4, 4, 0, None, 0, None) == bad
     assert lib.cgb200_log_probs_fwd(p, 4, None, 5, None, p, p, p, None, 2, 4, 0, None) == bad
     assert lib.cgb200_log_probs_fwd(p, 400, None, 129, None, p, p, p, None, 2, 400, 0, None) == bad
     assert lib.cgb200_log_probs_fwd(p, 4, p, 0, None, p, None, None, None, 2, 4, 0, None) == bad
+    assert lib.cgb200_log_probs_fwd(p, 4, None, 1, None, p, p, p, p + 4, 2, 4, 0, None) == bad
     assert lib.cgb200_log_probs_bwd(p, 4, None, p, None, None, p, p, 2, 4, 0, None) == bad
     assert lib.cgb200_distill_fwd(p, 4, p, p, 0, 0, 1.0, p, None, 2, 4, 0, None) == bad
     assert lib.cgb200_distill_fwd(p, 4, p, p, 2, 7, 1.0, p, None, 2, 4, 0, None) == bad
     assert lib.cgb200_distill_fwd(p, 4, p, p, 2, 0, 0.0, p, None, 2, 4, 0, None) == bad
+    assert lib.cgb200_distill_fwd(p, 4, p, p, 2, 0, 1.0, p, p + 8, 2, 4, 0, None) == bad
     assert lib.cgb200_distill_bwd(p, 4, p, p, 2, 0, 1.0, None, p, p, 2, 4, 0, None) == bad
 
 
