@@ -42,7 +42,7 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
 // the row needs is on its way before the first value is waited for.  EDGE: rows (or weight and bias) that do not start on 16-byte
 // boundaries or do not end on them; without it every chunk is inside the row or behind it.
 template <typename T, typename P, int CH, bool WARP, bool EDGE>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, float inv_n, T* __restrict__ y, float2* __restrict__ stats) {
+__global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, float inv_n, T* __restrict__ y, float2* __restrict__ stats) {
     constexpr int N = Chunk<T>::N;
     __shared__ float red[2][32];
     __shared__ uint4 last[EDGE && !WARP ? 32 : 1];     // each warp's last chunk, for the next warp
@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, flo
     const T* xr = (const T*)a.x + row * a.x_stride;
     T* yr = y + row * a.dim;
     const int k0 = WARP ? 0 : warp * 32 * CH, k = k0 + lane;       // this thread's first chunk, the next ones are 32 further
+    const bool before = EDGE && row > 0 && a.x_stride >= n && n >= N, behind = EDGE && row + 1 < a.rows && a.x_stride >= n && n >= N;
     uint4 raw[CH];
     Params<P, N> w[CH], b[CH];
     auto load_wb = [&]() {
@@ -70,15 +71,20 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, flo
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e0 = (k + 32 * c) * N;
-        if (EDGE) raw[c] = load_at(xr, row_phase(xr), k + 32 * c, n);
+        if (EDGE) raw[c] = load_at(xr, row_phase(xr), k + 32 * c, n, before, behind);
         else raw[c] = e0 < n ? *reinterpret_cast<const uint4*>(xr + e0) : make_uint4(0, 0, 0, 0);
     }
-    if (CH <= 2) load_wb();
+    if (CH <= 2 || WARP) load_wb();
     float v[CH][N];
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         unpack16(raw[c], v[c], (const T*)nullptr);
+        if (EDGE && (k + 32 * c) * N + N > n) {      // the row's end: what is the neighbour's goes
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if ((k + 32 * c) * N + i >= n) v[c][i] = 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) s += v[c][i];
     }
@@ -99,7 +105,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) ln_fwd_kernel(LnArgs a, flo
     }
     const float rstd = 1.f / sqrtf(row_sum<WARP>(q, red[1]) * inv_n + a.eps);
     if (stats != nullptr && (WARP ? lane : (int)threadIdx.x) == 0) stats[row] = make_float2(mean, rstd);
-    if (CH > 2) load_wb();
+    if (CH > 2 && !WARP) load_wb();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e0 = (k + 32 * c) * N;
@@ -583,9 +589,9 @@ static int ln_fwd(const LnArgs& a, void* y, float2* stats, cudaStream_t st) {
     launch_begin(K_LN_FWD, st);
     if (chunks <= 32 * kLnMaxChunks) {
         const int ch = pow2_at_least((chunks + 31) / 32);
-        const unsigned grid = (unsigned)((a.rows + 7) / 8);
-        if (edge) ln_fwd_launch<T, P, true, true>(ch, grid, 256, a, (T*)y, stats, st);
-        else ln_fwd_launch<T, P, true, false>(ch, grid, 256, a, (T*)y, stats, st);
+        const unsigned grid = (unsigned)((a.rows + 3) / 4);
+        if (edge) ln_fwd_launch<T, P, true, true>(ch, grid, 128, a, (T*)y, stats, st);
+        else ln_fwd_launch<T, P, true, false>(ch, grid, 128, a, (T*)y, stats, st);
     } else if (chunks <= 1024 * kLnMaxChunks) {
         // four chunks a thread; two and twice the threads took 39 instead of 31 us at 8192 x 4096 bf16
         const int ch = kLnMaxChunks, threads = (int)((chunks + 32 * ch - 1) / (32 * ch)) * 32;

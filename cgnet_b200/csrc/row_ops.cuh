@@ -133,21 +133,23 @@ __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int b
     for (int j = 0; j < 4; ++j) x[j] = bytes & 2 ? __funnelshift_r(x[j], x[j + 1], 16) : x[j];
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
-// Group g of a row of n values whose aligned groups start `ph` values before it; zeros outside the row.
+// Group g of a row of n values whose aligned groups start `ph` values before it; zeros outside the row.  `before`, `behind`: the
+// matrix has a row of as many values before and behind this one, so that a group at the row's end may be read whole: what
+// it holds of the neighbour is then in the result.
 template <typename T>
-__device__ __forceinline__ uint4 load_group(const T* row, int ph, int g, int n) {
+__device__ __forceinline__ uint4 load_group(const T* row, int ph, int g, int n, bool before = false, bool behind = false) {
     constexpr int N = Chunk<T>::N;
     const int e0 = g * N - ph;
-    if (e0 >= 0 && e0 + N <= n) return *reinterpret_cast<const uint4*>(row + e0);
+    if ((e0 >= 0 || before) && (e0 + N <= n || (behind && e0 < n))) return *reinterpret_cast<const uint4*>(row + e0);
     if (e0 < n) return load_pieces(row, e0, n, 0.f);
     return make_uint4(0, 0, 0, 0);
 }
 // Chunk k of such a row.
 template <typename T>
-__device__ __forceinline__ uint4 load_at(const T* row, int ph, int k, int n) {
-    const uint4 lo = load_group(row, ph, k, n);
+__device__ __forceinline__ uint4 load_at(const T* row, int ph, int k, int n, bool before = false, bool behind = false) {
+    const uint4 lo = load_group(row, ph, k, n, before, behind);
     if (ph == 0) return lo;
-    return shifted(lo, load_group(row, ph, k + 1, n), ph * (int)sizeof(T));
+    return shifted(lo, load_group(row, ph, k + 1, n, before, behind), ph * (int)sizeof(T));
 }
 // Writes the groups of a row of n values that end in this warp's chunks k0 + lane, k0 + 32 + lane, ... (CH of them, in `u`), `ph` as
 // above.  `before` is the last chunk before this warp's (any value where there is none).  The values of the warp's last
