@@ -208,6 +208,10 @@ __device__ __forceinline__ void gate(float (&g)[16], const float (&u)[16]) {
     for (int i = 0; i < 16; ++i) g[i] = activate_as<ACT, false>(g[i]).x * u[i];
 }
 
+// Alone on the GPU at 8192 rows, 2048 -> 5120, bf16: forward 237 us in inference (1450 TFLOP/s), 301 when g and u are kept (336 MB
+// more to write), both backward products 456 us (1.5 PFLOP/s, tensor pipe 83 %).  Not the epilogue but the main loop bounds the
+// forward: 625 cycles per 64-term stage in inference and 750 in training against 512 of MMA, because the 48 KB a stage brings into
+// the SM share the way from L2 with what the epilogue writes.  Height of a group of row tiles (4, 8, 16, 32): within 3 %.
 template <int PLANES, int BN, typename T, bool FWD>
 __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_constant__ FfGemmArgs a) {
     constexpr int kStage = PLANES * (kFfBM + BN) * kFfBK * 2;
