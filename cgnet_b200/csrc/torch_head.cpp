@@ -58,6 +58,7 @@ const Tensor& values_of(PyObject* o, const char* name, const Tensor* like = null
     const Tensor& t = tensor_of(o, name);
     if (type_code(t) < 0) fail(std::string(name) + " must be float32, bfloat16 or float16, got " + type_name(t));
     if (like != nullptr) check_device(t, name, *like);
+    if (t._fw_grad(0).defined()) fail(std::string(name) + " has a forward-mode derivative, which the operators of cgnet_b200.head do not pass on");
     return t;
 }
 void check_shape(const Tensor& t, const char* name, at::IntArrayRef want) {
@@ -77,7 +78,7 @@ Tensor classes_of(PyObject* o, const char* name, at::IntArrayRef want, const Ten
     const Tensor& t = THPVariable_Unpack(o);
     check_device(t, name, like);
     check_shape(t, name, want);
-    return t.to(at::kLong).contiguous();
+    return t.to(at::kLong).resolve_neg().contiguous();
 }
 // (rows, columns) whose columns are neighbours in memory; rows may be any distance apart
 // (a lazily negated view, such as the imaginary part of a conjugate, is negated first)

@@ -53,6 +53,17 @@ def test_refusals(call, message):
         call()
 
 
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwad
+    ids, scores = torch.zeros(4, 2, dtype=torch.long), torch.zeros(4, 2)
+    with fwad.dual_level():
+        d, dw = fwad.make_dual(X, torch.ones_like(X)), fwad.make_dual(W, torch.ones_like(W))
+        for call in (lambda: cg.layer_norm(d), lambda: cg.gated_feed_forward(X, W, dw), lambda: cg.log_probs(d),
+                     lambda: cg.distillation_loss(d, ids, scores)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
 def test_library_refusals_need_no_gpu():
     """The C entry points return a status for bad arguments before any CUDA call."""
     lib = _lib.load()
