@@ -383,18 +383,18 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         fence_mbar_init();
         for (int s = 0; s < stages && s < n_here; ++s) fetch(s, s);
     }
-    float w[NC][VE], dw[NC][VE], db[NC][VE];
+    uint64_t w[NC][VE / 2], dw[NC][VE / 2], db[NC][VE / 2];      // pairs of columns
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int e0 = (k + 32 * c) * VE;
+        float wv[VE];
         if (a.w != nullptr) {
-            load_params<P, VE>((const P*)a.w, e0, a.dim, w[c]);
+            load_params<P, VE>((const P*)a.w, (k + 32 * c) * VE, a.dim, wv);
         } else {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) w[c][i] = 1.f;
+            for (int i = 0; i < VE; ++i) wv[i] = 1.f;
         }
 #pragma unroll
-        for (int i = 0; i < VE; ++i) dw[c][i] = db[c][i] = 0.f;
+        for (int i = 0; i < VE / 2; ++i) w[c][i] = pair(wv[2 * i], wv[2 * i + 1]), dw[c][i] = db[c][i] = pair(0.f, 0.f);
     }
     __syncthreads();
     int s = 0, flip = 0;
@@ -409,36 +409,39 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         const T* xr = (const T*)a.x + row * a.x_stride;
         const T* gr = (const T*)a.dy + row * a.dy_stride;
         const RingRow qx = ring_row<T, EDGE>(xr, row, a.rows, a.x_stride, n), qg = ring_row<T, EDGE>(gr, row, a.rows, a.dy_stride, n);
-        float xh[NC][VE], g[NC][VE];
-        float s1 = ok, s2 = ok;
+        uint64_t xh[NC][VE / 2], g[NC][VE / 2];
+        uint64_t p1 = pair(ok, ok), p2 = p1;
+        const uint64_t mean2 = pair(-now.x, -now.x), rstd2 = pair(now.y, now.y), ok2 = p1;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int at = k + 32 * c;
+            float xv[VE], gv[VE];
             if (at * VE < n) {
-                unpack16(ring_at<T, EDGE>(place(s), qx, xr, at, n), xh[c], (const T*)nullptr);
-                unpack16(ring_at<T, EDGE>(place(s) + slot, qg, gr, at, n), g[c], (const T*)nullptr);
+                unpack16(ring_at<T, EDGE>(place(s), qx, xr, at, n), xv, (const T*)nullptr);
+                unpack16(ring_at<T, EDGE>(place(s) + slot, qg, gr, at, n), gv, (const T*)nullptr);
                 if (EDGE && (at + 1) * VE > n) {
 #pragma unroll
                     for (int j = 0; j < VE; ++j)
-                        if (at * VE + j >= n) xh[c][j] = g[c][j] = 0.f;
+                        if (at * VE + j >= n) xv[j] = gv[j] = 0.f;
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < VE; ++j) xh[c][j] = g[c][j] = 0.f;
+                for (int j = 0; j < VE; ++j) xv[j] = gv[j] = 0.f;
             }
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                xh[c][j] = (xh[c][j] - now.x) * now.y;       // beyond the row g is 0, so xh there counts for nothing
-                dw[c][j] = fmaf(g[c][j], xh[c][j], dw[c][j]);
-                db[c][j] += g[c][j];
-                g[c][j] *= w[c][j];
-                s1 += g[c][j];
-                s2 = fmaf(g[c][j], xh[c][j], s2);
+            for (int j = 0; j < VE / 2; ++j) {
+                const uint64_t x2 = mul2(add2(pair(xv[2 * j], xv[2 * j + 1]), mean2), rstd2);     // beyond the row g is 0, so it counts for nothing
+                const uint64_t g2 = pair(gv[2 * j], gv[2 * j + 1]), wg = mul2(g2, w[c][j]);
+                dw[c][j] = fma2(g2, x2, dw[c][j]);
+                db[c][j] = add2(db[c][j], g2);
+                p1 = add2(p1, wg);
+                p2 = fma2(wg, x2, p2);
+                xh[c][j] = x2, g[c][j] = wg;
             }
-            dw[c][0] += ok, db[c][0] += ok;
+            dw[c][0] = add2(dw[c][0], ok2), db[c][0] = add2(db[c][0], ok2);
         }
-        s1 = warp_sum(s1);
-        s2 = warp_sum(s2);
+        const float2 h1 = unpair(p1), h2 = unpair(p2);
+        const float s1 = warp_sum(h1.x + h1.y), s2 = warp_sum(h2.x + h2.y);
         float *r1 = red[flip], *r2 = red[flip + 2];
         flip ^= 1;
         if (lane == 0) r1[warp] = s1, r2[warp] = s2;
@@ -447,13 +450,17 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         if (t == 0 && i + stages < n_here) fetch(i + stages, s);
         const float m1 = warp_sum(lane < nwarps ? r1[lane] : 0.f) * inv_n, m2 = warp_sum(lane < nwarps ? r2[lane] : 0.f) * inv_n;
         if (a.dx != nullptr) {
+            const uint64_t m1n = pair(-m1, -m1), m2n = pair(-m2, -m2);
             T* dxr = (T*)a.dx + row * a.dim;
             uint4 out[NC];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 float o[VE];
 #pragma unroll
-                for (int j = 0; j < VE; ++j) o[j] = now.y * (g[c][j] - m1 - xh[c][j] * m2);
+                for (int j = 0; j < VE / 2; ++j) {
+                    const float2 d = unpair(mul2(rstd2, fma2(xh[c][j], m2n, add2(g[c][j], m1n))));
+                    o[2 * j] = d.x, o[2 * j + 1] = d.y;
+                }
                 out[c] = pack16(o, (const T*)nullptr);
                 if (!EDGE && (k + 32 * c) * VE < n) *reinterpret_cast<uint4*>(dxr + (k + 32 * c) * VE) = out[c];
             }
@@ -473,14 +480,25 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         for (int64_t i = max((int64_t)0, n_here - stages); i < n_here; ++i) mbar_drain(&full[i % stages], (uint32_t)(i / stages) & 1, polls);
     }
     if (a.part == nullptr) return;
-    float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+    // through the ring's memory, which no thread reads any more, so that neighbours write side by side: straight from the threads, a
+    // block's sums took as long as four of its rows
+    float* sums = (float*)ring;
+    const int pitch = (n + VE - 1) / VE * VE;
+    __syncthreads();
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int e0 = (k + 32 * c) * VE;
+        if (e0 >= n) continue;
 #pragma unroll
-        for (int j = 0; j < VE; ++j)
-            if (e0 + j < n) out[e0 + j] = dw[c][j], out[a.dim + e0 + j] = db[c][j];
+        for (int j = 0; j < VE; j += 4) {
+            const float2 v0 = unpair(dw[c][j / 2]), v1 = unpair(dw[c][j / 2 + 1]), u0 = unpair(db[c][j / 2]), u1 = unpair(db[c][j / 2 + 1]);
+            *(float4*)(sums + e0 + j) = make_float4(v0.x, v0.y, v1.x, v1.y);
+            *(float4*)(sums + pitch + e0 + j) = make_float4(u0.x, u0.y, u1.x, u1.y);
+        }
     }
+    __syncthreads();
+    float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+    for (int e = t; e < n; e += (int)blockDim.x) out[e] = sums[e], out[a.dim + e] = sums[pitch + e];
 }
 
 // Rows too long for registers: dx alone, one block per row, and x and dy again from L2 for the columns' sums below (512 x 65536 bf16,
@@ -686,7 +704,7 @@ static int ln_bwd_ring(const LnBwdShape& s, const LnBwdArgs& a, cudaStream_t st)
     const size_t slots = (size_t)2 * ring_groups<T>(a.dim, EDGE) * 16;
     const int per_sm = std::max(1, kLnBwdThreadsPerSM / s.threads);
     const int stages = (int)std::max<size_t>(2, std::min<size_t>(kLnRingStages, kLnRingBytes / per_sm / slots));
-    const size_t smem = stages * slots;
+    const size_t smem = stages * slots;      // two stages hold a block's sums: 8 bytes a column
     auto kern = ln_bwd_ring_kernel<T, P, NC, EDGE>;
     CGB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kern<<<s.grid, s.threads, smem, st>>>(a, stages, kDefaultWaitPolls);
