@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(128) ff_few_rows_kernel(FfArgs a) {
     float g[M], u[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) g[m] = u[m] = 0.f;
-    auto multiply = [&](const uint4& rg, const uint4& ru, int k) {
+    auto multiply = [&](const uint4& rg, const uint4& ru, int k, bool inside) {
         float vg[N], vu[N];
         unpack16(rg, vg, (const T*)nullptr);
         unpack16(ru, vu, (const T*)nullptr);
@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(128) ff_few_rows_kernel(FfArgs a) {
         for (int m = 0; m < M; ++m) {
             const T* x = (const T*)a.x + m * a.x_stride;
             float vx[N];
-            unpack16(EDGE ? load_at(x, row_phase(x), k, a.dim) : *reinterpret_cast<const uint4*>(x + k * N), vx, (const T*)nullptr);
+            const uint4 rx = !EDGE ? *reinterpret_cast<const uint4*>(x + k * N) : inside ? load_inside(x, row_phase(x), k) : load_at(x, row_phase(x), k, a.dim);
+            unpack16(rx, vx, (const T*)nullptr);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 g[m] = fmaf(vg[i], vx[i], g[m]);
@@ -72,10 +73,20 @@ __global__ void __launch_bounds__(128) ff_few_rows_kernel(FfArgs a) {
                 ru[c] = __ldcs(reinterpret_cast<const uint4*>(wu) + k + c * 32);
             }
 #pragma unroll
-            for (int c = 0; c < U; ++c) multiply(rg[c], ru[c], k + c * 32);
+            for (int c = 0; c < U; ++c) multiply(rg[c], ru[c], k + c * 32, true);
+        }
+    } else {
+        // behind the first 32 chunks, and with a whole group behind the last of a step, no group leaves the row
+        if (k < chunks) multiply(load_at(wg, pg, k, a.dim), load_at(wu, pu, k, a.dim), k, false);
+        for (k += 32; (k - lane + 2 * 32 + 1) * N <= a.dim; k += 2 * 32) {
+            uint4 rg[2], ru[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) rg[c] = load_inside(wg, pg, k + c * 32), ru[c] = load_inside(wu, pu, k + c * 32);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) multiply(rg[c], ru[c], k + c * 32, true);
         }
     }
-    for (; k < chunks; k += 32) multiply(load_at(wg, pg, k, a.dim), load_at(wu, pu, k, a.dim), k);
+    for (; k < chunks; k += 32) multiply(load_at(wg, pg, k, a.dim), load_at(wu, pu, k, a.dim), k, false);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
         g[m] = warp_sum(g[m]);

@@ -70,11 +70,28 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, flo
             }
         }
     };
+    if (EDGE && !(before && behind)) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int e0 = (k + 32 * c) * N;
-        if (EDGE) raw[c] = load_at(xr, row_phase(xr), k + 32 * c, n, before, behind);
-        else raw[c] = e0 < n ? *reinterpret_cast<const uint4*>(xr + e0) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < CH; ++c) raw[c] = load_at(xr, row_phase(xr), k + 32 * c, n, before, behind);
+    } else if (EDGE) {
+        const int ph = row_phase(xr);
+        uint4 next[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e0 = (k + 32 * c) * N - ph;
+            raw[c] = e0 < n ? *reinterpret_cast<const uint4*>(xr + e0) : make_uint4(0, 0, 0, 0);
+            next[c] = ph != 0 && e0 + N < n ? *reinterpret_cast<const uint4*>(xr + e0 + N) : make_uint4(0, 0, 0, 0);
+        }
+        if (ph != 0) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) raw[c] = shifted(raw[c], next[c], ph * (int)sizeof(T));
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e0 = (k + 32 * c) * N;
+            raw[c] = e0 < n ? *reinterpret_cast<const uint4*>(xr + e0) : make_uint4(0, 0, 0, 0);
+        }
     }
     if (WARP) load_wb();
     float v[CH][N];
@@ -343,8 +360,9 @@ __device__ __forceinline__ RingRow ring_row(const T* r, int64_t row, int64_t row
     return RingRow{ph, ph > 0 && (row == 0 || stride < n) ? 1 : 0, row == rows - 1 || stride < n ? (ph + n) / N : (ph + n + N - 1) / N};
 }
 template <typename T, bool EDGE>
-__device__ __forceinline__ uint4 ring_at(const uint4* slot, const RingRow& q, const T* r, int k, int n) {
+__device__ __forceinline__ uint4 ring_at(const uint4* slot, const RingRow& q, const T* r, int k, int n, bool whole) {
     if (!EDGE) return slot[k];
+    if (whole) return q.ph == 0 ? slot[k] : shifted(slot[k], slot[min(k + 1, q.g1 - 1)], q.ph * (int)sizeof(T));
     const uint4 lo = k >= q.g0 && k < q.g1 ? slot[k] : load_group(r, q.ph, k, n);
     if (q.ph == 0) return lo;
     const int j = k + 1;
@@ -410,6 +428,8 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
         const T* gr = (const T*)a.dy + row * a.dy_stride;
         const RingRow qx = ring_row<T, EDGE>(xr, row, a.rows, a.x_stride, n), qg = ring_row<T, EDGE>(gr, row, a.rows, a.dy_stride, n);
         uint64_t xh[NC][VE / 2], g[NC][VE / 2];
+        // every group of both rows is in the ring
+        const bool whole = EDGE && qx.g0 == 0 && qg.g0 == 0 && qx.g1 * VE >= qx.ph + n && qg.g1 * VE >= qg.ph + n;
         uint64_t p1 = pair(ok, ok), p2 = p1;
         const uint64_t mean2 = pair(-now.x, -now.x), rstd2 = pair(now.y, now.y), ok2 = p1;
 #pragma unroll
@@ -417,8 +437,8 @@ __global__ void __launch_bounds__(kLnBwdMaxThreads) ln_bwd_ring_kernel(LnBwdArgs
             const int at = k + 32 * c;
             float xv[VE], gv[VE];
             if (at * VE < n) {
-                unpack16(ring_at<T, EDGE>(place(s), qx, xr, at, n), xv, (const T*)nullptr);
-                unpack16(ring_at<T, EDGE>(place(s) + slot, qg, gr, at, n), gv, (const T*)nullptr);
+                unpack16(ring_at<T, EDGE>(place(s), qx, xr, at, n, whole), xv, (const T*)nullptr);
+                unpack16(ring_at<T, EDGE>(place(s) + slot, qg, gr, at, n, whole), gv, (const T*)nullptr);
                 if (EDGE && (at + 1) * VE > n) {
 #pragma unroll
                     for (int j = 0; j < VE; ++j)

@@ -151,6 +151,13 @@ __device__ __forceinline__ uint4 load_at(const T* row, int ph, int k, int n, boo
     if (ph == 0) return lo;
     return shifted(lo, load_group(row, ph, k + 1, n, before, behind), ph * (int)sizeof(T));
 }
+// The same where both groups are known to be whole.  Kept apart from the form above: behind a branch that may call load_pieces no
+// load starts before the one in front of it has been shifted.
+template <typename T>
+__device__ __forceinline__ uint4 load_inside(const T* row, int ph, int k) {
+    const uint4* g = reinterpret_cast<const uint4*>(row - ph) + k;
+    return ph == 0 ? g[0] : shifted(g[0], g[1], ph * (int)sizeof(T));
+}
 // Writes the groups of a row of n values that end in this warp's chunks k0 + lane, k0 + 32 + lane, ... (CH of them, in `u`), `ph` as
 // above.  `before` is the last chunk before this warp's (any value where there is none).  The values of the warp's last
 // chunk that lie in the group behind it are the next warp's, except at the end of the row.
@@ -158,7 +165,8 @@ template <typename T, int CH>
 __device__ __forceinline__ void store_groups(T* row, int ph, int k0, int n, const uint4 (&u)[CH], const uint4& before) {
     constexpr int N = Chunk<T>::N;
     const int lane = threadIdx.x & 31;
-    uint4 old = before;
+    uint4 old = before, first = before, last = before;
+    int last_e0 = n;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e0 = (k0 + 32 * c + lane) * N - ph;      // first value of the group
@@ -173,8 +181,13 @@ __device__ __forceinline__ void store_groups(T* row, int ph, int k0, int n, cons
             old = u[c];
         }
         if (e0 >= 0 && e0 + N <= n) *reinterpret_cast<uint4*>(row + e0) = out;
-        else if (e0 < n && e0 + N > 0) store_pieces(row, e0, n, out);
+        else if (e0 >= 0 && e0 < n) last = out, last_e0 = e0;
+        if (c == 0) first = out;
     }
+    // the groups at the row's ends, behind the loop: a call in it would keep its steps apart
+    const int first_e0 = (k0 + lane) * N - ph;
+    if (first_e0 < 0 && first_e0 + N > 0) store_pieces(row, first_e0, n, first);
+    if (last_e0 < n) store_pieces(row, last_e0, n, last);
 }
 
 // N parameter values (of any of the three types) from value e0 on, as they lie in memory (zeros outside [0, n)), and as float32.
