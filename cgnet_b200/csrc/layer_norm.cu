@@ -42,7 +42,7 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
 // the row needs is on its way before the first value is waited for.  EDGE: rows (or weight and bias) that do not start on 16-byte
 // boundaries or do not end on them; without it every chunk is inside the row or behind it.
 // Bound by the one read and the one write: 8192 x 4096 bf16 (134 MB) 29 us alone on the GPU = 4.6 TB/s, 33 with the copies in L2
-// cold; 3001 x 1023 fp16, rows starting anywhere, 9.4 us (shifting the groups costs three times the instructions of aligned rows).
+// cold; 3001 x 1023 fp16, rows starting anywhere, 6.7 us against 3.6 at 1024 columns, from L2 (shifting the groups doubles the instructions).
 template <typename T, typename P, int CH, bool WARP, bool EDGE>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, float inv_n, T* __restrict__ y, float2* __restrict__ stats) {
     constexpr int N = Chunk<T>::N;
@@ -57,11 +57,21 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, flo
     const bool before = EDGE && row > 0 && a.x_stride >= n && n >= N, behind = EDGE && row + 1 < a.rows && a.x_stride >= n && n >= N;
     uint4 raw[CH];
     Params<P, N> w[CH], b[CH];
+    const bool whole = EDGE && aligned16(a.w) && aligned16(a.b);
+    const int end = n / N * N;           // where a chunk begins that the row does not fill
+    P w_end = from_f32<P>(0.f), b_end = w_end;
     auto load_wb = [&]() {
+        if (whole && lane < n - end) {
+            if (a.w != nullptr) w_end = ((const P*)a.w)[end + lane];
+            if (a.b != nullptr) b_end = ((const P*)a.b)[end + lane];
+        }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int e0 = (k + 32 * c) * N;
-            if (EDGE) {
+            if (whole) {
+                if (a.w != nullptr) w[c].load_whole((const P*)a.w, e0, n);
+                if (a.b != nullptr) b[c].load_whole((const P*)a.b, e0, n);
+            } else if (EDGE) {
                 if (a.w != nullptr) w[c].load((const P*)a.w, e0, n);
                 if (a.b != nullptr) b[c].load((const P*)a.b, e0, n);
             } else if (e0 < n) {
@@ -94,55 +104,70 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, flo
         }
     }
     if (WARP) load_wb();
-    float v[CH][N];
-    float s = 0.f;
+    uint64_t v[CH][N / 2];              // pairs of columns
+    // what lies behind the row's end counts for nothing; only a warp that reaches it has to look
+    auto cut = [&](int c) {
+        if ((k0 + 32 * c + 32) * N <= n) return;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const int e = (k + 32 * c) * N + (EDGE ? i : 0);
+            const float2 d = unpair(v[c][i / 2]);
+            v[c][i / 2] = pair(e < n ? d.x : 0.f, (EDGE ? e + 1 : e) < n ? d.y : 0.f);
+        }
+    };
+    uint64_t s2 = pair(0.f, 0.f), q2 = s2;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        unpack16(raw[c], v[c], (const T*)nullptr);
-        if (EDGE && (k + 32 * c) * N + N > n) {      // the row's end: what is the neighbour's goes
+        float t[N];
+        unpack16(raw[c], t, (const T*)nullptr);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if ((k + 32 * c) * N + i >= n) v[c][i] = 0.f;
-        }
+        for (int i = 0; i < N; i += 2) v[c][i / 2] = pair(t[i], t[i + 1]);
+        if (EDGE) cut(c);               // values of the next row
 #pragma unroll
-        for (int i = 0; i < N; ++i) s += v[c][i];
+        for (int i = 0; i < N / 2; ++i) s2 = add2(s2, v[c][i]);
     }
-    const float mean = row_sum<WARP>(s, red[0]) * inv_n;
-    float q = 0.f;
+    const float2 s = unpair(s2);
+    const float mean = row_sum<WARP>(s.x + s.y, red[0]) * inv_n;
+    const uint64_t mean2 = pair(-mean, -mean);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e0 = (k + 32 * c) * N;
-        if (EDGE ? e0 + N > n : e0 >= n) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[c][i] = EDGE && e0 + i < n ? v[c][i] : mean;     // counts for nothing
-        }
+        for (int i = 0; i < N / 2; ++i) v[c][i] = add2(v[c][i], mean2);
+        cut(c);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[c][i] -= mean;
-            q = fmaf(v[c][i], v[c][i], q);
-        }
+        for (int i = 0; i < N / 2; ++i) q2 = fma2(v[c][i], v[c][i], q2);
     }
-    const float rstd = 1.f / sqrtf(row_sum<WARP>(q, red[1]) * inv_n + a.eps);
+    const float2 q = unpair(q2);
+    const float rstd = 1.f / sqrtf(row_sum<WARP>(q.x + q.y, red[1]) * inv_n + a.eps);
+    const uint64_t rstd2 = pair(rstd, rstd);
     if (stats != nullptr && (WARP ? lane : (int)threadIdx.x) == 0) stats[row] = make_float2(mean, rstd);
     if (!WARP) load_wb();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e0 = (k + 32 * c) * N;
-        float wv[N], bv[N];
+        float t[N];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) v[c][i] = mul2(v[c][i], rstd2);
+        if (whole && end != n && end >= e0 - lane * N && end < e0 + (32 - lane) * N) {       // the same in the whole warp
+            w[c].place_end(w_end, e0, n);
+            b[c].place_end(b_end, e0, n);
+        }
         if (a.w != nullptr) {
-            w[c].get(wv);
+            w[c].get(t);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[c][i] *= rstd * wv[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[c][i] *= rstd;
+            for (int i = 0; i < N; i += 2) v[c][i / 2] = mul2(v[c][i / 2], pair(t[i], t[i + 1]));
         }
         if (a.b != nullptr) {
-            b[c].get(bv);
+            b[c].get(t);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[c][i] += bv[i];
+            for (int i = 0; i < N; i += 2) v[c][i / 2] = add2(v[c][i / 2], pair(t[i], t[i + 1]));
         }
-        raw[c] = pack16(v[c], (const T*)nullptr);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 d = unpair(v[c][i / 2]);
+            t[i] = d.x, t[i + 1] = d.y;
+        }
+        raw[c] = pack16(t, (const T*)nullptr);
         if (!EDGE && e0 < n) *reinterpret_cast<uint4*>(yr + e0) = raw[c];
     }
     if (EDGE) {

@@ -130,7 +130,7 @@ __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int b
 #pragma unroll
     for (int j = 0; j < 5; ++j) x[j] = bytes & 4 ? x[j + 1] : x[j];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = bytes & 2 ? __funnelshift_r(x[j], x[j + 1], 16) : x[j];
+    for (int j = 0; j < 4; ++j) x[j] = __funnelshift_r(x[j], x[j + 1], (bytes & 2) * 8);
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
 // Group g of a row of n values whose aligned groups start `ph` values before it; zeros outside the row.  `before`, `behind`: the
@@ -206,6 +206,26 @@ struct Params {
         } else {
 #pragma unroll
             for (int c = 0; c < W; ++c) u[c] = load_pieces(w, e0 + c * Chunk<P>::N, n, 0.f);
+        }
+    }
+    // In two steps, so that no call and no wait stands between a thread's loads (w aligned; e0 multiples of N that grow by N from lane to
+    // lane): what is whole is fetched at once, and the chunk that the end falls into is put together later from its values, which
+    // the lanes have fetched one each (`mine`: value n / N * N + lane).
+    __device__ __forceinline__ void load_whole(const P* w, int e0, int n) {
+#pragma unroll
+        for (int c = 0; c < W; ++c) u[c] = e0 + N <= n ? *(reinterpret_cast<const uint4*>(w + e0) + c) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void place_end(P mine, int e0, int n) {
+        float t[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = __shfl_sync(0xffffffffu, to_f32(mine), i);
+        if (e0 != n / N * N) return;
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+            float part[Chunk<P>::N];
+#pragma unroll
+            for (int i = 0; i < Chunk<P>::N; ++i) part[i] = t[c * Chunk<P>::N + i];
+            u[c] = pack16(part, (const P*)nullptr);      // of this type already: nothing is rounded
         }
     }
     __device__ __forceinline__ void get(float (&v)[N]) const {
