@@ -38,11 +38,13 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
     return WARP ? warp_sum(v) : block_sum(v, buf);
 }
 
-// One row per warp (WARP) or per block; its values stay in registers between the three steps, so x is read once, and everything
-// the row needs is on its way before the first value is waited for.  EDGE: rows (or weight and bias) that do not start on 16-byte
-// boundaries or do not end on them; without it every chunk is inside the row or behind it.
-// Bound by the one read and the one write: 8192 x 4096 bf16 (134 MB) 29 us alone on the GPU = 4.6 TB/s, 33 with the copies in L2
-// cold; 3001 x 1023 fp16, rows starting anywhere, 6.7 us against 3.6 at 1024 columns, from L2 (shifting the groups doubles the instructions).
+// One row per warp (WARP) or per block; its values stay in registers between the three steps, so x is read once.  A warp has weight
+// and bias on their way before the first value is waited for; a block fetches them chunk by chunk at the end (with all of them in
+// registers 8192 x 4096 bf16 took 27 instead of 25 us, and 81 instead of 33 with float32 weights, which spilled).  EDGE: rows (or
+// weight and bias) that do not start on 16-byte boundaries or do not end on them; without it every chunk is inside the row or
+// behind it.
+// Bound by the one read and the one write: 8192 x 4096 bf16 (134 MB) 25 us in a row of calls = 5.3 TB/s.  Rows that start anywhere
+// take twice the instructions, for shifting the groups: 3001 x 1023 fp16 6.7 us against 3.6 at 1024 columns.
 template <typename T, typename P, int CH, bool WARP, bool EDGE>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, float inv_n, T* __restrict__ y, float2* __restrict__ stats) {
     constexpr int N = Chunk<T>::N;
@@ -60,13 +62,13 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, flo
     const bool whole = EDGE && aligned16(a.w) && aligned16(a.b);
     const int end = n / N * N;           // where a chunk begins that the row does not fill
     P w_end = from_f32<P>(0.f), b_end = w_end;
-    auto load_wb = [&]() {
-        if (whole && lane < n - end) {
+    auto load_wb = [&](int from, int to) {
+        if (from == 0 && whole && lane < n - end) {
             if (a.w != nullptr) w_end = ((const P*)a.w)[end + lane];
             if (a.b != nullptr) b_end = ((const P*)a.b)[end + lane];
         }
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
+        for (int c = from; c < to; ++c) {
             const int e0 = (k + 32 * c) * N;
             if (whole) {
                 if (a.w != nullptr) w[c].load_whole((const P*)a.w, e0, n);
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, flo
             raw[c] = e0 < n ? *reinterpret_cast<const uint4*>(xr + e0) : make_uint4(0, 0, 0, 0);
         }
     }
-    if (WARP) load_wb();
+    if (WARP) load_wb(0, CH);
     uint64_t v[CH][N / 2];              // pairs of columns
     // what lies behind the row's end counts for nothing; only a warp that reaches it has to look
     auto cut = [&](int c) {
@@ -141,11 +143,11 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) ln_fwd_kernel(LnArgs a, flo
     const float rstd = 1.f / sqrtf(row_sum<WARP>(q.x + q.y, red[1]) * inv_n + a.eps);
     const uint64_t rstd2 = pair(rstd, rstd);
     if (stats != nullptr && (WARP ? lane : (int)threadIdx.x) == 0) stats[row] = make_float2(mean, rstd);
-    if (!WARP) load_wb();
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int e0 = (k + 32 * c) * N;
         float t[N];
+        if (!WARP) load_wb(c, c + 1);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) v[c][i] = mul2(v[c][i], rstd2);
         if (whole && end != n && end >= e0 - lane * N && end < e0 + (32 - lane) * N) {       // the same in the whole warp
