@@ -603,7 +603,7 @@ __global__ void ln_bwd_cols_kernel(LnBwdArgs a, int64_t rows_per_part) {
 }
 
 // Partial sums [parts][2][dim] -> dw, db: 32 columns per block, thread row y adds parts y, y + 32, ... and the sums of the thread
-// rows are added by a tree.  148 parts of 4096 columns: 6.5 us.
+// rows are added by a tree.  296 parts of 4096 columns: 6.8 us.
 template <typename P>
 __global__ void __launch_bounds__(1024) ln_param_reduce_kernel(const float* __restrict__ part, int parts, int64_t dim, P* __restrict__ dw,
                                                                P* __restrict__ db) {
