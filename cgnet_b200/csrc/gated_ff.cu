@@ -402,6 +402,23 @@ __global__ void __launch_bounds__(256) ff_reduce_kernel(FfReduceArgs a) {
     }
 }
 
+// The forward with a split contraction: the parts of g and u, added in order, and what is made of them.
+template <typename T>
+__global__ void __launch_bounds__(256) ff_join_kernel(FfArgs a, const float* g_part, const float* u_part, int splits) {
+    const int64_t n = a.rows * a.hidden;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float g = g_part[i], u = u_part[i];
+#pragma unroll 4
+        for (int k = 1; k < splits; ++k) g += g_part[k * n + i], u += u_part[k * n + i];
+        ((T*)a.h)[i] = from_f32<T>(activate<false>(a.act, g).x * u);
+        if (a.gu != nullptr) {
+            const int64_t m = i / a.hidden, j = i - m * a.hidden;
+            a.gu[m * a.gu_pitch + j] = g;
+            a.gu[(a.rows + m) * a.gu_pitch + j] = u;
+        }
+    }
+}
+
 // ---- which path, and what it needs -------------------------------------------------------------------------------------
 // The tensor cores are used from this length of the longest contraction on (forward: dim; backward: rows or 2 hidden), or from this
 // much work (rows x dim x hidden).  CUDA cores / tensor cores, us, launches of a graph: 16 bits, forward 16 x 64 -> 64 5.0 / 6.3,
@@ -414,9 +431,14 @@ struct FfLimits {
 static FfLimits ff_limits(int dtype) { return dtype == CGB200_F32 ? FfLimits{768, 640, 16 << 20} : FfLimits{128, 160, 8 << 20}; }
 
 constexpr int kFfOutputStages = 8;
+// A forward whose tiles keep at most half of the SMs busy is split along dim from this many stages on.  Whole / split, us, launches of a
+// graph: bf16 16 x 1024 -> 1000 9.1 / 8.0, 16 x 4096 -> 1000 19.3 / 9.7, 500 x 2048 -> 1000 13.3 / 13.1, 156 x 3330 -> 342 30.8 / 15.7;
+// float32 300 x 640 -> 500 20.1 / 16.6, 156 x 3330 -> 342 78.7 / 22.6.
+static int ff_split_stages(int dtype) { return dtype == CGB200_F32 ? 8 : 16; }
 
 struct FfPlan {
     bool tensor;
+    bool joined;                          // the forward's contraction is split: g and u are products of their own, joined afterwards
     int planes, bn;
     bool pack[3];                         // x, Wg, Wu
     int64_t pitch_d, pitch_h;             // of packed operands (dim columns) and of dg, du (hidden columns)
@@ -465,7 +487,16 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     };
     // wide tiles move less through shared memory; narrow ones fill the SMs where the wide ones do not
     q.bn = q.planes == 3 || units_at(256) < kNumSM ? 128 : 256;
-    if (fwd) {
+    q.joined = fwd && 2 * units_at(128) <= kNumSM && dk >= ff_split_stages(dtype);
+    if (q.joined) {
+        for (int i = 0; i < 2; ++i) {
+            FfProblem& p = q.problem[q.n_problems++];
+            p.a_map[0] = 0, p.b_map[0] = 1 + i;
+            p.sources = 1, p.kblk = dk, p.sets = 1;
+            p.tiles_i = (int)ti, p.tiles_j = (a.hidden + q.bn - 1) / q.bn;
+            p.n_i = a.rows, p.n_j = a.hidden;
+        }
+    } else if (fwd) {
         FfProblem& p = q.problem[q.n_problems++];
         p.a_map[0] = 0, p.b_map[0] = 1, p.b_map[1] = 2;
         p.sources = 1, p.kblk = dk, p.sets = 1;
@@ -499,7 +530,9 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     for (int i = 0; i < q.n_problems; ++i) {
         FfProblem& p = q.problem[i];
         const int stages = p.sources * p.kblk, length = stages + kFfOutputStages;
-        int splits = fwd || length <= 1.5 * share ? 1 : (int)std::min(8.0, length / std::max(0.5 * share, 2.0 * kFfOutputStages) + 0.999);
+        int splits = q.joined                          ? (int)std::max<int64_t>(2, kNumSM / (2 * ti * p.tiles_j))
+                     : fwd || length <= 1.5 * share ? 1
+                                                    : (int)std::min(8.0, length / std::max(0.5 * share, 2.0 * kFfOutputStages) + 0.999);
         splits = std::max(1, std::min(splits, stages / 4));
         p.kper = (stages + splits - 1) / splits;
         p.splits = (stages + p.kper - 1) / p.kper;
@@ -629,6 +662,7 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
     for (int i = 0; i < q.n_problems; ++i) {
         FfProblem& p = g.p[i];
         p.out_map[0] = p.out_map[1] = -1;
+        if (q.joined) continue;               // parts only
         if (fwd) {
             p.out[0] = a.h;
             p.h_aligned = at16(a.h) && a.hidden % Chunk<T>::N == 0;
@@ -651,11 +685,20 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
     }
     g.idesc_type = half ? 0u : (1u << 7) | (1u << 10);
     g.act = a.act, g.polls = kDefaultWaitPolls;
+    const bool fused = fwd && !q.joined;
     int rc;
-    if constexpr (PLANES == 3) rc = fwd ? ff_gemm_launch<3, 128, T, true>(g, kid, st) : ff_gemm_launch<3, 128, T, false>(g, kid, st);
-    else if (q.bn == 256) rc = fwd ? ff_gemm_launch<1, 256, T, true>(g, kid, st) : ff_gemm_launch<1, 256, T, false>(g, kid, st);
-    else rc = fwd ? ff_gemm_launch<1, 128, T, true>(g, kid, st) : ff_gemm_launch<1, 128, T, false>(g, kid, st);
+    if constexpr (PLANES == 3) rc = fused ? ff_gemm_launch<3, 128, T, true>(g, kid, st) : ff_gemm_launch<3, 128, T, false>(g, kid, st);
+    else if (q.bn == 256) rc = fused ? ff_gemm_launch<1, 256, T, true>(g, kid, st) : ff_gemm_launch<1, 256, T, false>(g, kid, st);
+    else rc = fused ? ff_gemm_launch<1, 128, T, true>(g, kid, st) : ff_gemm_launch<1, 128, T, false>(g, kid, st);
     if (rc != CGB200_OK) return rc;
+    if (q.joined) {
+        const int64_t n = a.rows * a.hidden;
+        launch_begin(kid, st);
+        ff_join_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, kNumSM * 16), 256, 0, st>>>(a, g.p[0].part, g.p[1].part, g.p[0].splits);
+        launch_end(kid, st);
+        CGB_CUDA(cudaGetLastError());
+        return CGB200_OK;
+    }
     FfReduceArgs r{};
     bool any = false;
     int64_t n = 0;
