@@ -422,13 +422,13 @@ __global__ void __launch_bounds__(256) ff_join_kernel(FfArgs a, const float* g_p
 // ---- which path, and what it needs -------------------------------------------------------------------------------------
 // The tensor cores are used from this length of the longest contraction on (forward: dim; backward: rows or 2 hidden), or from this
 // much work (rows x dim x hidden).  CUDA cores / tensor cores, us, launches of a graph: 16 bits, forward 16 x 64 -> 64 5.0 / 6.3,
-// 16 x 128 -> 256 6.8 / 6.4, 10 x 976 -> 104 36 / 9.6; backward 7.0 / 7.2, 19 / 8.7, 11 / 7.8.  float32 (three planes, a copy in
-// front), forward 100 x 256 -> 256 9.5 / 13, 32 x 1024 -> 128 27 / 25; backward 16 / 19, 1000 x 48 -> 48 28 / 21.
+// 16 x 128 -> 256 6.8 / 6.4, 10 x 976 -> 104 36 / 8.0; backward 7.0 / 7.2, 19 / 8.7, 11 / 7.8.  float32 (three planes, a copy in
+// front), forward 100 x 256 -> 256 8.9 / 12.5, 100 x 512 -> 256 15.1 / 14.4, 32 x 640 -> 128 17.5 / 15.2; backward 16 / 19, 1000 x 48 -> 48 28 / 21.
 struct FfLimits {
     int forward, backward;
     int64_t work;
 };
-static FfLimits ff_limits(int dtype) { return dtype == CGB200_F32 ? FfLimits{768, 640, 16 << 20} : FfLimits{128, 160, 8 << 20}; }
+static FfLimits ff_limits(int dtype) { return dtype == CGB200_F32 ? FfLimits{512, 640, 16 << 20} : FfLimits{128, 160, 8 << 20}; }
 
 constexpr int kFfOutputStages = 8;
 // A forward whose tiles keep at most half of the SMs busy is split along dim from this many stages on.  Whole / split, us, launches of a
