@@ -118,6 +118,17 @@ def test_layer_norm_without_parameters_and_with_float32_ones(dtype, weight, bias
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [1023, 2049, 4097, 8200, 16381])
+def test_layer_norm_long_rows_with_float32_weights(dim, dtype):
+    """Rows of a warp and of a block that end inside a group, and weights that start on and off 16-byte boundaries."""
+    g = gen(dim)
+    for lo in (0, 1, 3):
+        w, b = (1 + 0.2 * randn(g, dim + lo))[lo:], randn(g, dim + lo)[lo:]
+        check_norm((randn(g, 7, dim) + randn(g, 7, 1)).to(dtype), w, b, 1e-5, randn(g, 7, dim).to(dtype))
+        check_norm((randn(g, 7, dim + 2) + randn(g, 7, 1)).to(dtype)[:, 1:dim + 1], w.to(dtype), b.to(dtype), 1e-5, randn(g, 7, dim).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_layer_norm_layouts(dtype):
     """Rows inside wider rows, rows that start anywhere, transposed and broadcast inputs, more than two dimensions."""
     g = gen(5)
@@ -234,6 +245,15 @@ def test_gated_feed_forward_activations_and_layouts(act, dtype):
                  randn(g, rows, 260).to(dtype)[:, 3:203])
     check_ff(randn(g, 1, 64).to(dtype).expand(9, 64), (randn(g, 80, 64) / 8).to(dtype), (randn(g, 80, 64) / 8).to(dtype), act,
              randn(g, 1, 80).to(dtype).expand(9, 80))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, dim, hidden", [(5, 1031, 70), (156, 1330, 342), (129, 1024, 257), (16, 520, 1000), (500, 2048, 128)])
+def test_gated_feed_forward_of_few_tiles(rows, dim, hidden, dtype):
+    """A forward whose contraction is split over blocks, with and without the projections kept for a backward."""
+    g = gen(rows + dim + hidden)
+    check_ff(randn(g, rows, dim).to(dtype), (randn(g, hidden, dim) * dim ** -0.5).to(dtype), (randn(g, hidden, dim) * dim ** -0.5).to(dtype),
+             ("silu", "gelu", "relu")[rows % 3], randn(g, rows, hidden).to(dtype))
 
 
 def test_gated_feed_forward_parts_and_shapes():
