@@ -465,7 +465,10 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                 }
                 if (++acc == 2) acc = 0, acc_ph ^= 1;
             } else {
-                constexpr int kSums = JW / (FWD ? 32 : 64);       // 32 columns each; a forward's: g's, then u's
+                // 32 columns each of this warp's half of the tile; a forward's: g's, then u's
+                constexpr int kSums = JW / 64;
+                static_assert(kSums * 64 == JW && kAccCols + JW / 2 + (FWD ? BN / 2 : 0) + 32 * kSums + BN <= kTmemCols,
+                              "the last column read (second accumulator, right half, small products) must be one of the block's");
                 float sum[FWD ? 2 * kSums : kSums][32];
 #pragma unroll
                 for (int c = 0; c < (FWD ? 2 * kSums : kSums); ++c)
