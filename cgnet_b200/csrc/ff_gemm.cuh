@@ -367,6 +367,11 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             const bool rows_here = row0 < p.n_i;
             // a block of columns of this warp's half: 32 of a plain product, 16 of g and as many of u
             constexpr int kCols = FWD ? 16 : 32, kBlocks = JW / 2 / kCols;
+            // The copies that this warp has started still read the staging area until they are waited for, and a block goes from units that
+            // leave by copies to units that threads write: those wait too (write_block's barrier holds the other lanes back).
+            auto staging_free = [&] {
+                if (lane == 0) tma_store_wait<0>();
+            };
             auto emit = [&](int c, const float* v, const float* w) {
                 const int col0 = t.j0 + side * (JW / 2) + c * kCols;
                 if (!rows_here || col0 >= p.n_j) return;
@@ -377,7 +382,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                     for (int i = 0; i < 16; ++i) g[i] = v[i], u[i] = w[i];
                     const bool keep = p.out_map[0] >= 0;
                     if (keep) {
-                        if (lane == 0) tma_store_wait<0>();
+                        staging_free();
                         __syncwarp();
                         uint4 q[4];
                         pack_row(g, q, (const float*)nullptr);
@@ -403,12 +408,13 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                             }
                         }
                     } else {
-                        if (keep && lane == 0) tma_store_wait<0>();
+                        staging_free();
                         write_block<16>(g, st, (T*)p.out[0], row0, p.n_i, p.n_j, col0, p.n_j);
                         fence_proxy_async();
                     }
                 } else if (p.splits > 1) {
                     float* part = p.part + ((int64_t)t.split * p.sets + t.set) * p.n_i * p.n_j;
+                    staging_free();
                     write_block<32>(v, st, part, row0, p.n_i, p.n_j, col0, p.n_j);
                 } else if (p.out_map[t.set] >= 0) {
                     const CUtensorMap* map = &a.map[p.out_map[t.set]];
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                         if (lane == 0) tma_store(map, bytes + flip, col0, (int)row0, 0);
                         flip ^= 2048;
                     } else {
-                        if (lane == 0) tma_store_wait<0>();
+                        staging_free();
                         __syncwarp();
                         pack_row(v, q, (const float*)nullptr);
                         put_row(bytes, q);
@@ -437,6 +443,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                         }
                     }
                 } else if (p.out[t.set] != nullptr) {
+                    staging_free();
                     write_block<32>(v, st, (T*)p.out[t.set], row0, p.n_i, p.n_j, col0, p.n_j);
                 }
             };

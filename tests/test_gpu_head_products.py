@@ -23,3 +23,43 @@ def test_float32_forward_of_several_tiles_a_block(rows, dim, hidden):
     with torch.no_grad():
         h = cg.gated_feed_forward(x, wg, wu)
         assert all(torch.equal(cg.gated_feed_forward(x, wg, wu), h) for _ in range(5))
+
+
+# (rows, dim, hidden): one of dx and [dWg; dWu] leaves by bulk copies, the other in parts written by threads, and some blocks have a
+# unit of the former directly before one of the latter.  dx first: the first four; dW first: the others.
+MIXED = [(1652, 880, 288), (4096, 512, 512), (1904, 856, 259), (6180, 296, 775), (1052, 144, 3415), (2901, 360, 4644)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows, dim, hidden", MIXED)
+def test_backward_units_that_leave_in_different_ways(rows, dim, hidden, dtype):
+    import cgnet_b200 as cg
+    x, wg, wu, dh = operands(rows, dim, hidden, dtype)
+    check_ff(x, wg, wu, "gelu", dh)
+    h = cg.gated_feed_forward(x, wg, wu, activation="gelu")
+    grads = torch.autograd.grad(h, (x, wg, wu), dh, retain_graph=True)
+    for _ in range(10):
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(h, (x, wg, wu), dh, retain_graph=True), grads))
+
+
+def test_weight_gradients_of_different_alignment():
+    """The C interface takes outputs of any alignment: one gradient leaves by copies, the other is written by threads, one stage apart."""
+    from cgnet_b200 import _lib
+    lib, rows, dim, hidden = _lib.load(), 64, 1024, 4096
+    x, wg, wu, dh = operands(rows, dim, hidden, torch.bfloat16)
+    gate_up = torch.empty(2, rows, hidden, device=x.device)
+    h, ws = torch.empty_like(dh), torch.empty(1 << 24, dtype=torch.uint8, device=x.device)
+    stream = torch.cuda.current_stream().cuda_stream
+    operand_args = (x.data_ptr(), dim, wg.data_ptr(), dim, wu.data_ptr(), dim)
+    assert lib.cgb200_gated_ff_fwd(*operand_args, 0, h.data_ptr(), gate_up.data_ptr(), rows, dim, hidden, _lib.BF16, ws.data_ptr(), ws.numel(), stream) == 0
+
+    def gradients(offset):
+        gate, upper = (torch.zeros(hidden * dim + 8, dtype=torch.bfloat16, device=x.device) for _ in range(2))
+        out = upper[offset:offset + hidden * dim]
+        assert lib.cgb200_gated_ff_bwd(*operand_args, 0, gate_up.data_ptr(), dh.data_ptr(), hidden, None, gate.data_ptr(), out.data_ptr(), rows, dim,
+                                       hidden, _lib.BF16, ws.data_ptr(), ws.numel(), stream) == 0, lib.cgb200_last_error()
+        assert not upper[:offset].any() and not upper[offset + hidden * dim:].any()
+        return gate, out
+    want = gradients(0)
+    for _ in range(10):
+        assert all(torch.equal(p, q) for p, q in zip(gradients(1), want))
