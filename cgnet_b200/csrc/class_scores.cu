@@ -818,8 +818,10 @@ __global__ void __launch_bounds__(kScThreads, 5) scores_grad_kernel(ScoreGradArg
     float* wts = (float*)(ids + K);
     int* start = (int*)(wts + K);
     const float4 st = on ? ((const float4*)a.f.stats)[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool dead = st.y == 0.f || st.w == 0.f;       // no row, no distribution, or no teacher
-    const float g = dead ? 0.f : a.g_loss[row] * a.f.temperature, gp = g * st.y;
+    // a class beyond the last, or a NaN among the teacher's scores, left its sum NaN: then so is the whole row's gradient, as its loss
+    const bool unknown = st.w != st.w;
+    const bool dead = !unknown && (st.y == 0.f || st.w == 0.f);       // no row, no distribution, or no teacher
+    const float g = dead ? 0.f : a.g_loss[row] * a.f.temperature, gp = unknown ? __uint_as_float(0x7fffffffu) : g * st.y;
     if (!dead)
         for (int k = t; k < K; k += G) {
             const int64_t id = a.f.t_ids[row * K + k];

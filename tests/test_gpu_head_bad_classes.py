@@ -1,0 +1,36 @@
+"""Classes beyond the last and NaN scores: which gradients they spoil, and which they leave alone."""
+import pytest
+import torch
+
+from test_gpu_head import TYPES, check_distill, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [20, 700, 3000, 70000])
+def test_distillation_gradient_of_a_row_that_is_nan(classes, dtype):
+    """The row's loss and its whole gradient are NaN, every other row is what it is without the bad entry."""
+    import cgnet_b200 as cg
+    g = gen(classes)
+    z = (2 * randn(g, 6, classes)).to(dtype)
+    ids = torch.randint(0, classes, (6, 5), generator=g, device=z.device)
+    scores = randn(g, 6, 5)
+    g_loss = randn(g, 6)
+    bad_ids, bad_scores = ids.clone(), scores.clone()
+    bad_ids[1, 3] = classes                     # one of five
+    bad_ids[2] = torch.tensor([1 << 40, -1, -1, -1, -1], device=z.device)        # the only one
+    bad_scores[4, 2] = float("nan")
+    leaf = z.clone().requires_grad_()
+    want_loss = cg.distillation_loss(leaf, ids, scores, 2.0)
+    (want,) = torch.autograd.grad(want_loss, leaf, g_loss)
+    loss = cg.distillation_loss(leaf, bad_ids, bad_scores, 2.0)
+    (dz,) = torch.autograd.grad(loss, leaf, g_loss)
+    good = [0, 3, 5]
+    assert torch.isnan(loss[[1, 2, 4]]).all() and torch.isnan(dz[[1, 2, 4]]).all()
+    assert torch.equal(loss[good], want_loss[good]) and torch.equal(dz[good], want[good])
+    for row in (1, 2, 4):                       # a row by itself: several blocks share it
+        leaf = z[row:row + 1].clone().requires_grad_()
+        (dz,) = torch.autograd.grad(cg.distillation_loss(leaf, bad_ids[row:row + 1], bad_scores[row:row + 1].to(dtype), 2.0), leaf, g_loss[:1])
+        assert torch.isnan(dz).all()
+    check_distill(z[good], ids[good], scores[good], 2.0, g_loss[good])
