@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(kScThreads, 5) scores_grad_kernel(ScoreGradArg
         const int64_t tgt = a.f.targets != nullptr ? a.f.targets[row] : -1;
         const bool dead = st.y == 0.f;                                          // a row without a distribution
         float g_lp = a.g_lp != nullptr && tgt >= 0 && !dead ? a.g_lp[row] : 0.f;
-        if (tgt >= V) g_lp = __uint_as_float(0x7fffffffu);
+        if (tgt >= V && a.g_lp != nullptr) g_lp = __uint_as_float(0x7fffffffu);      // the entropy's gradient does not know the target
         const float g_ent = a.g_ent != nullptr && !dead ? a.g_ent[row] : 0.f;
         // -p (g_lp + g_H (ln 2 a + log(1 / s) + H)),  p = 2^a / s
         const float base = g_ent == 0.f ? g_lp : g_lp + g_ent * (logf(st.y) + a.f.entropy[row]), slope = g_ent * (float)kLn2;

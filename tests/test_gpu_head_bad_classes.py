@@ -34,3 +34,20 @@ def test_distillation_gradient_of_a_row_that_is_nan(classes, dtype):
         (dz,) = torch.autograd.grad(cg.distillation_loss(leaf, bad_ids[row:row + 1], bad_scores[row:row + 1].to(dtype), 2.0), leaf, g_loss[:1])
         assert torch.isnan(dz).all()
     check_distill(z[good], ids[good], scores[good], 2.0, g_loss[good])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [20, 3000])
+def test_entropy_gradient_of_a_row_whose_target_is_beyond_the_last_class(classes, dtype):
+    """The log probability is NaN and so is a gradient through it; the entropy does not depend on the target."""
+    import cgnet_b200 as cg
+    g = gen(classes)
+    z = (2 * randn(g, 4, classes)).to(dtype).requires_grad_()
+    target = torch.tensor([1, classes, 1 << 40, -1], device=z.device)
+    g_ent = randn(g, 4)
+    out = cg.log_probs(z, target)
+    (want,) = torch.autograd.grad(cg.log_probs(z).entropy, z, g_ent)
+    (dz,) = torch.autograd.grad(out.entropy, z, g_ent, retain_graph=True)
+    assert torch.isfinite(want).all() and torch.equal(dz, want)
+    (dz,) = torch.autograd.grad(out.log_prob, z, g_ent)
+    assert torch.isnan(dz[1:3]).all() and torch.isfinite(dz[[0, 3]]).all()
