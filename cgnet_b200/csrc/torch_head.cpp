@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -391,19 +392,14 @@ Tensor distillation_loss(PyObject* const* a) {
 }
 
 // ---- module --------------------------------------------------------------------------------------------------------------------
+// Errors keep their type: one that Python code raised below this call (saved-tensor hooks, such as the one by which activation
+// checkpointing ends its recomputation) goes on as it is, and an allocation that failed is torch.OutOfMemoryError.
 template <typename F>
 PyObject* guarded(const char* name, Py_ssize_t given, Py_ssize_t want, F f) {
     if (given != want) return PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, got %zd", name, want, given);
-    try {
-        return f();
-    } catch (const c10::Error& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-    } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown error");
-    }
-    return nullptr;
+    HANDLE_TH_ERRORS
+    return f();
+    END_HANDLE_TH_ERRORS
 }
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded("layer_norm", n, 4, [&] { return THPVariable_Wrap(layer_norm(a)); });
