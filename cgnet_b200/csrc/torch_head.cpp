@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <stdexcept>
@@ -59,6 +60,8 @@ const Tensor& values_of(PyObject* o, const char* name, const Tensor* like = null
     const Tensor& t = tensor_of(o, name);
     if (type_code(t) < 0) fail(std::string(name) + " must be float32, bfloat16 or float16, got " + type_name(t));
     if (like != nullptr) check_device(t, name, *like);
+    // a trace would hold the allocation of the results and not the kernel that writes them
+    if (torch::jit::tracer::isTracing()) fail("the operators of cgnet_b200.head cannot be recorded by torch.jit.trace");
     if (t._fw_grad(0).defined()) fail(std::string(name) + " has a forward-mode derivative, which the operators of cgnet_b200.head do not pass on");
     return t;
 }

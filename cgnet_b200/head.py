@@ -11,7 +11,7 @@ in float32 or more whatever that type, and each result is rounded once.  All ari
 current stream; the checks of the arguments, the allocations and the autograd nodes are C++ too (``_torch_head.so``,
 ``csrc/torch_head.cpp``).  There is no CPU path and no fallback: a missing library or a bad argument raises RuntimeError before
 anything is launched.  Every operator is differentiable once (in reverse mode), can be captured in a CUDA graph, and gives the same bits from run
-to run for the same tensors.  (As with any torch operator, capture a backward pass only while no eager graph of the same leaves
+to run for the same tensors; ``torch.jit.trace`` is refused.  (As with any torch operator, capture a backward pass only while no eager graph of the same leaves
 is alive: torch ties a leaf's gradient accumulation to the stream it was first used on.)  The order of a row's sums follows
 the 16-byte groups it lies in, so its last bits can depend on its address modulo 16.
 """

@@ -85,3 +85,13 @@ def test_memory_that_is_not_there():
     with pytest.raises(torch.OutOfMemoryError):
         cg.gated_feed_forward(x, w, w)
     assert cg.gated_feed_forward(x[:3], w, w).shape == (3, 1 << 16)
+
+
+def test_tracing_is_refused():
+    """A trace would return the memory that the kernels never write."""
+    x, w = torch.zeros(4, 6), torch.zeros(5, 6)
+    ids, scores = torch.zeros(4, 2, dtype=torch.long), torch.zeros(4, 2)
+    for call in (lambda t: cg.layer_norm(t), lambda t: cg.gated_feed_forward(t, w, w), lambda t: cg.log_probs(t).entropy,
+                 lambda t: cg.distillation_loss(t, ids, scores)):
+        with pytest.raises(RuntimeError, match="torch.jit.trace"):
+            torch.jit.trace(call, (x,))
