@@ -1,0 +1,110 @@
+"""Accuracy of the gated block's tensor-core products by themselves, through the C interface: the kept projections g and u, and the
+backward's products with g = u = 1 kept and relu, where dg = du = dh exactly."""
+import pytest
+import torch
+
+from test_gpu_head import U, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def operands(x, wg, wu):
+    return x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0)
+
+
+def workspace(lib, x, wg, wu, code, gradients):
+    n = lib.cgb200_gated_ff_workspace_bytes(*operands(x, wg, wu), x.shape[0], x.shape[1], wg.shape[0], code, gradients)
+    assert n >= 0
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=x.device)
+
+
+def code_of(t):
+    from cgnet_b200 import _lib
+    return {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[t]
+
+
+def projections(x, wg, wu):
+    from cgnet_b200 import _lib
+    lib, code, (rows, dim), hidden = _lib.load(), code_of(x.dtype), x.shape, wg.shape[0]
+    pitch = -(-hidden // 4) * 4
+    kept, h, ws = torch.empty(2, rows, pitch, device=x.device), torch.empty(rows, hidden, dtype=x.dtype, device=x.device), workspace(lib, x, wg, wu, code, 0)
+    assert lib.cgb200_gated_ff_fwd(*operands(x, wg, wu), 2, h.data_ptr(), kept.data_ptr(), rows, dim, hidden, code, ws.data_ptr(), ws.numel(), stream()) == 0
+    return kept[0, :, :hidden], kept[1, :, :hidden]
+
+
+def gradients(x, wg, wu, dh, kept=None):
+    """dx, dWg, dWu for relu; g = u = 1 unless given as [2][rows][pitch]."""
+    from cgnet_b200 import _lib
+    lib, code, (rows, dim), hidden = _lib.load(), code_of(x.dtype), x.shape, wg.shape[0]
+    if kept is None:
+        kept = torch.ones(2, rows, -(-hidden // 4) * 4, device=x.device)
+    dx, dwg, dwu, ws = torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu), workspace(lib, x, wg, wu, code, 7)
+    assert lib.cgb200_gated_ff_bwd(*operands(x, wg, wu), 2, kept.data_ptr(), dh.data_ptr(), dh.stride(0), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), rows,
+                                   dim, hidden, code, ws.data_ptr(), ws.numel(), stream()) == 0, lib.cgb200_last_error()
+    return dx, dwg, dwu
+
+
+def rms(t):
+    return float((t.double() ** 2).mean().sqrt())
+
+
+# the fused forward with one and with both accumulators and several tiles a block; the split one; both layouts of the backward
+SIZES = [(700, 520, 700), (1200, 2048, 900), (156, 1330, 342), (300, 4096, 128)]
+
+
+@pytest.mark.parametrize("rows, dim, hidden", SIZES)
+def test_float32_products_are_off_by_roundings_of_float32(rows, dim, hidden):
+    """Root mean square of the error over that of sqrt(sum (a b)^2), which a random walk of roundings scales with.
+
+    A flush holds 16 truncating additions of 16 terms each; addition j is off by at most one step, 2 u |acc|, with |acc| about
+    sqrt(16 j): together 2 u * 4 * sum sqrt(j) = 358 u against sqrt(256) = 16, that is 22 u, and flushes are independent of one another.
+    Their sum in registers, the parts of a split and the products left out (2 u at most, random) add less than 5 u.  Products
+    formed from planes on the CPU are off by 0.1 u so, by 41 without the third plane of one operand, 58 without either, 46 without the
+    product of the second ones."""
+    g = gen(rows + dim + hidden)
+    x, wg, wu, dh = randn(g, rows, dim), randn(g, hidden, dim), randn(g, hidden, dim), randn(g, rows, hidden)
+    x64, wg64, wu64, dh64 = (t.double() for t in (x, wg, wu, dh))
+    p, q = projections(x, wg, wu)
+    dx, dwg, dwu = gradients(x, wg, wu, dh)
+    for name, got, want, square in (("g", p, x64 @ wg64.t(), x64 ** 2 @ wg64.t() ** 2), ("u", q, x64 @ wu64.t(), x64 ** 2 @ wu64.t() ** 2),
+                                    ("dx", dx, dh64 @ (wg64 + wu64), dh64 ** 2 @ (wg64 ** 2 + wu64 ** 2)),
+                                    ("dwg", dwg, dh64.t() @ x64, dh64.t() ** 2 @ x64 ** 2), ("dwu", dwu, dh64.t() @ x64, dh64.t() ** 2 @ x64 ** 2)):
+        off = rms(got - want) / rms(square.sqrt())
+        assert off <= 32 * U, f"{name}: {off / U:.1f} u"
+
+
+@pytest.mark.parametrize("rows, dim, hidden", SIZES)
+def test_float32_products_of_two_terms(rows, dim, hidden):
+    """Rows with two values each, the second nearly the first's negative times the weights' ratio where it matters most: the leading planes
+    cancel and the result is what the small ones hold.  Adding zeros is exact, so an output of n terms is off by at most 2 n u of
+    its absolute sum, 2 u for the products left out, and the roundings of lead + rest and of the sum of flushes or parts.  (Planes on the
+    CPU: 0.6 u; 85 to 197 without one of the small products.)"""
+    g = gen(rows * 3 + dim + hidden)
+
+    def sparse(r, c):
+        t = torch.zeros(r, c, device="cuda")
+        at = torch.stack([torch.randperm(c, generator=g, device="cuda")[:2] for _ in range(r)])
+        v = 1 + torch.rand(r, 1, generator=g, device="cuda")
+        pair = torch.cat([v, -v * (1 + 2.0 ** -9 * torch.rand(r, 1, generator=g, device="cuda"))], 1)
+        return t.scatter_(1, at, pair)
+    x, dh = sparse(rows, dim), sparse(rows, hidden)
+    # all weights of a row nearly the same
+    wg = (1 + torch.rand(hidden, 1, generator=g, device="cuda")) * (1 + 2.0 ** -9 * torch.rand(hidden, dim, generator=g, device="cuda"))
+    wu = (1 + torch.rand(hidden, 1, generator=g, device="cuda")) * (1 + 2.0 ** -9 * torch.rand(hidden, dim, generator=g, device="cuda"))
+    x64, wg64, wu64, dh64 = (t.double() for t in (x, wg, wu, dh))
+    p, q = projections(x, wg, wu)
+    dx, dwg, dwu = gradients(x, wg, wu, dh)
+
+    def check(name, got, want, size, terms):
+        off = (got.double() - want).abs() - (2 * terms + 5) * U * size
+        assert float(off.max()) <= 0, f"{name}: {float(((got.double() - want).abs() / size.clamp(min=1e-30)).max()) / U:.1f} u"
+    ax, adh, nx, ndh = x64.abs(), dh64.abs(), (x64 != 0).double(), (dh64 != 0).double()
+    check("g", p, x64 @ wg64.t(), ax @ wg64.t(), 2)
+    check("u", q, x64 @ wu64.t(), ax @ wu64.t(), 2)
+    check("dx", dx, dh64 @ (wg64 + wu64), adh @ (wg64 + wu64), 4)
+    for name, got in (("dwg", dwg), ("dwu", dwu)):
+        check(name, got, dh64.t() @ x64, adh.t() @ ax, ndh.t() @ nx)
