@@ -14,6 +14,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "row_ops.cuh"
 #include "tc_ptx.cuh"
 
@@ -29,6 +31,9 @@ constexpr int kFfStaging = 32 * 32;            // floats of an epilogue warp's s
 constexpr size_t kFfSmem = 1024 + kFfStageBytes + kFfEpiWarps * kFfStaging * sizeof(float);
 static_assert(kFfSmem <= kMaxDynSmem, "stages and staging must fit a block's shared memory");
 
+// Tensor maps of a launch: operands (the backward's dg and du for dx, and for the weights' gradients where those are scaled apart), outputs
+enum FfMap { kMapX, kMapWg, kMapWu, kMapDg, kMapDu, kMapDgCols, kMapDuCols, kMapOut, kMapOutWg, kMapOutWu };
+
 struct FfProblem {
     int a_map[2], b_map[2];     // tensor maps of A and B: by source of the contraction (dx), set of rows (dW: A), half of the columns (forward: B)
     int a_mn, b_mn;             // 1: the operand's i / j axis is the contiguous one
@@ -42,9 +47,10 @@ struct FfProblem {
     void* out[2];               // per set; the forward: h
     int out_map[2];             // tensor map of the output by bulk copies, -1: written by threads; the forward: [0] g and u, -1: not kept
     float* part;                // [splits][sets * n_i][n_j] where splits > 1
+    const uint32_t* amax[2];    // per set, half precision's backward: largest value of each row of A before it was scaled; null: not scaled
 };
 struct FfGemmArgs {
-    CUtensorMap map[8];         // x, Wg, Wu, dg, du, then outputs
+    CUtensorMap map[10];        // kMap...
     FfProblem p[2];
     int problems, units;
     uint32_t idesc_type;        // operand format bits of the instruction descriptor
@@ -102,6 +108,12 @@ __device__ __forceinline__ uint64_t box_desc(uint32_t saddr, int mn) {
     return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(mn ? kFfBox >> 4 : 1) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
            ((uint64_t)2 << 61);
 }
+
+// Power of two that brings values up to `amax` (the bits of a float32, 0: none) below 2^15, and its inverse.  The largest factor is
+// 2^126, so that the inverse is not subnormal.
+__device__ __forceinline__ uint32_t scale_exponent(uint32_t amax) { return amax == 0 ? 127u : min(127 + 14 + 127 - (amax >> 23), 253u); }
+__device__ __forceinline__ float scale_of(uint32_t amax) { return __uint_as_float(scale_exponent(amax) << 23); }
+__device__ __forceinline__ float unscale_of(uint32_t amax) { return __uint_as_float((254u - scale_exponent(amax)) << 23); }
 
 // act(g) and its derivative
 template <int ACT, bool GRAD>
@@ -372,10 +384,20 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             auto staging_free = [&] {
                 if (lane == 0) tma_store_wait<0>();
             };
-            auto emit = [&](int c, const float* v, const float* w) {
+            constexpr bool SCALED = !FWD && std::is_same<T, __half>::value;
+            const uint32_t* amax = SCALED ? p.amax[t.set] : nullptr;
+            const float back = amax != nullptr && row0 + lane < p.n_i ? unscale_of(amax[row0 + lane]) : 1.f;
+            auto emit = [&](int c, const float* given, const float* w) {
                 const int col0 = t.j0 + side * (JW / 2) + c * kCols;
                 if (!rows_here || col0 >= p.n_j) return;
                 char* bytes = (char*)st;
+                float unscaled[SCALED ? 32 : 1];
+                const float* v = given;
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) unscaled[i] = given[i] * back;
+                    v = unscaled;
+                }
                 if constexpr (FWD) {
                     float g[16], u[16];
 #pragma unroll

@@ -334,8 +334,9 @@ __global__ void __launch_bounds__(256) ff_pack_kernel(FfPackArgs a) {
     }
 }
 
-// dg and du, as operands of the products behind them, in the type of x: 1.4 times the rounding error of the formula's own gradients,
-// and half of what a second read of float32 planes would cost.  At the HBM roof: 8192 x 5120 bf16 (419 MB read, 132 written) 83 us.
+// dg and du, as operands of the products behind them, in the type of x (half precision: ff_range_kernel).  In bfloat16 that rounding adds
+// as much error to the gradients as their own: 1.4 times the error of one rounding (relative, 8192 rows, 2048 -> 5120: 2.34e-3 against
+// 1.66e-3); a second plane of each would double the products (456 us).  At the HBM roof: 8192 x 5120 bf16 (419 MB read, 132 written) 83 us.
 template <typename T>
 __global__ void __launch_bounds__(256) ff_dgu_kernel(FfArgs a, void* dg, void* du, int64_t pitch) {
     const int64_t chunks = pitch / 8, n = a.rows * chunks;
@@ -356,6 +357,111 @@ __global__ void __launch_bounds__(256) ff_dgu_kernel(FfArgs a, void* dg, void* d
         }
         store_operand<T>(operand_at<T>(dg, r * pitch + e0), a.rows * pitch, gv);
         store_operand<T>(operand_at<T>(du, r * pitch + e0), a.rows * pitch, uv);
+    }
+}
+
+// Half precision's dg and du may leave its range, on either side, where the gradients behind them do not.  So each is scaled by a
+// power of two, which costs no digits, and the products' epilogue takes it back: row by row for dx (a large row costs no other one
+// its small values), and a second copy unit by unit for the weights' gradients, whose sums run down the rows.  The factors come
+// from the largest finite values, found first: 8192 x 5120 99 us, and 122 for both copies (683 MB, 5.6 TB/s), against 83 unscaled.
+// A block has `w` lanes of eight units side by side and `steps` rows for each of the others: eight where the rows keep the SMs busy, so that
+// few blocks meet at one unit's largest value, fewer where they do not (256 x 1024: 17 us a kernel with eight).
+constexpr int kFfRangeSteps = 8;
+struct FfRange {
+    uint32_t *rows, *cols;      // largest |dg|, |du| of a row, [rows]; of a unit, [2][pitch]; bits of a float32; null where not wanted
+    int64_t pitch;
+    int w, steps;               // w: a power of two up to 32
+    __half *dg, *du;            // [rows][pitch], by rows
+    __half *dg_cols, *du_cols;  // by units
+};
+// dg and du of eight units, in place of g and u
+template <int ACT>
+__device__ __forceinline__ void turn_gradients(float (&g)[8], float (&u)[8], const float (&dh)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 f = activate_as<ACT, true>(g[i]);
+        g[i] = dh[i] * u[i] * f.y;
+        u[i] = dh[i] * f.x;
+    }
+}
+template <bool WRITE>
+__global__ void __launch_bounds__(256, 4) ff_range_kernel(FfArgs a, FfRange q) {
+    __shared__ uint32_t most[WRITE ? 1 : 8 * 32 * 16];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = q.w, at = (int)threadIdx.x & (w - 1);
+    const int64_t e0 = ((int64_t)blockIdx.y * w + at) * 8, row0 = (int64_t)blockIdx.x * (256 / w) * q.steps + threadIdx.x / w;
+    const float* g = a.gu;
+    const float* u = a.gu + a.rows * a.gu_pitch;
+    uint32_t top[16];           // of this thread's units
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top[i] = 0;
+    float sg[8], su[8];
+    if (WRITE && q.cols != nullptr && e0 < q.pitch) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sg[i] = scale_of(q.cols[e0 + i]), su[i] = scale_of(q.cols[q.pitch + e0 + i]);
+    }
+#pragma unroll 2
+    for (int s = 0; s < q.steps; ++s) {
+        const int64_t r = row0 + (int64_t)s * (256 / w);
+        const bool in = r < a.rows && e0 < q.pitch;
+        uint32_t big = 0;
+        if (in) {
+            float gv[8], uv[8], dv[8];
+            load_params<float, 8>(g + r * a.gu_pitch, e0, a.hidden, gv);
+            load_params<float, 8>(u + r * a.gu_pitch, e0, a.hidden, uv);
+            load_params<__half, 8>((const __half*)a.dh + r * a.dh_stride, e0, a.hidden, dv);
+            if (a.act == CGB200_ACT_RELU) turn_gradients<CGB200_ACT_RELU>(gv, uv, dv);
+            else if (a.act == CGB200_ACT_SILU) turn_gradients<CGB200_ACT_SILU>(gv, uv, dv);
+            else turn_gradients<CGB200_ACT_GELU>(gv, uv, dv);
+            if (WRITE) {
+                float x[8], y[8];
+                if (q.rows != nullptr) {
+                    const float sr = scale_of(q.rows[r]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = gv[i] * sr, y[i] = uv[i] * sr;
+                    *reinterpret_cast<uint4*>(q.dg + r * q.pitch + e0) = pack16(x, (const __half*)nullptr);
+                    *reinterpret_cast<uint4*>(q.du + r * q.pitch + e0) = pack16(y, (const __half*)nullptr);
+                }
+                if (q.cols != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = gv[i] * sg[i], y[i] = uv[i] * su[i];
+                    *reinterpret_cast<uint4*>(q.dg_cols + r * q.pitch + e0) = pack16(x, (const __half*)nullptr);
+                    *reinterpret_cast<uint4*>(q.du_cols + r * q.pitch + e0) = pack16(y, (const __half*)nullptr);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    // an infinity or NaN spoils its own row and unit, but is no measure for them
+                    uint32_t bg = __float_as_uint(fabsf(gv[i])), bu = __float_as_uint(fabsf(uv[i]));
+                    bg = bg < 0x7f800000u ? bg : 0u, bu = bu < 0x7f800000u ? bu : 0u;
+                    top[i] = max(top[i], bg), top[8 + i] = max(top[8 + i], bu);
+                    big = max(big, max(bg, bu));
+                }
+            }
+        }
+        if (!WRITE && q.rows != nullptr) {
+            if (w == 32) {
+                big = __reduce_max_sync(0xffffffffu, big);
+            } else {
+                for (int o = w / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+            }
+            if (at == 0 && r < a.rows && big != 0) atomicMax(q.rows + r, big);
+        }
+    }
+    if (WRITE || q.cols == nullptr) return;
+    // the rows of a warp, then its block's warps
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        for (int o = 16; o >= w; o >>= 1) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+        most[(warp * 16 + i) * 32 + lane] = top[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < w * 16; i += 256) {
+        const int unit = i / 16, side = i % 16 / 8, j = i % 8;
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = max(m, most[(k * 16 + side * 8 + j) * 32 + unit]);
+        const int64_t col = ((int64_t)blockIdx.y * w + unit) * 8 + j;
+        if (m != 0 && col < q.pitch) atomicMax(q.cols + side * q.pitch + col, m);
     }
 }
 
@@ -442,7 +548,7 @@ struct FfPlan {
     int planes, bn;
     bool pack[3];                         // x, Wg, Wu
     int64_t pitch_d, pitch_h;             // of packed operands (dim columns) and of dg, du (hidden columns)
-    int64_t off_pack[3], off_dg, off_du, off_part[2], bytes;
+    int64_t off_pack[3], off_dg, off_du, off_dg_cols, off_du_cols, off_amax, off_part[2], bytes;
     int n_problems;
     FfProblem problem[2];
 };
@@ -472,9 +578,12 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
         q.off_pack[i] = at;
         if (q.pack[i]) at += up(q.planes * rows[i] * q.pitch_d * 2, 256);
     }
-    if (!fwd) {
-        q.off_dg = at, at += up(q.planes * a.rows * q.pitch_h * 2, 256);
-        q.off_du = at, at += up(q.planes * a.rows * q.pitch_h * 2, 256);
+    const bool scaled = !fwd && dtype == CGB200_F16;
+    const int64_t d_bytes = up(q.planes * a.rows * q.pitch_h * 2, 256);
+    if (!fwd && (!scaled || (grads & 1))) q.off_dg = at, q.off_du = at + d_bytes, at += 2 * d_bytes;
+    if (scaled) {
+        if (grads & 6) q.off_dg_cols = at, q.off_du_cols = at + d_bytes, at += 2 * d_bytes;
+        q.off_amax = at, at += up((a.rows + 2 * q.pitch_h) * 4, 256);
     }
     const int64_t ti = (a.rows + kFfBM - 1) / kFfBM;
     const int hk = (a.hidden + kFfBK - 1) / kFfBK, dk = (a.dim + kFfBK - 1) / kFfBK;
@@ -491,21 +600,21 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     if (q.joined) {
         for (int i = 0; i < 2; ++i) {
             FfProblem& p = q.problem[q.n_problems++];
-            p.a_map[0] = 0, p.b_map[0] = 1 + i;
+            p.a_map[0] = kMapX, p.b_map[0] = kMapWg + i;
             p.sources = 1, p.kblk = dk, p.sets = 1;
             p.tiles_i = (int)ti, p.tiles_j = (a.hidden + q.bn - 1) / q.bn;
             p.n_i = a.rows, p.n_j = a.hidden;
         }
     } else if (fwd) {
         FfProblem& p = q.problem[q.n_problems++];
-        p.a_map[0] = 0, p.b_map[0] = 1, p.b_map[1] = 2;
+        p.a_map[0] = kMapX, p.b_map[0] = kMapWg, p.b_map[1] = kMapWu;
         p.sources = 1, p.kblk = dk, p.sets = 1;
         p.tiles_i = (int)ti, p.tiles_j = (a.hidden + q.bn / 2 - 1) / (q.bn / 2);
         p.n_i = a.rows, p.n_j = a.hidden;
     }
     if (grads & 1) {
         FfProblem& p = q.problem[q.n_problems++];
-        p.a_map[0] = 3, p.a_map[1] = 4, p.b_map[0] = 1, p.b_map[1] = 2, p.b_mn = 1;
+        p.a_map[0] = kMapDg, p.a_map[1] = kMapDu, p.b_map[0] = kMapWg, p.b_map[1] = kMapWu, p.b_mn = 1;
         p.sources = 2, p.kblk = hk, p.sets = 1;
         p.tiles_i = (int)ti, p.tiles_j = (a.dim + q.bn - 1) / q.bn;
         p.n_i = a.rows, p.n_j = a.dim;
@@ -513,7 +622,8 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     }
     if (w_sets > 0) {
         FfProblem& p = q.problem[q.n_problems++];
-        p.a_map[0] = (grads & 2) ? 3 : 4, p.a_map[1] = 4, p.b_map[0] = 0, p.a_mn = p.b_mn = 1;
+        const int dg = scaled ? kMapDgCols : kMapDg, du = scaled ? kMapDuCols : kMapDu;
+        p.a_map[0] = (grads & 2) ? dg : du, p.a_map[1] = du, p.b_map[0] = kMapX, p.a_mn = p.b_mn = 1;
         p.sources = 1, p.kblk = mk, p.sets = w_sets;
         p.tiles_i = th, p.tiles_j = (a.dim + q.bn - 1) / q.bn;
         p.n_i = a.hidden, p.n_j = a.dim;
@@ -634,19 +744,47 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
     }
     FfGemmArgs g{};
     bool ok = true;
-    const bool half = std::is_same<T, __half>::value;
+    constexpr bool half = std::is_same<T, __half>::value;
+    uint32_t *row_max = nullptr, *col_max = nullptr;
     for (int i = 0; i < 3; ++i) {
         const bool used = fwd || (i == 0 ? (grads & 6) != 0 : (grads & 1) != 0);
-        if (used) ok = ok && ff_map(&g.map[i], enc, src[i], stride[i], rows[i], a.dim, PLANES, half);
+        if (used) ok = ok && ff_map(&g.map[kMapX + i], enc, src[i], stride[i], rows[i], a.dim, PLANES, half);
     }
     if (!fwd) {
-        void *dg = ws + q.off_dg, *du = ws + q.off_du;
-        launch_begin(kid, st);
-        ff_dgu_kernel<T><<<(unsigned)std::min<int64_t>((a.rows * q.pitch_h / 8 + 255) / 256, kNumSM * 16), 256, 0, st>>>(a, dg, du, q.pitch_h);
-        launch_end(kid, st);
-        CGB_CUDA(cudaGetLastError());
-        ok = ok && ff_map(&g.map[3], enc, dg, q.pitch_h, a.rows, a.hidden, PLANES, half);
-        ok = ok && ff_map(&g.map[4], enc, du, q.pitch_h, a.rows, a.hidden, PLANES, half);
+        void *dg = ws + q.off_dg, *du = ws + q.off_du, *dg_cols = ws + q.off_dg_cols, *du_cols = ws + q.off_du_cols;
+        if constexpr (std::is_same<T, __half>::value) {
+            FfRange r{};
+            row_max = (uint32_t*)(ws + q.off_amax), col_max = row_max + a.rows;
+            if (grads & 1) r.rows = row_max, r.dg = (__half*)dg, r.du = (__half*)du;
+            if (grads & 6) r.cols = col_max, r.dg_cols = (__half*)dg_cols, r.du_cols = (__half*)du_cols;
+            r.pitch = q.pitch_h, r.w = 1;
+            while (r.w < 32 && r.w < q.pitch_h / 8) r.w *= 2;
+            CGB_CUDA(cudaMemsetAsync(row_max, 0, (a.rows + 2 * q.pitch_h) * 4, st));
+            const int64_t side = (q.pitch_h / 8 + r.w - 1) / r.w, one = (a.rows * r.w + 255) / 256;      // blocks; of one row a thread
+            r.steps = (int)std::max<int64_t>(1, std::min<int64_t>(kFfRangeSteps, one * side / (kNumSM * 8)));
+            const dim3 grid((unsigned)((one + r.steps - 1) / r.steps), (unsigned)side);
+            launch_begin(kid, st);
+            ff_range_kernel<false><<<grid, 256, 0, st>>>(a, r);
+            launch_end(kid, st);
+            CGB_CUDA(cudaGetLastError());
+            launch_begin(kid, st);
+            ff_range_kernel<true><<<grid, 256, 0, st>>>(a, r);
+            launch_end(kid, st);
+            CGB_CUDA(cudaGetLastError());
+        } else {
+            launch_begin(kid, st);
+            ff_dgu_kernel<T><<<(unsigned)std::min<int64_t>((a.rows * q.pitch_h / 8 + 255) / 256, kNumSM * 16), 256, 0, st>>>(a, dg, du, q.pitch_h);
+            launch_end(kid, st);
+            CGB_CUDA(cudaGetLastError());
+        }
+        if (!half || (grads & 1)) {
+            ok = ok && ff_map(&g.map[kMapDg], enc, dg, q.pitch_h, a.rows, a.hidden, PLANES, half);
+            ok = ok && ff_map(&g.map[kMapDu], enc, du, q.pitch_h, a.rows, a.hidden, PLANES, half);
+        }
+        if (half && (grads & 6)) {
+            ok = ok && ff_map(&g.map[kMapDgCols], enc, dg_cols, q.pitch_h, a.rows, a.hidden, PLANES, half);
+            ok = ok && ff_map(&g.map[kMapDuCols], enc, du_cols, q.pitch_h, a.rows, a.hidden, PLANES, half);
+        }
     }
     if (!ok) {
         set_error("gated feed-forward: an operand's layout was refused by the driver");
@@ -667,14 +805,15 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
             p.out[0] = a.h;
             p.h_aligned = at16(a.h) && a.hidden % Chunk<T>::N == 0;
             if (a.gu != nullptr) {
-                p.out_map[0] = 5;
-                ok = ok && ff_out_map<float>(&g.map[5], enc, a.gu, a.gu_pitch, a.rows, a.hidden, 2);
+                p.out_map[0] = kMapOut;
+                ok = ok && ff_out_map<float>(&g.map[kMapOut], enc, a.gu, a.gu_pitch, a.rows, a.hidden, 2);
             }
             continue;
         }
+        for (int k = 0; half && k < p.sets; ++k) p.amax[k] = !p.a_mn ? row_max : col_max + (p.a_map[k] == kMapDuCols ? q.pitch_h : 0);
         for (int k = 0; k < p.sets; ++k)
             if (p.splits == 1 && p.out[k] != nullptr && at16(p.out[k]) && a.dim % Chunk<T>::N == 0) {
-                const int m = p.a_mn ? 6 + k : 5;
+                const int m = p.a_mn ? kMapOutWg + k : kMapOut;
                 p.out_map[k] = m;
                 ok = ok && ff_out_map<T>(&g.map[m], enc, p.out[k], a.dim, p.n_i, a.dim, 1);
             }

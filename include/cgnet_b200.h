@@ -279,7 +279,8 @@ int cgb200_raycast_sphere(const float* vertices, int64_t n_vertices, const int32
 /*
  * The operators between a network's invariant embedding and its answers (no counterpart in the reference's kernels, which
  * leaves them to torch).  Matrices are row-major with the given number of values between rows (`stride`), values of one of
- * three types; sums, norms and softmax statistics are held in float32 or more and every result is rounded once.  Pointers
+ * three types; sums, norms and softmax statistics are held in float32 or more and every result is rounded once (one exception, in
+ * the gated block's backward, is described there).  Pointers
  * need the alignment of their type only, except where more is said.  Results do not depend on timing (no float atomics); the order of
  * a row's sums follows the 16-byte groups it lies in, so its last bits can depend on its address modulo 16.
  */
@@ -312,6 +313,9 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
  * the weights' gradients.  workspace: cgb200_gated_ff_workspace_bytes bytes (`gradients` = 0 for the forward, else the sum of 1 for
  * dx, 2 for dw_gate and 4 for dw_up, as the call asks for them; the operands' addresses and strides decide whether they have to
  * be copied), 256-byte aligned, contents undefined; one workspace serves one call at a time.
+ * On the tensor cores the backward rounds the gradients of the two projections to `dtype` before it multiplies them; in
+ * CGB200_F16 they are scaled by a power of two per row (dx) and per hidden unit (dw_gate, dw_up) and the products scaled back, so
+ * that values beyond that type's range on either side are not lost.
  * A tensor-core block that gives up on a bounded wait fills what it still owes with NaN.
  * Small products run on the CUDA cores, others on the tensor cores (float32 in three bfloat16 parts, accurate to float32).  A row of
  * x that is not finite spoils that row of h and dx; in float32 it may come out as NaN where the formula gives an infinity.

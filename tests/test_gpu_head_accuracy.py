@@ -3,7 +3,7 @@ backward's products with g = u = 1 kept and relu, where dg = du = dh exactly."""
 import pytest
 import torch
 
-from test_gpu_head import U, gen, randn
+from test_gpu_head import U, gen, half, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,87 @@ def test_float32_products_of_two_terms(rows, dim, hidden):
     check("dx", dx, dh64 @ (wg64 + wu64), adh @ (wg64 + wu64), 4)
     for name, got in (("dwg", dwg), ("dwu", dwu)):
         check(name, got, dh64.t() @ x64, adh.t() @ ax, ndh.t() @ nx)
+
+
+# CUDA cores; tensor cores with rows and units that fill no tile; several tiles with split and with whole contractions; one row, one unit
+RANGE_SIZES = [(100, 64, 64), (300, 104, 200), (1111, 1000, 1365), (700, 64, 24), (3000, 48, 9), (5, 40, 800), (2000, 520, 1032)]
+
+
+def range_bounds(x, wg, wu, dh, kept):
+    """dx, dWg, dWu of relu with their bounds: dg and du are off by 4 u (float32) and by half a step of fp16, of which a subnormal one is
+    2^-25 of the power of two that brings the row's (dx) or the unit's (dW) largest value to 2^14 or more: 2^-39 of that value."""
+    x, wg, wu, dh, g, u = (t.double() for t in (x, wg, wu, dh, kept[0], kept[1]))
+    dg, du = dh * u * (g > 0), dh * g.clamp(min=0)
+    e = half(torch.float16) + 4 * U
+    most = torch.maximum(dg.abs().amax(1), du.abs().amax(1))[:, None]
+    edg, edu = e * dg.abs() + 2.0 ** -39 * most, e * du.abs() + 2.0 ** -39 * most
+    rows, hidden = dh.shape
+    out = [(dg @ wg + du @ wu, edg @ wg.abs() + edu @ wu.abs() + (4 * hidden + 8) * U * (dg.abs() @ wg.abs() + du.abs() @ wu.abs()))]
+    for d in (dg, du):
+        ed = e * d.abs() + 2.0 ** -39 * d.abs().amax(0)
+        out.append((d.t() @ x, ed.t() @ x.abs() + (2 * rows + 8) * U * (d.abs().t() @ x.abs())))
+    return out
+
+
+def check_range(x, wg, wu, dh, kept):
+    got = gradients(x, wg, wu, dh, kept)
+    for name, q, (want, tol) in zip(("dx", "dwg", "dwu"), got, range_bounds(x, wg, wu, dh, kept[:, :, :dh.shape[1]])):
+        assert float(want.abs().max()) < 6e4, "the case itself leaves the range"
+        off = (q.double() - want).abs() - tol - half(torch.float16) * (want.abs() + tol) - 2.0 ** -25
+        assert float(off.max()) <= 0, (name, float(off.max()), bool(torch.isfinite(q).all()))
+
+
+@pytest.mark.parametrize("rows, dim, hidden", RANGE_SIZES)
+@pytest.mark.parametrize("case", ["large", "small", "rows", "units", "zeros"])
+def test_half_precision_gradients_whose_factors_leave_its_range(case, rows, dim, hidden):
+    """dg and du beyond 65504 or below 6e-8 behind gradients that are neither, in all rows, in some rows, in some units."""
+    g = gen(rows + dim + hidden)
+    pitch = -(-hidden // 4) * 4
+    x, wg, wu, dh, kept = randn(g, rows, dim), randn(g, hidden, dim), randn(g, hidden, dim), randn(g, rows, hidden), randn(g, 2, rows, pitch)
+    few = torch.arange(rows, device="cuda") % 7 == 0
+    if case == "large":
+        dh, kept, wg, wu, x = 300 * dh, 300 * kept, 1e-4 * wg, 1e-4 * wu, 1e-4 * x
+    elif case == "small":
+        dh, kept, x, wg, wu = 3e-7 * dh, 0.1 * kept, 300 * x, 300 * wg, 300 * wu
+    elif case == "rows":        # large rows with small inputs beside small rows with ordinary ones
+        size = torch.where(few, 3e2, 1e-4)[:, None]
+        dh, kept, wg, wu, x = size * dh, torch.where(few, 300.0, 1.0)[:, None] * kept, 1e-3 * wg, 1e-3 * wu, torch.where(few, 1e-4, 1.0)[:, None] * x
+    elif case == "units":
+        some = torch.arange(hidden, device="cuda") % 5 == 1
+        wide = torch.arange(pitch, device="cuda") % 5 == 1
+        dh, kept = torch.where(some, 300.0, 1e-5) * dh, torch.where(wide, 300.0, 1.0) * kept
+        wg, wu, x = torch.where(some, 1e-4, 1.0)[:, None] * wg, torch.where(some, 1e-4, 1.0)[:, None] * wu, 1e-3 * x
+    else:
+        dh = torch.where(few[:, None], dh, torch.zeros_like(dh))
+        dh[:, ::3] = 0
+    x, wg, wu, dh = (t.half() for t in (x, wg, wu, dh))
+    check_range(x, wg, wu, dh, kept)
+
+
+@pytest.mark.parametrize("rows, dim, hidden", RANGE_SIZES)
+def test_half_precision_infinities_stay_in_their_row_and_unit(rows, dim, hidden):
+    g = gen(rows + dim + hidden)
+    x, wg, wu, dh = (t.half() for t in (randn(g, rows, dim), randn(g, hidden, dim) / 8, randn(g, hidden, dim) / 8, randn(g, rows, hidden)))
+    kept = randn(g, 2, rows, -(-hidden // 4) * 4).abs() + 0.1
+    want = gradients(x, wg, wu, dh, kept)
+    bad = dh.clone()
+    bad[2, 3], bad[4, 5] = float("inf"), float("nan")
+    got = gradients(x, wg, wu, bad, kept)
+    rows_left = [r for r in range(rows) if r not in (2, 4)]
+    units_left = [j for j in range(hidden) if j not in (3, 5)]
+    assert torch.equal(got[0][rows_left], want[0][rows_left]) and not torch.isfinite(got[0][[2, 4]]).any()
+    for p, q in zip(got[1:], want[1:]):
+        assert torch.equal(p[units_left], q[units_left]) and not torch.isfinite(p[[3, 5]]).any()
+
+
+@pytest.mark.parametrize("gradient", [1, 2, 4, 3, 5, 6])
+def test_half_precision_gradients_one_by_one(gradient):
+    """Only the copies that a call's gradients need are made: the same bits as all of them together."""
+    import cgnet_b200 as cg
+    g = gen(gradient)
+    x, wg, wu, dh = (t.half() for t in (randn(g, 300, 104), randn(g, 200, 104) / 8, randn(g, 200, 104) / 8, 300 * randn(g, 300, 200)))
+    full = [t.clone().requires_grad_() for t in (x, wg, wu)]
+    want = torch.autograd.grad(cg.gated_feed_forward(*full, activation="relu"), full, dh)
+    part = [t.clone().requires_grad_(bool(gradient >> i & 1)) for i, t in enumerate((x, wg, wu))]
+    got = torch.autograd.grad(cg.gated_feed_forward(*part, activation="relu"), [t for t in part if t.requires_grad], dh)
+    assert all(torch.equal(p, q) for p, q in zip(got, [w for w, t in zip(want, part) if t.requires_grad]))
