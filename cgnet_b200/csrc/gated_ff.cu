@@ -537,6 +537,10 @@ struct FfLimits {
 static FfLimits ff_limits(int dtype) { return dtype == CGB200_F32 ? FfLimits{512, 640, 16 << 20} : FfLimits{128, 160, 8 << 20}; }
 
 constexpr int kFfOutputStages = 8;
+// Stages of 16-bit operands that one accumulator takes: the tensor core truncates each of its additions, four a stage, so a long sum of one
+// sign comes out low, by 1.7e-4 after 512 stages, 8e-4 after 2048 (measured; half a step of bfloat16 is 3.9e-3, of float16 4.9e-4).
+// Longer contractions go in parts that are added, rounded, in float32.  (float32 operands are flushed every kFfFlush stages.)
+static int ff_longest(int dtype) { return dtype == CGB200_F32 ? 1 << 30 : dtype == CGB200_BF16 ? 512 : 256; }
 // A forward whose tiles keep at most half of the SMs busy is split along dim from this many stages on.  Whole / split, us, launches of a
 // graph: bf16 16 x 1024 -> 1000 9.1 / 8.0, 16 x 4096 -> 1000 19.3 / 9.7, 500 x 2048 -> 1000 13.3 / 13.1, 156 x 3330 -> 342 30.8 / 15.7;
 // float32 300 x 640 -> 500 20.1 / 16.6, 156 x 3330 -> 342 78.7 / 22.6.
@@ -596,7 +600,8 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     };
     // wide tiles move less through shared memory; narrow ones fill the SMs where the wide ones do not
     q.bn = q.planes == 3 || units_at(256) < kNumSM ? 128 : 256;
-    q.joined = fwd && 2 * units_at(128) <= kNumSM && dk >= ff_split_stages(dtype);
+    const int longest = ff_longest(dtype);
+    q.joined = fwd && ((2 * units_at(128) <= kNumSM && dk >= ff_split_stages(dtype)) || dk > longest);
     if (q.joined) {
         for (int i = 0; i < 2; ++i) {
             FfProblem& p = q.problem[q.n_problems++];
@@ -643,7 +648,7 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
         int splits = q.joined                          ? (int)std::max<int64_t>(2, kNumSM / (2 * ti * p.tiles_j))
                      : fwd || length <= 1.5 * share ? 1
                                                     : (int)std::min(8.0, length / std::max(0.5 * share, 2.0 * kFfOutputStages) + 0.999);
-        splits = std::max(1, std::min(splits, stages / 4));
+        splits = std::max(std::max(1, std::min(splits, stages / 4)), stages / longest + (stages % longest != 0));
         p.kper = (stages + splits - 1) / splits;
         p.splits = (stages + p.kper - 1) / p.kper;
     }

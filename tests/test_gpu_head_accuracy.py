@@ -192,3 +192,33 @@ def test_half_precision_gradients_one_by_one(gradient):
     part = [t.clone().requires_grad_(bool(gradient >> i & 1)) for i, t in enumerate((x, wg, wu))]
     got = torch.autograd.grad(cg.gated_feed_forward(*part, activation="relu"), [t for t in part if t.requires_grad], dh)
     assert all(torch.equal(p, q) for p, q in zip(got, [w for w, t in zip(want, part) if t.requires_grad]))
+
+
+@pytest.mark.parametrize("dtype, terms", [(torch.bfloat16, 32768), (torch.float16, 16384)])
+def test_long_sums_of_one_sign(dtype, terms):
+    """The tensor core truncates as it adds, so a sum of one sign comes out low, the more the longer it is.  In parts of at most `terms` terms
+    its relative error is no more than the largest of its parts', and one rounding for each part.  How far a sum of `terms` terms is off
+    is measured by a call of that length; a part of the same length may be off twice as far, for a step of float32 is between u and
+    2 u of a value, depending on where the sum ends."""
+    def positive(g, *shape):
+        return (1 + torch.rand(*shape, generator=g, device="cuda")).to(dtype)
+    # a forward of more tiles than are split to fill the SMs
+    g, rows, dim, hidden = gen(1), 5000, 65560, 130
+    x, w = positive(g, rows, dim), positive(g, hidden, dim)
+    some = torch.cat([torch.arange(150), torch.arange(rows - 150, rows)])
+
+    def error(n):
+        want = sum(x[some, i:min(i + 8192, n)].double() @ w[:, i:min(i + 8192, n)].double().t() for i in range(0, n, 8192))
+        return max(float(((got[some].double() - want) / want).abs().max()) for got in projections(x[:, :n], w[:, :n], w[:, :n]))
+    one = error(terms)
+    assert one <= half(dtype) / 4, one / U
+    assert error(dim) <= 2 * one + (dim / terms + 8) * U
+    # weights' gradients; rounding them is random over the 64 x 64 values: half a step / sqrt(3) / 64, five times that at most
+    rows, dim, hidden = 1 << 19, 64, 64
+    size = 1 + torch.arange(64, device="cuda") / 64
+    x, dh = (2.0 ** -9 * size * positive(g, rows, dim).float()).to(dtype), (2.0 ** -7 * size * positive(g, rows, hidden).float()).to(dtype)
+    w = torch.zeros(hidden, dim, dtype=dtype, device="cuda")
+    want = dh.double().t() @ x.double()
+    for got in gradients(x, w, w, dh)[1:]:
+        off = abs(float(((got.double() - want) / want).mean()))
+        assert off <= 2 * one + (rows / terms + 8) * U + 5 * half(dtype) / 3 ** 0.5 / 64, off / U
