@@ -58,7 +58,9 @@ def gated_feed_forward(x, w_gate, w_up, activation="silu"):
     """``act(x w_gate^T) * (x w_up^T)`` over the last axis: x ``(..., dim)``, weights ``(hidden, dim)``, all of one type;
     ``activation`` is ``"silu"``, ``"gelu"`` (the exact one, with erf) or ``"relu"``.
 
-    A call that will be differentiated keeps both projections in float32 (8 bytes per row and hidden unit) for its backward."""
+    A call that will be differentiated keeps both projections in float32 (8 bytes per row and hidden unit) for its backward.  Values
+    that are not finite spoil the results of their own row of x, or of their own hidden unit, and no others; float32 operands are
+    multiplied in parts on the tensor cores, where a projection with an infinite term may be NaN instead of infinite."""
     return (_native or _load()).gated_feed_forward(x, w_gate, w_up, activation)
 
 

@@ -318,7 +318,8 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
  * that values beyond that type's range on either side are not lost.
  * A tensor-core block that gives up on a bounded wait fills what it still owes with NaN.
  * Small products run on the CUDA cores, others on the tensor cores (float32 in three bfloat16 parts, accurate to float32).  A row of
- * x that is not finite spoils that row of h and dx; in float32 it may come out as NaN where the formula gives an infinity.
+ * x that is not finite spoils that row of h and dx, a row of w_gate or w_up that is not finite that column of h.  In CGB200_F32 a
+ * projection with an infinite term may come out as NaN where the formula gives an infinity.
  */
 #define CGB200_ACT_SILU         0   /* g / (1 + exp(-g))                  */
 #define CGB200_ACT_GELU         1   /* g * (1 + erf(g / sqrt 2)) / 2      */

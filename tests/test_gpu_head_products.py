@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_head import check_ff, gen, randn
+from test_gpu_head import TYPES, check_ff, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,24 @@ def test_weight_gradients_of_different_alignment():
     want = gradients(0)
     for _ in range(10):
         assert all(torch.equal(p, q) for p, q in zip(gradients(1), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, dim, hidden", [(3, 100, 50), (40, 60, 70), (300, 520, 400), (20, 1100, 90)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_values_that_are_not_finite_stay_in_their_row_and_unit(rows, dim, hidden, dtype, bad):
+    """In float32 on the tensor cores an infinite term makes NaN of what may be an infinity, everywhere else it is the formula's."""
+    import cgnet_b200 as cg
+    x, wg, wu, _ = operands(rows, dim, hidden, dtype)
+    want = cg.gated_feed_forward(x, wg, wu, activation="relu")
+    xb, wb = x.clone(), wu.clone()
+    xb[2, 5], wb[7, 3] = bad, bad
+    got = cg.gated_feed_forward(xb, wg, wb, activation="relu")
+    r, u = [i for i in range(rows) if i != 2], [j for j in range(hidden) if j != 7]
+    assert torch.equal(got[r][:, u], want[r][:, u])
+    g, up = xb.double() @ wg.double().t(), xb.double() @ wb.double().t()
+    formula = (g.clamp(min=0) * up)
+    spoilt = ~torch.isfinite(formula)
+    assert not torch.isfinite(got[spoilt]).any() and spoilt[r, 7].sum() > 0 and spoilt[2].sum() > 0
+    if dtype != torch.float32 or dim < 512:
+        assert torch.equal(torch.isnan(got), torch.isnan(formula)) and torch.equal(torch.isinf(got), torch.isinf(formula))
