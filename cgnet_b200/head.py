@@ -121,7 +121,9 @@ class GatedFeedForward(nn.Module):
 
 class InvariantHead(nn.Module):
     """Classifier on the invariant embedding: ``norm`` (layer norm) -> ``ff`` (gated hidden layer) -> ``scores`` (linear),
-    ``(..., dim) -> (..., classes)`` logits.  ``SphericalCNN(..., head=(hidden, classes))`` builds one."""
+    ``(..., dim) -> (..., classes)`` logits.  ``SphericalCNN(..., head=(hidden, classes))`` builds one, in float32; with another
+    ``dtype`` the embedding is converted to it first and the logits are of it.  (``torch.autocast`` does not change what the operators
+    compute in: their types are their arguments'.)"""
 
     def __init__(self, dim, hidden, classes, activation="silu", device="cuda", dtype=torch.float32):
         super().__init__()
@@ -130,4 +132,4 @@ class InvariantHead(nn.Module):
         self.scores = nn.Linear(hidden, classes, device=device, dtype=dtype)
 
     def forward(self, x):
-        return self.scores(self.ff(self.norm(x)))
+        return self.scores(self.ff(self.norm(x.to(self.norm.weight.dtype))))
