@@ -31,8 +31,8 @@ constexpr int kFfStaging = 32 * 32;            // floats of an epilogue warp's s
 constexpr size_t kFfSmem = 1024 + kFfStageBytes + kFfEpiWarps * kFfStaging * sizeof(float);
 static_assert(kFfSmem <= kMaxDynSmem, "stages and staging must fit a block's shared memory");
 
-// Tensor maps of a launch: operands (the backward's dg and du for dx, and for the weights' gradients where those are scaled apart), outputs
-enum FfMap { kMapX, kMapWg, kMapWu, kMapDg, kMapDu, kMapDgCols, kMapDuCols, kMapOut, kMapOutWg, kMapOutWu };
+// Tensor maps of a launch: operands (the backward's dg and du; half precision's scaled copies by rows and by units), outputs
+enum FfMap { kMapX, kMapWg, kMapWu, kMapDg, kMapDu, kMapDgRows, kMapDuRows, kMapDgCols, kMapDuCols, kMapOut, kMapOutWg, kMapOutWu, kMaps };
 
 struct FfProblem {
     int a_map[2], b_map[2];     // tensor maps of A and B: by source of the contraction (dx), set of rows (dW: A), half of the columns (forward: B)
@@ -47,10 +47,13 @@ struct FfProblem {
     void* out[2];               // per set; the forward: h
     int out_map[2];             // tensor map of the output by bulk copies, -1: written by threads; the forward: [0] g and u, -1: not kept
     float* part;                // [splits][sets * n_i][n_j] where splits > 1
-    const uint32_t* amax[2];    // per set, half precision's backward: largest value of each row of A before it was scaled; null: not scaled
+    // half precision's backward, per set: whether a tile of rows is read from the scaled copy, that copy's map (by source or set, as
+    // a_map), and the largest value of each row, which tells its scale; null: never
+    const uint32_t *flag[2], *amax[2];
+    int a_scaled[2];
 };
 struct FfGemmArgs {
-    CUtensorMap map[10];        // kMap...
+    CUtensorMap map[kMaps];
     FfProblem p[2];
     int problems, units;
     uint32_t idesc_type;        // operand format bits of the instruction descriptor
@@ -109,6 +112,9 @@ __device__ __forceinline__ uint64_t box_desc(uint32_t saddr, int mn) {
            ((uint64_t)2 << 61);
 }
 
+// Half precision keeps a row or unit of dg and du as it is where its largest value is in this range: a subnormal value's rounding, 2^-25,
+// is then at most 2^-10 of the largest one's.
+__device__ __forceinline__ bool fits_half(uint32_t amax) { return amax == 0 || (amax >= __float_as_uint(0.0625f) && amax <= __float_as_uint(65504.f)); }
 // Power of two that brings values up to `amax` (the bits of a float32, 0: none) below 2^15, and its inverse.  The largest factor is
 // 2^126, so that the inverse is not subnormal.
 __device__ __forceinline__ uint32_t scale_exponent(uint32_t amax) { return amax == 0 ? 127u : min(127 + 14 + 127 - (amax >> 23), 253u); }
@@ -252,6 +258,9 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_ptr, polls = a.polls;
+    constexpr bool SCALED = !FWD && std::is_same<T, __half>::value;
+    auto scaled = [&](const FfUnit& t) { return SCALED && t.p->flag[t.set] != nullptr && t.p->flag[t.set][t.i0 / kFfBM] != 0; };
+
     // Units are listed longest first; blocks take them in turn, there and back, so that who had a long one gets a short one next.
     // (In an odd round the places may lie beyond the last unit for this block while other blocks still have one: it is done then.)
     auto unit_of = [&](int n) { return n * (int)gridDim.x + (n & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); };
@@ -268,8 +277,9 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
                 // in registers: what the loop looked up in the arguments each time cost it more than the copies' own time
                 const int kblk = t.p->kblk, a_mn = t.p->a_mn, b_mn = t.p->b_mn, i0 = (int)t.i0, j0 = t.j0, k1 = t.k1;
                 const bool two = t.p->sources > 1;
-                const CUtensorMap* a0 = &a.map[t.p->a_map[t.p->sets > 1 ? t.set : 0]];
-                const CUtensorMap* a1 = &a.map[t.p->a_map[1]];
+                const int* maps = scaled(t) ? t.p->a_scaled : t.p->a_map;
+                const CUtensorMap* a0 = &a.map[maps[t.p->sets > 1 ? t.set : 0]];
+                const CUtensorMap* a1 = &a.map[maps[1]];
                 const CUtensorMap *b0 = &a.map[t.p->b_map[0]], *b1 = &a.map[t.p->b_map[1]];
                 for (int it = t.k0; it < k1; ++it) {
                     if (!mbar_wait(&empty[s], ph, failed, polls)) {
@@ -384,9 +394,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             auto staging_free = [&] {
                 if (lane == 0) tma_store_wait<0>();
             };
-            constexpr bool SCALED = !FWD && std::is_same<T, __half>::value;
-            const uint32_t* amax = SCALED ? p.amax[t.set] : nullptr;
-            const float back = amax != nullptr && row0 + lane < p.n_i ? unscale_of(amax[row0 + lane]) : 1.f;
+            const float back = scaled(t) && row0 + lane < p.n_i ? unscale_of(p.amax[t.set][row0 + lane]) : 1.f;
             auto emit = [&](int c, const float* given, const float* w) {
                 const int col0 = t.j0 + side * (JW / 2) + c * kCols;
                 if (!rows_here || col0 >= p.n_j) return;

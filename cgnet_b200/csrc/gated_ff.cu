@@ -360,21 +360,22 @@ __global__ void __launch_bounds__(256) ff_dgu_kernel(FfArgs a, void* dg, void* d
     }
 }
 
-// Half precision's dg and du may leave its range, on either side, where the gradients behind them do not.  So each is scaled by a
-// power of two, which costs no digits, and the products' epilogue takes it back: row by row for dx (a large row costs no other one
-// its small values), and a second copy unit by unit for the weights' gradients, whose sums run down the rows.  The factors come
-// from the largest finite values, found first: 8192 x 5120 99 us, and 122 for both copies (683 MB, 5.6 TB/s), against 83 unscaled.
-// A block has `w` lanes of eight units side by side and `steps` rows for each of the others: eight where the rows keep the SMs busy, so that
-// few blocks meet at one unit's largest value, fewer where they do not (256 x 1024: 17 us a kernel with eight).
-constexpr int kFfRangeSteps = 8;
+// Half precision's dg and du may leave its range, on either side, where the gradients behind them do not.  The largest finite value of
+// each row and each hidden unit is found as they are written.  Where one is out of range (fits_half), its tile of 128 rows, for
+// dx, or of 128 units, for the weights' gradients, is written once more, each row or unit scaled by a power of two of its own,
+// which costs no digits; the products read that copy instead and their epilogue scales back.  (By rows and by units, because a factor
+// may not change along a contraction, and so that a large row or unit costs no other one its small values.)
 struct FfRange {
-    uint32_t *rows, *cols;      // largest |dg|, |du| of a row, [rows]; of a unit, [2][pitch]; bits of a float32; null where not wanted
+    uint32_t *rows, *cols;              // largest |dg|, |du| of a row, [rows]; of a unit, [2][pitch]; bits of a float32; null where not wanted
+    uint32_t *row_flag, *col_flag;      // per tile, [row tiles], [2][unit tiles]
     int64_t pitch;
-    int w, steps;               // w: a power of two up to 32
-    __half *dg, *du;            // [rows][pitch], by rows
-    __half *dg_cols, *du_cols;  // by units
+    int w, steps;                       // lanes side by side (a power of two from 2 to 32), rows of a thread in the first kernel
+    __half *dg, *du;                    // [rows][pitch]
+    __half *dg_rows, *du_rows, *dg_cols, *du_cols;
 };
-// dg and du of eight units, in place of g and u
+constexpr int kFfRangeSteps = 8;
+
+// dg and du of eight units of a row
 template <int ACT>
 __device__ __forceinline__ void turn_gradients(float (&g)[8], float (&u)[8], const float (&dh)[8]) {
 #pragma unroll
@@ -384,61 +385,44 @@ __device__ __forceinline__ void turn_gradients(float (&g)[8], float (&u)[8], con
         u[i] = dh[i] * f.x;
     }
 }
-template <bool WRITE>
+__device__ __forceinline__ void load_gradients(const FfArgs& a, int64_t r, int64_t e0, float (&dg)[8], float (&du)[8]) {
+    float dh[8];
+    load_params<float, 8>(a.gu + r * a.gu_pitch, e0, a.hidden, dg);
+    load_params<float, 8>(a.gu + (a.rows + r) * a.gu_pitch, e0, a.hidden, du);
+    load_params<__half, 8>((const __half*)a.dh + r * a.dh_stride, e0, a.hidden, dh);
+    if (a.act == CGB200_ACT_RELU) turn_gradients<CGB200_ACT_RELU>(dg, du, dh);
+    else if (a.act == CGB200_ACT_SILU) turn_gradients<CGB200_ACT_SILU>(dg, du, dh);
+    else turn_gradients<CGB200_ACT_GELU>(dg, du, dh);
+}
+// A block has `w` lanes of eight units side by side and `steps` rows for each of the others: eight where the rows keep the SMs busy, so that
+// few blocks meet at one unit's largest value, fewer where they do not (256 x 1024: 17 us with eight, 6 with one).
+// 8192 x 5120 112 us (551 MB, 4.9 TB/s; 83 without the maxima); the kernel behind it 5 where nothing is out of range, 122 where everything is.
 __global__ void __launch_bounds__(256, 4) ff_range_kernel(FfArgs a, FfRange q) {
-    __shared__ uint32_t most[WRITE ? 1 : 8 * 32 * 16];
+    __shared__ uint32_t most[8 * 16 * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = q.w, at = (int)threadIdx.x & (w - 1);
     const int64_t e0 = ((int64_t)blockIdx.y * w + at) * 8, row0 = (int64_t)blockIdx.x * (256 / w) * q.steps + threadIdx.x / w;
-    const float* g = a.gu;
-    const float* u = a.gu + a.rows * a.gu_pitch;
     uint32_t top[16];           // of this thread's units
 #pragma unroll
     for (int i = 0; i < 16; ++i) top[i] = 0;
-    float sg[8], su[8];
-    if (WRITE && q.cols != nullptr && e0 < q.pitch) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sg[i] = scale_of(q.cols[e0 + i]), su[i] = scale_of(q.cols[q.pitch + e0 + i]);
-    }
 #pragma unroll 2
     for (int s = 0; s < q.steps; ++s) {
         const int64_t r = row0 + (int64_t)s * (256 / w);
-        const bool in = r < a.rows && e0 < q.pitch;
         uint32_t big = 0;
-        if (in) {
-            float gv[8], uv[8], dv[8];
-            load_params<float, 8>(g + r * a.gu_pitch, e0, a.hidden, gv);
-            load_params<float, 8>(u + r * a.gu_pitch, e0, a.hidden, uv);
-            load_params<__half, 8>((const __half*)a.dh + r * a.dh_stride, e0, a.hidden, dv);
-            if (a.act == CGB200_ACT_RELU) turn_gradients<CGB200_ACT_RELU>(gv, uv, dv);
-            else if (a.act == CGB200_ACT_SILU) turn_gradients<CGB200_ACT_SILU>(gv, uv, dv);
-            else turn_gradients<CGB200_ACT_GELU>(gv, uv, dv);
-            if (WRITE) {
-                float x[8], y[8];
-                if (q.rows != nullptr) {
-                    const float sr = scale_of(q.rows[r]);
+        if (r < a.rows && e0 < q.pitch) {
+            float dg[8], du[8];
+            load_gradients(a, r, e0, dg, du);
+            *reinterpret_cast<uint4*>(q.dg + r * q.pitch + e0) = pack16(dg, (const __half*)nullptr);
+            *reinterpret_cast<uint4*>(q.du + r * q.pitch + e0) = pack16(du, (const __half*)nullptr);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = gv[i] * sr, y[i] = uv[i] * sr;
-                    *reinterpret_cast<uint4*>(q.dg + r * q.pitch + e0) = pack16(x, (const __half*)nullptr);
-                    *reinterpret_cast<uint4*>(q.du + r * q.pitch + e0) = pack16(y, (const __half*)nullptr);
-                }
-                if (q.cols != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = gv[i] * sg[i], y[i] = uv[i] * su[i];
-                    *reinterpret_cast<uint4*>(q.dg_cols + r * q.pitch + e0) = pack16(x, (const __half*)nullptr);
-                    *reinterpret_cast<uint4*>(q.du_cols + r * q.pitch + e0) = pack16(y, (const __half*)nullptr);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    // an infinity or NaN spoils its own row and unit, but is no measure for them
-                    uint32_t bg = __float_as_uint(fabsf(gv[i])), bu = __float_as_uint(fabsf(uv[i]));
-                    bg = bg < 0x7f800000u ? bg : 0u, bu = bu < 0x7f800000u ? bu : 0u;
-                    top[i] = max(top[i], bg), top[8 + i] = max(top[8 + i], bu);
-                    big = max(big, max(bg, bu));
-                }
+            for (int i = 0; i < 8; ++i) {
+                // an infinity or NaN spoils its own row and unit, but is no measure for them
+                uint32_t bg = __float_as_uint(fabsf(dg[i])), bu = __float_as_uint(fabsf(du[i]));
+                bg = bg < 0x7f800000u ? bg : 0u, bu = bu < 0x7f800000u ? bu : 0u;
+                top[i] = max(top[i], bg), top[8 + i] = max(top[8 + i], bu);
+                big = max(big, max(bg, bu));
             }
         }
-        if (!WRITE && q.rows != nullptr) {
+        if (q.rows != nullptr) {
             if (w == 32) {
                 big = __reduce_max_sync(0xffffffffu, big);
             } else {
@@ -447,7 +431,7 @@ __global__ void __launch_bounds__(256, 4) ff_range_kernel(FfArgs a, FfRange q) {
             if (at == 0 && r < a.rows && big != 0) atomicMax(q.rows + r, big);
         }
     }
-    if (WRITE || q.cols == nullptr) return;
+    if (q.cols == nullptr) return;
     // the rows of a warp, then its block's warps
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -462,6 +446,46 @@ __global__ void __launch_bounds__(256, 4) ff_range_kernel(FfArgs a, FfRange q) {
         for (int k = 0; k < 8; ++k) m = max(m, most[(k * 16 + side * 8 + j) * 32 + unit]);
         const int64_t col = ((int64_t)blockIdx.y * w + unit) * 8 + j;
         if (m != 0 && col < q.pitch) atomicMax(q.cols + side * q.pitch + col, m);
+    }
+}
+// The scaled copies of the tiles that need one, and the flags of all: a block has 128 rows and 8 w units, which are one or two tiles.
+__global__ void __launch_bounds__(256) ff_rescale_kernel(FfArgs a, FfRange q) {
+    __shared__ uint32_t flags;        // 1: the rows; 2, 4: the first and second tile of units in dg; 8, 16: in du
+    const int w = q.w, at = (int)threadIdx.x & (w - 1), t = (int)threadIdx.x;
+    const int64_t r0 = (int64_t)blockIdx.x * kFfBM, u0 = (int64_t)blockIdx.y * w * 8, e0 = u0 + at * 8;
+    if (t == 0) flags = 0;
+    __syncthreads();
+    uint32_t mine = 0;
+    if (q.rows != nullptr && t < kFfBM && r0 + t < a.rows && !fits_half(q.rows[r0 + t])) mine = 1;
+    if (q.cols != nullptr && t < w * 8 && u0 + t < q.pitch) {
+        if (!fits_half(q.cols[u0 + t])) mine |= 2u << (t / kFfBM);
+        if (!fits_half(q.cols[q.pitch + u0 + t])) mine |= 8u << (t / kFfBM);
+    }
+    mine = __reduce_or_sync(0xffffffffu, mine);
+    if ((t & 31) == 0 && mine != 0) atomicOr(&flags, mine);
+    __syncthreads();
+    mine = flags;
+    if (t == 0 && blockIdx.y == 0 && q.rows != nullptr) q.row_flag[blockIdx.x] = mine & 1;
+    const int64_t tiles = (q.pitch + kFfBM - 1) / kFfBM, tile = u0 / kFfBM + t / 2;
+    if (t < 4 && blockIdx.x == 0 && q.cols != nullptr && tile < tiles) q.col_flag[t % 2 * tiles + tile] = mine >> (1 + t % 2 * 2 + t / 2) & 1;
+    if (mine == 0 || e0 >= q.pitch) return;
+    const bool by_rows = mine & 1, dg_cols = mine >> (1 + at * 8 / kFfBM) & 1, du_cols = mine >> (3 + at * 8 / kFfBM) & 1;
+    if (!by_rows && !dg_cols && !du_cols) return;
+    float sg[8], su[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sg[i] = dg_cols ? scale_of(q.cols[e0 + i]) : 1.f, su[i] = du_cols ? scale_of(q.cols[q.pitch + e0 + i]) : 1.f;
+    for (int64_t r = r0 + t / w; r < min(a.rows, r0 + kFfBM); r += 256 / w) {
+        float dg[8], du[8], x[8];
+        load_gradients(a, r, e0, dg, du);
+        const float sr = by_rows ? scale_of(q.rows[r]) : 1.f;
+        auto leave = [&](__half* out, const float (&v)[8], const float* each) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = v[i] * (each != nullptr ? each[i] : sr);
+            *reinterpret_cast<uint4*>(out + r * q.pitch + e0) = pack16(x, (const __half*)nullptr);
+        };
+        if (by_rows) leave(q.dg_rows, dg, nullptr), leave(q.du_rows, du, nullptr);
+        if (dg_cols) leave(q.dg_cols, dg, sg);
+        if (du_cols) leave(q.du_cols, du, su);
     }
 }
 
@@ -552,7 +576,8 @@ struct FfPlan {
     int planes, bn;
     bool pack[3];                         // x, Wg, Wu
     int64_t pitch_d, pitch_h;             // of packed operands (dim columns) and of dg, du (hidden columns)
-    int64_t off_pack[3], off_dg, off_du, off_dg_cols, off_du_cols, off_amax, off_part[2], bytes;
+    int64_t off_pack[3], off_dg, off_du, off_rows, off_cols, off_amax, off_part[2], bytes;      // off_rows, off_cols: scaled copies of dg, du
+    int64_t d_bytes;                      // of dg or du
     int n_problems;
     FfProblem problem[2];
 };
@@ -582,12 +607,12 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
         q.off_pack[i] = at;
         if (q.pack[i]) at += up(q.planes * rows[i] * q.pitch_d * 2, 256);
     }
-    const bool scaled = !fwd && dtype == CGB200_F16;
-    const int64_t d_bytes = up(q.planes * a.rows * q.pitch_h * 2, 256);
-    if (!fwd && (!scaled || (grads & 1))) q.off_dg = at, q.off_du = at + d_bytes, at += 2 * d_bytes;
-    if (scaled) {
-        if (grads & 6) q.off_dg_cols = at, q.off_du_cols = at + d_bytes, at += 2 * d_bytes;
-        q.off_amax = at, at += up((a.rows + 2 * q.pitch_h) * 4, 256);
+    q.d_bytes = up(q.planes * a.rows * q.pitch_h * 2, 256);
+    if (!fwd) q.off_dg = at, q.off_du = at + q.d_bytes, at += 2 * q.d_bytes;
+    if (!fwd && dtype == CGB200_F16) {
+        if (grads & 1) q.off_rows = at, at += 2 * q.d_bytes;
+        if (grads & 6) q.off_cols = at, at += 2 * q.d_bytes;
+        q.off_amax = at, at += up((a.rows + 2 * q.pitch_h + (a.rows + kFfBM - 1) / kFfBM + 2 * ((q.pitch_h + kFfBM - 1) / kFfBM)) * 4, 256);
     }
     const int64_t ti = (a.rows + kFfBM - 1) / kFfBM;
     const int hk = (a.hidden + kFfBK - 1) / kFfBK, dk = (a.dim + kFfBK - 1) / kFfBK;
@@ -619,7 +644,7 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     }
     if (grads & 1) {
         FfProblem& p = q.problem[q.n_problems++];
-        p.a_map[0] = kMapDg, p.a_map[1] = kMapDu, p.b_map[0] = kMapWg, p.b_map[1] = kMapWu, p.b_mn = 1;
+        p.a_map[0] = kMapDg, p.a_map[1] = kMapDu, p.a_scaled[0] = kMapDgRows, p.a_scaled[1] = kMapDuRows, p.b_map[0] = kMapWg, p.b_map[1] = kMapWu, p.b_mn = 1;
         p.sources = 2, p.kblk = hk, p.sets = 1;
         p.tiles_i = (int)ti, p.tiles_j = (a.dim + q.bn - 1) / q.bn;
         p.n_i = a.rows, p.n_j = a.dim;
@@ -627,8 +652,8 @@ static FfPlan ff_plan(const FfArgs& a, int dtype, int grads) {
     }
     if (w_sets > 0) {
         FfProblem& p = q.problem[q.n_problems++];
-        const int dg = scaled ? kMapDgCols : kMapDg, du = scaled ? kMapDuCols : kMapDu;
-        p.a_map[0] = (grads & 2) ? dg : du, p.a_map[1] = du, p.b_map[0] = kMapX, p.a_mn = p.b_mn = 1;
+        p.a_map[0] = (grads & 2) ? kMapDg : kMapDu, p.a_map[1] = kMapDu, p.b_map[0] = kMapX, p.a_mn = p.b_mn = 1;
+        p.a_scaled[0] = (grads & 2) ? kMapDgCols : kMapDuCols, p.a_scaled[1] = kMapDuCols;
         p.sources = 1, p.kblk = mk, p.sets = w_sets;
         p.tiles_i = th, p.tiles_j = (a.dim + q.bn - 1) / q.bn;
         p.n_i = a.hidden, p.n_j = a.dim;
@@ -750,46 +775,44 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
     FfGemmArgs g{};
     bool ok = true;
     constexpr bool half = std::is_same<T, __half>::value;
-    uint32_t *row_max = nullptr, *col_max = nullptr;
+    FfRange range{};
     for (int i = 0; i < 3; ++i) {
         const bool used = fwd || (i == 0 ? (grads & 6) != 0 : (grads & 1) != 0);
         if (used) ok = ok && ff_map(&g.map[kMapX + i], enc, src[i], stride[i], rows[i], a.dim, PLANES, half);
     }
     if (!fwd) {
-        void *dg = ws + q.off_dg, *du = ws + q.off_du, *dg_cols = ws + q.off_dg_cols, *du_cols = ws + q.off_du_cols;
-        if constexpr (std::is_same<T, __half>::value) {
-            FfRange r{};
-            row_max = (uint32_t*)(ws + q.off_amax), col_max = row_max + a.rows;
-            if (grads & 1) r.rows = row_max, r.dg = (__half*)dg, r.du = (__half*)du;
-            if (grads & 6) r.cols = col_max, r.dg_cols = (__half*)dg_cols, r.du_cols = (__half*)du_cols;
-            r.pitch = q.pitch_h, r.w = 1;
-            while (r.w < 32 && r.w < q.pitch_h / 8) r.w *= 2;
-            CGB_CUDA(cudaMemsetAsync(row_max, 0, (a.rows + 2 * q.pitch_h) * 4, st));
-            const int64_t side = (q.pitch_h / 8 + r.w - 1) / r.w, one = (a.rows * r.w + 255) / 256;      // blocks; of one row a thread
-            r.steps = (int)std::max<int64_t>(1, std::min<int64_t>(kFfRangeSteps, one * side / (kNumSM * 8)));
-            const dim3 grid((unsigned)((one + r.steps - 1) / r.steps), (unsigned)side);
+        void *dg = ws + q.off_dg, *du = ws + q.off_du;
+        if constexpr (half) {
+            range.pitch = q.pitch_h, range.w = 2;
+            range.dg = (__half*)dg, range.du = (__half*)du;
+            uint32_t* words = (uint32_t*)(ws + q.off_amax);
+            if (grads & 1) range.rows = words, range.dg_rows = (__half*)(ws + q.off_rows), range.du_rows = (__half*)(ws + q.off_rows + q.d_bytes);
+            if (grads & 6) range.cols = words + a.rows, range.dg_cols = (__half*)(ws + q.off_cols), range.du_cols = (__half*)(ws + q.off_cols + q.d_bytes);
+            words += a.rows + 2 * q.pitch_h;
+            range.row_flag = words, range.col_flag = words + (a.rows + kFfBM - 1) / kFfBM;
+            while (range.w < 32 && range.w < q.pitch_h / 8) range.w *= 2;
+            const int64_t side = (q.pitch_h / 8 + range.w - 1) / range.w, one = (a.rows * range.w + 255) / 256;      // blocks; of one row a thread
+            range.steps = (int)std::max<int64_t>(1, std::min<int64_t>(kFfRangeSteps, one * side / (kNumSM * 8)));
+            CGB_CUDA(cudaMemsetAsync(ws + q.off_amax, 0, (a.rows + 2 * q.pitch_h) * 4, st));
             launch_begin(kid, st);
-            ff_range_kernel<false><<<grid, 256, 0, st>>>(a, r);
+            ff_range_kernel<<<dim3((unsigned)((one + range.steps - 1) / range.steps), (unsigned)side), 256, 0, st>>>(a, range);
             launch_end(kid, st);
             CGB_CUDA(cudaGetLastError());
             launch_begin(kid, st);
-            ff_range_kernel<true><<<grid, 256, 0, st>>>(a, r);
+            ff_rescale_kernel<<<dim3((unsigned)((a.rows + kFfBM - 1) / kFfBM), (unsigned)side), 256, 0, st>>>(a, range);
             launch_end(kid, st);
             CGB_CUDA(cudaGetLastError());
+            void* copies[4] = {range.dg_rows, range.du_rows, range.dg_cols, range.du_cols};
+            for (int i = 0; i < 4; ++i)
+                if (copies[i] != nullptr) ok = ok && ff_map(&g.map[kMapDgRows + i], enc, copies[i], q.pitch_h, a.rows, a.hidden, PLANES, half);
         } else {
             launch_begin(kid, st);
             ff_dgu_kernel<T><<<(unsigned)std::min<int64_t>((a.rows * q.pitch_h / 8 + 255) / 256, kNumSM * 16), 256, 0, st>>>(a, dg, du, q.pitch_h);
             launch_end(kid, st);
             CGB_CUDA(cudaGetLastError());
         }
-        if (!half || (grads & 1)) {
-            ok = ok && ff_map(&g.map[kMapDg], enc, dg, q.pitch_h, a.rows, a.hidden, PLANES, half);
-            ok = ok && ff_map(&g.map[kMapDu], enc, du, q.pitch_h, a.rows, a.hidden, PLANES, half);
-        }
-        if (half && (grads & 6)) {
-            ok = ok && ff_map(&g.map[kMapDgCols], enc, dg_cols, q.pitch_h, a.rows, a.hidden, PLANES, half);
-            ok = ok && ff_map(&g.map[kMapDuCols], enc, du_cols, q.pitch_h, a.rows, a.hidden, PLANES, half);
-        }
+        ok = ok && ff_map(&g.map[kMapDg], enc, dg, q.pitch_h, a.rows, a.hidden, PLANES, half);
+        ok = ok && ff_map(&g.map[kMapDu], enc, du, q.pitch_h, a.rows, a.hidden, PLANES, half);
     }
     if (!ok) {
         set_error("gated feed-forward: an operand's layout was refused by the driver");
@@ -815,7 +838,11 @@ static int ff_tensor(const FfArgs& a, const FfPlan& q, int grads, char* ws, cuda
             }
             continue;
         }
-        for (int k = 0; half && k < p.sets; ++k) p.amax[k] = !p.a_mn ? row_max : col_max + (p.a_map[k] == kMapDuCols ? q.pitch_h : 0);
+        for (int k = 0; half && k < p.sets; ++k) {
+            const bool du = p.a_map[k] == kMapDu;
+            p.amax[k] = !p.a_mn ? range.rows : range.cols + (du ? q.pitch_h : 0);
+            p.flag[k] = !p.a_mn ? range.row_flag : range.col_flag + (du ? (q.pitch_h + kFfBM - 1) / kFfBM : 0);
+        }
         for (int k = 0; k < p.sets; ++k)
             if (p.splits == 1 && p.out[k] != nullptr && at16(p.out[k]) && a.dim % Chunk<T>::N == 0) {
                 const int m = p.a_mn ? kMapOutWg + k : kMapOut;

@@ -9,7 +9,7 @@ The reference leaves this part to torch (BatchNorm1d, Linear + ReLU, Linear, Log
 the last axis of a tensor of any leading shape, in float32, bfloat16 or float16; sums, norms and softmax statistics are held
 in float32 or more whatever that type, and each result is rounded once.  The gated block's backward rounds one thing more: on the
 tensor cores, the gradients of its two projections take the type of x before they are multiplied (a 16-bit gradient's error is
-1.4 times one rounding's; in float16 they are scaled by powers of two, so that none leaves that type's range).  All arithmetic happens in libcgnet_b200.so on the
+1.4 times one rounding's; in float16 those that would leave that type's range are scaled by powers of two).  All arithmetic happens in libcgnet_b200.so on the
 current stream; the checks of the arguments, the allocations and the autograd nodes are C++ too (``_torch_head.so``,
 ``csrc/torch_head.cpp``).  There is no CPU path and no fallback: a missing library or a bad argument raises RuntimeError before
 anything is launched.  Every operator is differentiable once (in reverse mode), can be captured in a CUDA graph, and gives the same bits from run

@@ -314,8 +314,8 @@ int cgb200_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64
  * dx, 2 for dw_gate and 4 for dw_up, as the call asks for them; the operands' addresses and strides decide whether they have to
  * be copied), 256-byte aligned, contents undefined; one workspace serves one call at a time.
  * On the tensor cores the backward rounds the gradients of the two projections to `dtype` before it multiplies them; in
- * CGB200_F16 they are scaled by a power of two per row (dx) and per hidden unit (dw_gate, dw_up) and the products scaled back, so
- * that values beyond that type's range on either side are not lost.
+ * CGB200_F16 those that would leave that type's range, on either side, are scaled by a power of two per row (for dx) or per hidden
+ * unit (for dw_gate and dw_up) and the products scaled back.
  * A tensor-core block that gives up on a bounded wait fills what it still owes with NaN.
  * Small products run on the CUDA cores, others on the tensor cores (float32 in three bfloat16 parts, accurate to float32).  A row of
  * x that is not finite spoils that row of h and dx, a row of w_gate or w_up that is not finite that column of h.  In CGB200_F32 a
