@@ -396,7 +396,7 @@ __device__ __forceinline__ void load_gradients(const FfArgs& a, int64_t r, int64
 }
 // A block has `w` lanes of eight units side by side and `steps` rows for each of the others: eight where the rows keep the SMs busy, so that
 // few blocks meet at one unit's largest value, fewer where they do not (256 x 1024: 17 us with eight, 6 with one).
-// 8192 x 5120 112 us (551 MB, 4.9 TB/s; 83 without the maxima); the kernel behind it 5 where nothing is out of range, 122 where everything is.
+// 8192 x 5120 112 us (551 MB, 4.9 TB/s; 83 without the maxima); the kernel behind it 5 where nothing is out of range, 147 where everything is.
 __global__ void __launch_bounds__(256, 4) ff_range_kernel(FfArgs a, FfRange q) {
     __shared__ uint32_t most[8 * 16 * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = q.w, at = (int)threadIdx.x & (w - 1);
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(256) ff_join_kernel(FfArgs a, const float* g_p
 // The tensor cores are used from this length of the longest contraction on (forward: dim; backward: rows or 2 hidden), or from this
 // much work (rows x dim x hidden).  CUDA cores / tensor cores, us, launches of a graph: 16 bits, forward 16 x 64 -> 64 5.0 / 6.3,
 // 16 x 128 -> 256 6.8 / 6.4, 10 x 976 -> 104 36 / 8.0; backward 7.0 / 7.2, 19 / 8.7, 11 / 7.8.  float32 (three planes, a copy in
-// front), forward 100 x 256 -> 256 8.9 / 12.5, 100 x 512 -> 256 15.1 / 14.4, 32 x 640 -> 128 17.5 / 15.2; backward 16 / 19, 1000 x 48 -> 48 28 / 21.
+// front), forward 100 x 256 -> 256 8.8 / 12.1, 100 x 512 -> 256 14.6 / 13.5, 32 x 640 -> 128 17.1 / 14.5; backward 16 / 19, 1000 x 48 -> 48 28 / 21.
 struct FfLimits {
     int forward, backward;
     int64_t work;
@@ -567,7 +567,7 @@ constexpr int kFfOutputStages = 8;
 static int ff_longest(int dtype) { return dtype == CGB200_F32 ? 1 << 30 : dtype == CGB200_BF16 ? 512 : 256; }
 // A forward whose tiles keep at most half of the SMs busy is split along dim from this many stages on.  Whole / split, us, launches of a
 // graph: bf16 16 x 1024 -> 1000 9.1 / 8.0, 16 x 4096 -> 1000 19.3 / 9.7, 500 x 2048 -> 1000 13.3 / 13.1, 156 x 3330 -> 342 30.8 / 15.7;
-// float32 300 x 640 -> 500 20.1 / 16.6, 156 x 3330 -> 342 78.7 / 22.6.
+// float32 300 x 640 -> 500 19.9 / 16.4, 156 x 3330 -> 342 78.8 / 22.5.
 static int ff_split_stages(int dtype) { return dtype == CGB200_F32 ? 8 : 16; }
 
 struct FfPlan {
