@@ -206,10 +206,11 @@ __device__ __forceinline__ float weight_of(const ScoreArgs& a, float t, float tm
 template <typename T>
 __device__ __forceinline__ float distill_loss(const ScoreArgs& a, int64_t row, const T* zr, const Stat& st, const Entry& first, int t, int G,
                                               double* buf, bool whole_block, float2& teacher) {
-    float mx = first.t, some = first.t != -INFINITY ? 1.f : 0.f;      // a NaN counts as an entry
+    float mx = first.t, some = first.t != -INFINITY || first.bad ? 1.f : 0.f;      // a NaN counts, and a class beyond the last
     for (int k = t + G; k < a.n_t; k += G) {
-        const float v = a.t_ids[row * a.n_t + k] < 0 ? -INFINITY : load_score(a.t_scores, a.t_dtype, row * a.n_t + k);
-        if (v != -INFINITY) some = 1.f;
+        const int64_t id = a.t_ids[row * a.n_t + k];
+        const float v = id < 0 ? -INFINITY : load_score(a.t_scores, a.t_dtype, row * a.n_t + k);
+        if (v != -INFINITY || id >= a.classes) some = 1.f;
         mx = fmaxf(mx, v);
     }
     const bool any = row_max_f(some, buf, whole_block) > 0.f;       // the same in all threads of the row

@@ -225,3 +225,28 @@ def test_long_sums_of_one_sign(dtype, terms):
     for got in gradients(x, w, w, dh)[1:]:
         off = abs(float(((got.double() - want) / want).mean()))
         assert off <= 2 * one + (rows / terms + 8) * U + 5 * half(dtype) / 3 ** 0.5 / 64, off / U
+
+
+def test_half_precision_backward_in_a_captured_graph():
+    """One graph, replayed with gradients inside, above and below the range: which tiles are scaled is decided on the GPU."""
+    import cgnet_b200 as cg
+    g = gen(3)
+    x, wg, wu, dh = (t.half() for t in (randn(g, 300, 104), randn(g, 264, 104) / 10, randn(g, 264, 104) / 10, randn(g, 300, 264)))
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+
+    def step():
+        return torch.autograd.grad(cg.gated_feed_forward(*leaves, activation="gelu"), leaves, dh)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for size in (1.0, 1e-5, 1e4, 1.0):
+        new = size * randn(g, 300, 264)
+        new[130:] = new[130:].clamp(-1, 1)
+        dh.copy_(new)
+        graph.replay()
+        assert all(torch.equal(p.nan_to_num(7.0), q.nan_to_num(7.0)) for p, q in zip(grads, step())), size

@@ -51,3 +51,18 @@ def test_entropy_gradient_of_a_row_whose_target_is_beyond_the_last_class(classes
     assert torch.isfinite(want).all() and torch.equal(dz, want)
     (dz,) = torch.autograd.grad(out.log_prob, z, g_ent)
     assert torch.isnan(dz[1:3]).all() and torch.isfinite(dz[[0, 3]]).all()
+
+
+@pytest.mark.parametrize("entries", [1, 40, 300])
+@pytest.mark.parametrize("classes", [20, 3000])
+def test_a_class_beyond_the_last_counts_whatever_its_score(classes, entries):
+    """Scores of -inf have weight 0 and a row of nothing else loss 0, but not where a class does not exist."""
+    import cgnet_b200 as cg
+    g = gen(classes + entries)
+    z = randn(g, 3, classes).requires_grad_()
+    ids = torch.randint(0, classes, (3, entries), generator=g, device=z.device)
+    ids[1, entries - 1] = classes
+    loss = cg.distillation_loss(z, ids, torch.full((3, entries), float("-inf"), device=z.device))
+    (dz,) = torch.autograd.grad(loss.sum(), z)
+    assert torch.isnan(loss[1]) and torch.isnan(dz[1]).all()
+    assert not loss[[0, 2]].any() and not dz[[0, 2]].any()
