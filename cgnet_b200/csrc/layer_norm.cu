@@ -5,7 +5,8 @@
 //   dw = sum over rows of dy * xh,     db = sum over rows of dy
 //
 // Everything is held in float32 between the loads and the one rounding of each result.  The variance is taken over centred
-// values that stay in registers (not as a difference of moments), so a large common offset of a row costs no digits.
+// values that stay in registers (not as a difference of moments), so a large common offset of a row costs it no digits; the mean's own
+// rounding, a few units of 2^-24 of it, stays in y.
 #include <cooperative_groups.h>
 
 #include <algorithm>
