@@ -197,9 +197,12 @@ __device__ __forceinline__ Entry entry_of(const ScoreArgs& a, int64_t row, const
     if (!e.bad) e.id = (int)id, e.z = to_f32(zr[id]);
     return e;
 }
-// Weight of an entry before the division by the sum of all: exp((t - tmax) / T).
+// Weight of an entry before the division by the sum of all: exp((t - tmax) / T).  What the exponent loses when it is rounded to float32,
+// up to |exponent| 2^-24, is made good to first order.
 __device__ __forceinline__ float weight_of(const ScoreArgs& a, float t, float tmax) {
-    return expf((float)(((double)t - (double)tmax) * a.inv_temperature));
+    const double x = ((double)t - (double)tmax) * a.inv_temperature;
+    const float hi = (float)x, w = expf(hi);
+    return hi < -200.f ? w : fmaf(w, (float)(x - (double)hi), w);
 }
 // Loss of a row from its statistics; `first` is this thread's first entry, fetched while the row was read.  Leaves what the
 // backward needs of the teacher, (tmax, 1 / sum of weights), 1 / sum = 0 for a row without entries.

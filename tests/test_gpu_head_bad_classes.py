@@ -1,4 +1,4 @@
-"""Classes beyond the last and NaN scores: which gradients they spoil, and which they leave alone."""
+"""Classes beyond the last and NaN scores: which gradients they spoil, and which they leave alone.  Scores far below the best."""
 import pytest
 import torch
 
@@ -66,3 +66,14 @@ def test_a_class_beyond_the_last_counts_whatever_its_score(classes, entries):
     (dz,) = torch.autograd.grad(loss.sum(), z)
     assert torch.isnan(loss[1]) and torch.isnan(dz[1]).all()
     assert not loss[[0, 2]].any() and not dz[[0, 2]].any()
+
+
+@pytest.mark.parametrize("classes, entries", [(50, 12), (700, 100), (3000, 500), (90000, 300)])
+def test_distillation_of_scores_far_below_the_best(classes, entries):
+    """Weights down to e^-80: each is off by a few roundings of its own, not by its exponent's."""
+    g = gen(classes)
+    z = 2 * randn(g, 40, classes)
+    ids = torch.stack([torch.randperm(classes, generator=g, device=z.device)[:entries] for _ in range(40)])
+    scores = -40 * torch.rand(40, entries, generator=g, device=z.device)
+    for temp in (0.5, 1.0, 3.0):
+        check_distill(z, ids, scores, temp, 1 + randn(g, 40).abs())
